@@ -412,6 +412,36 @@ enum { TKV_PREFILL_DEFAULT = 0,
        TKV_PREFILL_TWO_TILES = 2    /* two query tiles per CTA, their softmax groups out of step; without either flag the library
                                        chooses (two from 1 536 new tokens on) */ };
 int32_t tkv_prefill_attn_enqueue(const TkvPool* pool, const TkvPrefillAttn* args, void* stream);
+/* Decode attention that also accumulates the softmax weight every cached token received, the measure by which the eviction
+ * calls below cut a cache.  For sequence s and kv head h, with w the weights of the n_q_heads / n_kv_heads query heads that read h:
+ *     out = sum over t < kv_lens[s] of w[t] * v[t]           scores[s][h][t] = decay * scores[s][h][t] + sum over the query heads of w[t]
+ * for t < kv_lens[s]; scores at and behind kv_lens[s] are left alone, so a row that grows is zeroed by its owner (decay 0 does not
+ * read the old value: the last step's weights alone).  A sequence of length 0 gets zeros in out.  No counterpart in the reference.
+ * F16 or E4M3 pool (per-block scales applied), 16-token blocks, head_dim 64 or 128, 1..8 query heads per kv head.  With F16 q a
+ * score is exact but for F32 accumulation and out is rounded to F16 once; F32 q is taken as two F16 terms (2^-22), so its elements
+ * have to lie inside F16's range.  kv_lens is device memory read when the kernel runs; max_kv_len bounds it.  Calls that share
+ * scratch have to be ordered (one stream, or events), two graphs that were captured with the same scratch included.             */
+typedef struct TkvScoredAttn {
+    uint32_t n_seqs, n_q_heads, table_stride, layer, max_kv_len;
+    uint32_t score_stride;        /* floats from one kv head's row of scores to the next; at least max_kv_len      */
+    float sm_scale;               /* usually 1 / sqrt(head_dim)                                                    */
+    float decay;                  /* in [0, 1]; 1 accumulates, 0 overwrites                                        */
+    int32_t q_dtype;              /* TKV_DTYPE_F16 or TKV_DTYPE_F32, of q and out                                  */
+    uint32_t reserved;
+    uint64_t q;                   /* [n_seqs][n_q_heads][head_dim]                                                 */
+    uint64_t out;                 /* same shape and type                                                           */
+    uint64_t tables;              /* u32 [n_seqs][table_stride] block ids                                          */
+    uint64_t kv_lens;             /* u32 [n_seqs]                                                                  */
+    uint64_t scores;              /* f32 [n_seqs][n_kv_heads][score_stride] of this layer                          */
+    uint64_t scratch;             /* tkv_scored_attn_scratch_bytes(...) bytes of device memory, 256-byte aligned   */
+    uint64_t scratch_bytes;
+    uint64_t status;              /* 0, or a device u32 (zero it before the launch): TKV_ERR_INVALID_CONFIG if kv_lens held a value
+                                     above max_kv_len (clamped to it) or a table entry named a block outside the pool (never read);
+                                     out and scores are then not valid                                             */
+} TkvScoredAttn;
+uint64_t tkv_scored_attn_scratch_bytes(uint32_t n_seqs, uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t max_kv_len);
+int32_t tkv_scored_attn_enqueue(const TkvPool* pool, const TkvScoredAttn* args, void* stream);
+
 /* Device self-check of the tcgen05 path's operand plumbing (tensor-map copy with the 128-byte swizzle,
  * shared-memory and instruction descriptors, tensor-memory reads) on operands of small dyadic values whose
  * products and sums are exact: mismatches[0..3] count wrong accumulators for E4M3 K-major, E4M3 x E5M2

@@ -10,6 +10,7 @@ const SOURCES: &[&str] = &[
     "tkv_attention.cu",
     "tkv_attention_tc.cu",
     "tkv_prefill_tc.cu",
+    "tkv_scored_attn.cu",
     "tkv_prefix_index.cu",
     "tkv_hostobj.cpp",
     "tkv_session.cpp",

@@ -206,6 +206,29 @@ pub struct TkvPrefillAttn {
 
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
+pub struct TkvScoredAttn {
+    pub n_seqs: u32,
+    pub n_q_heads: u32,
+    pub table_stride: u32,
+    pub layer: u32,
+    pub max_kv_len: u32,
+    pub score_stride: u32,
+    pub sm_scale: f32,
+    pub decay: f32,
+    pub q_dtype: i32,
+    pub reserved: u32,
+    pub q: u64,
+    pub out: u64,
+    pub tables: u64,
+    pub kv_lens: u64,
+    pub scores: u64,
+    pub scratch: u64,
+    pub scratch_bytes: u64,
+    pub status: u64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
 pub struct TkvSessionHeader {
     pub position: u64,
     pub seed: u64,
@@ -363,6 +386,8 @@ extern "C" {
     pub fn tkv_decode_attn_scratch_bytes(n_seqs: u32, n_q_heads: u32, head_dim: u32, max_kv_len: u32, split_tokens: u32) -> u64;
     pub fn tkv_decode_attn_enqueue(pool: *const TkvPool, args: *const TkvDecodeAttn, stream: *mut c_void) -> i32;
     pub fn tkv_prefill_attn_enqueue(pool: *const TkvPool, args: *const TkvPrefillAttn, stream: *mut c_void) -> i32;
+    pub fn tkv_scored_attn_scratch_bytes(n_seqs: u32, n_q_heads: u32, n_kv_heads: u32, head_dim: u32, max_kv_len: u32) -> u64;
+    pub fn tkv_scored_attn_enqueue(pool: *const TkvPool, args: *const TkvScoredAttn, stream: *mut c_void) -> i32;
     pub fn tkv_selfcheck_tensor_cores(mismatches: *mut u64) -> i32;
     pub fn tkv_session_wire_size(h: *const TkvSessionHeader) -> usize;
     pub fn tkv_session_pack(h: *const TkvSessionHeader, blocks: *const u32, logits: *const f32, out: *mut u8, cap: usize, written: *mut usize) -> i32;

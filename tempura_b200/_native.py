@@ -63,6 +63,12 @@ class TkvPrefillAttn(C.Structure):
         (n, C.c_uint32) for n in ("flags", "reserved")] + [(n, C.c_uint64) for n in ("q", "out", "table", "status")]
 
 
+class TkvScoredAttn(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("n_seqs", "n_q_heads", "table_stride", "layer", "max_kv_len", "score_stride")] + [
+        ("sm_scale", C.c_float), ("decay", C.c_float), ("q_dtype", C.c_int32), ("reserved", C.c_uint32)] + [
+        (n, C.c_uint64) for n in ("q", "out", "tables", "kv_lens", "scores", "scratch", "scratch_bytes", "status")]
+
+
 class TkvPrefixBatch(C.Structure):
     _fields_ = [(n, C.c_uint32) for n in ("n_seqs", "stride", "page_stride", "reserved")] + [
         (n, C.c_uint64) for n in ("tokens", "lens", "pages", "page_lens")]
@@ -166,6 +172,8 @@ SIGNATURES = {
     "tkv_ipc_close": (_i32, [_u64, _u64]),
     "tkv_decode_attn_scratch_bytes": (_u64, [_u32, _u32, _u32, _u32, _u32]),
     "tkv_decode_attn_enqueue": (_i32, [C.POINTER(TkvPool), C.POINTER(TkvDecodeAttn), _vp]),
+    "tkv_scored_attn_scratch_bytes": (_u64, [_u32, _u32, _u32, _u32, _u32]),
+    "tkv_scored_attn_enqueue": (_i32, [C.POINTER(TkvPool), C.POINTER(TkvScoredAttn), _vp]),
     "tkv_selfcheck_tensor_cores": (_i32, [_u64p]),
     "tkv_session_wire_size": (_sz, [C.POINTER(TkvSessionHeader)]),
     "tkv_session_pack": (_i32, [C.POINTER(TkvSessionHeader), _u32p, C.POINTER(C.c_float), _u8p, _sz, _szp]),

@@ -23,6 +23,18 @@ _TORCH_VIEW = {N.DTYPE_F32: torch.float32, N.DTYPE_F16: torch.float16, N.DTYPE_E
 KvDtype = {"f32": N.DTYPE_F32, "f16": N.DTYPE_F16, "e4m3": N.DTYPE_E4M3}
 
 
+_Q_DTYPE = {torch.float16: N.DTYPE_F16, torch.float32: N.DTYPE_F32}
+
+
+def _check_batch(pool: "Pool", q: torch.Tensor, tables: torch.Tensor, kv_lens: torch.Tensor) -> None:
+    """What the attention handles expect of a batch's tensors."""
+    assert q.is_cuda and q.dtype in _Q_DTYPE and q.is_contiguous() and q.dim() == 3 and q.device.index == pool.device
+    assert q.shape[2] == pool.head_dim
+    assert tables.dtype == torch.int32 and tables.is_contiguous() and tables.dim() == 2 and tables.device == q.device
+    assert kv_lens.dtype == torch.int32 and kv_lens.is_contiguous() and kv_lens.device == q.device
+    assert tables.shape[0] == q.shape[0] == kv_lens.numel()
+
+
 def _u32(x) -> np.ndarray:
     return np.ascontiguousarray(np.asarray(x, dtype=np.uint32))
 
@@ -442,6 +454,44 @@ def decode_attention(pool: Pool, layer: int, q: torch.Tensor, tables: torch.Tens
     if int(attn.status.item()) != 0:
         raise TkvError(int(attn.status.item()), "decode attention: a bounded wait inside the kernel gave up")
     return out
+
+
+class ScoredDecodeAttention:
+    """Decode attention that also accumulates, per cached token and kv head, the softmax weight the token received:
+    ``scores[layer, s, h, t] = decay * scores[layer, s, h, t] + sum of the weights of the query heads that read kv head h``
+    for ``t < kv_lens[s]``; the rest of ``scores`` is left alone (a new token's entry is zeroed by its owner, or ``decay`` is 0).
+    ``q`` is f16 or f32 ``[n_seqs, n_q_heads, head_dim]`` (``out`` has its type), ``tables`` int32 ``[n_seqs, table_stride]``,
+    ``kv_lens`` int32 ``[n_seqs]`` read when the kernel runs, ``scores`` f32 ``[n_layers, n_seqs, n_kv_heads, score_stride]``,
+    all on the pool's device.  Output and workspace are made once, so a decode loop or a graph capture only issues launches;
+    enqueues of one handle share the workspace and have to be ordered."""
+
+    def __init__(self, pool: Pool, q: torch.Tensor, tables: torch.Tensor, kv_lens: torch.Tensor, scores: torch.Tensor, max_kv_len: int,
+                 sm_scale: Optional[float] = None, decay: float = 1.0):
+        _check_batch(pool, q, tables, kv_lens)
+        n_seqs, n_q_heads, head_dim = q.shape
+        assert scores.dtype == torch.float32 and scores.is_contiguous() and scores.device == q.device and scores.dim() == 4
+        assert scores.shape[:3] == (pool.n_layers, n_seqs, pool.n_kv_heads)
+        self.pool, self.q, self.tables, self.kv_lens, self.scores = pool, q, tables, kv_lens, scores
+        self.sm_scale = 1.0 / float(head_dim) ** 0.5 if sm_scale is None else sm_scale
+        self.out = torch.empty_like(q)
+        need = int(lib().tkv_scored_attn_scratch_bytes(n_seqs, n_q_heads, pool.n_kv_heads, head_dim, max_kv_len))
+        self.scratch = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=q.device)
+        self._pool_c = pool.c_struct()
+        self._args = {}
+        row = n_seqs * pool.n_kv_heads * scores.shape[3] * 4
+        self._mk = lambda layer: N.TkvScoredAttn(n_seqs, n_q_heads, tables.shape[1], layer, max_kv_len, scores.shape[3], self.sm_scale, decay,
+                                                 _Q_DTYPE[q.dtype], 0, q.data_ptr(), self.out.data_ptr(), tables.data_ptr(), kv_lens.data_ptr(),
+                                                 scores.data_ptr() + layer * row, self.scratch.data_ptr(), need, self.status.data_ptr())
+
+    def enqueue(self, layer: int, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+        if stream is None:
+            stream = torch.cuda.current_stream(self.pool.device)
+        args = self._args.get(layer)
+        if args is None:
+            args = self._args[layer] = C.byref(self._mk(layer))
+        check(lib().tkv_scored_attn_enqueue(C.byref(self._pool_c), args, C.c_void_p(stream.cuda_stream)))
+        return self.out
 
 
 class PrefixIndex:

@@ -1,0 +1,288 @@
+"""The operators of a cache under a decode loop -- scored decode attention, shared-prefix attention, eviction (select and compact) --
+against plain implementations in 64 bits.
+
+Tolerances.  A weight is 2^(x - M) / L with x accumulated in F32 from exact F16 products: for |x| < 32 in the log2 domain an
+error of 16 roundings (8 k-steps of the MMA in two chains, their sum, the scale, the subtraction, and as many again for the
+truncating adds inside an MMA) of 2^-24 * 32 each is 3.1e-5 at the very worst, times ln 2 for the weight, plus 2^-22 of the exp2: 2.2e-5
+relative; F32 q adds its own 2^-22 per element times sqrt(128) terms of random sign, below 1e-5 of |x| <= 32.  Bound used: 4e-5 of the weight
+and 1e-7 of the row's largest weight.
+out: an F16 probability is off by 2^-12 of itself (half a step, 2^-11 relative spacing at most 2^-11: eps / 2 = 2^-11), so out by at most
+2^-11 * sum |w v| <= 2^-11 * max |v|; the weights' own 4e-5 and the final rounding to F16, 2^-11 * |out|, come on top.  With F32 q the
+probabilities keep 22 bits: 4e-5 * max |v| covers all."""
+import numpy as np
+import pytest
+
+from tempura_b200 import _native as N
+
+pytestmark = pytest.mark.gpu
+BS = 16
+
+
+@pytest.fixture(scope="module")
+def H():
+    import torch
+    assert torch.cuda.is_available()
+    from tempura_b200 import handoff
+    return handoff
+
+
+class Cache:
+    """A pool of garbage (NaN, infinities) with a batch's rows written into shuffled blocks, and its values in 64 bits."""
+
+    def __init__(self, H, lens, kv_heads, head_dim, dtype, layers=1, seed=0, shared=None, spare=3):
+        import torch
+        g = torch.Generator().manual_seed(seed)
+        self.lens, self.kv_heads, self.head_dim = list(lens), kv_heads, head_dim
+        width = max(1, max((t + BS - 1) // BS for t in self.lens))
+        rows, count, first = [], 0, {}
+        for s, t in enumerate(self.lens):
+            nb = (t + BS - 1) // BS
+            row = []
+            if shared is not None and shared[s] is not None:          # (group, prefix blocks)
+                grp, pre = shared[s]
+                if grp not in first:
+                    first[grp] = list(range(count, count + pre))
+                    count += pre
+                row = first[grp][:nb]
+            row = row + list(range(count, count + nb - len(row)))
+            count = max([count] + [r + 1 for r in row])
+            rows.append(row + [-1] * (width - nb))                    # never read: -1 is outside every pool
+        total = count + spare
+        perm = torch.randperm(total, generator=g)
+        self.tables = torch.tensor([[int(perm[b]) if b >= 0 else -1 for b in r] for r in rows], dtype=torch.int32)
+        scaled = dtype == "e4m3"
+        self.pool = H.Pool.allocate(0, layers, kv_heads, head_dim, BS, total, "f16" if dtype == "f16" else "e4m3", scales=scaled, fill_byte=None)
+        self.values = {}
+        for layer in range(layers):
+            for is_v in (False, True):
+                x = torch.randn((total, BS, kv_heads, head_dim), generator=g) * 0.5
+                x[..., head_dim // 3] *= 6
+                x = x.to(torch.float16)
+                view = self.pool.blocks(layer, is_v)
+                live = torch.zeros((total, BS), dtype=torch.bool)
+                for s, t in enumerate(self.lens):
+                    for b in range((t + BS - 1) // BS):
+                        live[int(self.tables[s, b]), : min(BS, t - b * BS)] = True
+                if dtype == "f16":
+                    val = x.double()
+                    bad = torch.full_like(x, float("nan"))
+                    bad[..., ::2] = float("inf")
+                    view.copy_(torch.where(live[:, :, None, None], x, bad))
+                else:
+                    y, sc = x.float(), torch.ones((total, kv_heads))
+                    if scaled:
+                        sc = (torch.where(live[:, :, None, None], y, torch.zeros_like(y)).abs().amax(dim=(1, 3)) / 448).clamp_min(1e-6)
+                        sc[::3] *= 64                               # blocks of very different scales side by side
+                        y = y / sc[:, None, :, None]
+                    y = torch.where(y.abs() < 2.0 ** -6, torch.zeros_like(y), y).clamp(-448, 448).to(torch.float8_e4m3fn)
+                    val = y.float().double() * sc.double()[:, None, :, None]
+                    raw = torch.where(live[:, :, None, None], y.view(torch.uint8), torch.full(y.shape, 0x7F, dtype=torch.uint8))   # NaN bytes
+                    view.copy_(raw)
+                    if scaled:
+                        (self.pool.v_scales if is_v else self.pool.k_scales)[layer].copy_(sc)
+                self.values[layer, is_v] = val
+        self.dev_tables = self.tables.cuda()
+        self.dev_lens = torch.tensor(self.lens, dtype=torch.int32).cuda()
+        torch.cuda.synchronize()
+
+    def rows(self, layer, is_v, s, n=None):
+        """[tokens, kv_heads, head_dim] of sequence s in 64 bits."""
+        n = self.lens[s] if n is None else n
+        blocks = self.tables[s, : (n + BS - 1) // BS].long()
+        return self.values[layer, is_v][blocks].flatten(0, 1)[:n]
+
+    def attention(self, layer, q, scale):
+        """Per sequence: (out [heads, dim], weights [heads, tokens], max |v| per kv head)."""
+        import torch
+        res = []
+        hq = q.shape[1]
+        grp = hq // self.kv_heads
+        for s in range(len(self.lens)):
+            if self.lens[s] == 0:
+                res.append((torch.zeros(hq, self.head_dim, dtype=torch.float64), torch.zeros(hq, 0, dtype=torch.float64), torch.zeros(hq, 1, dtype=torch.float64)))
+                continue
+            k = self.rows(layer, False, s).repeat_interleave(grp, dim=1)
+            v = self.rows(layer, True, s).repeat_interleave(grp, dim=1)
+            x = torch.einsum("hd,thd->ht", q[s].double(), k) * scale
+            w = torch.softmax(x, dim=1)
+            res.append((torch.einsum("ht,thd->hd", w, v), w, v.abs().amax(dim=(0, 2))[:, None]))
+        return res
+
+
+def out_close(got, want, vmax, f32):
+    import torch
+    got = got.double().cpu()
+    bound = (4e-5 if f32 else 2.0 ** -11 + 4e-5) * vmax + (2.0 ** -23 if f32 else 2.0 ** -11) * want.abs() + 1e-7
+    err = (got - want).abs()
+    assert torch.isfinite(got).all()
+    assert (err <= bound).all(), f"off by {(err / bound).max():.2f} of the bound"
+
+
+def scores_close(got, want, start):
+    """got, want: after the step; `start`: before it."""
+    import torch
+    got = got.double().cpu()
+    w = want - start
+    bound = 4e-5 * w.abs() + 2.0 ** -22 * want.abs() + 1e-7 * w.abs().max().clamp_min(0)
+    err = (got - want).abs()
+    assert (err <= bound).all(), f"off by {(err / bound.clamp_min(1e-30)).max():.2f} of the bound"
+
+
+# ---- scored decode attention ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f16", "e4m3", "e4m3 unscaled"])
+@pytest.mark.parametrize("kv_heads,head_dim,group", [(8, 128, 4), (4, 64, 8), (1, 128, 1), (5, 128, 3), (3, 64, 2), (16, 64, 1), (2, 128, 8)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_scored_attention(H, dtype, kv_heads, head_dim, group, f32):
+    import torch
+    lens = [1, 15, 0, 16, 17, 63, 64, 65, 400, 1029, 33, 0]
+    c = Cache(H, lens, kv_heads, head_dim, dtype, layers=2, seed=kv_heads * 7 + head_dim)
+    g = torch.Generator().manual_seed(5)
+    q = torch.randn((len(lens), kv_heads * group, head_dim), generator=g) * 2
+    q = q if f32 else q.to(torch.float16)
+    stride = max(lens) + 3
+    start = torch.rand((2, len(lens), kv_heads, stride), generator=g)
+    for s, t in enumerate(lens):
+        start[:, s, :, t:] = float("nan")                            # behind the end: never read, never written
+    scores = start.cuda()
+    decay = 0.75
+    attn = H.ScoredDecodeAttention(c.pool, q.cuda(), c.dev_tables, c.dev_lens, scores, max(lens), decay=decay)
+    for layer in (1, 0):
+        out = attn.enqueue(layer).clone()
+        assert int(attn.status.item()) == 0
+        for s, (want, w, vmax) in enumerate(c.attention(layer, q, attn.sm_scale)):
+            out_close(out[s], want, vmax, f32)
+            t = lens[s]
+            if t:
+                before = start[layer, s, :, :t].double() * decay
+                scores_close(scores[layer, s, :, :t], before + w.view(kv_heads, group, t).sum(dim=1), before)
+    assert torch.equal(torch.isnan(scores).cpu(), torch.isnan(start))
+
+
+def test_scored_attention_long_context_overwrites_at_decay_zero(H):
+    """One sequence split over the whole grid, its scores starting as NaN: decay 0 does not read them.  The weights of a row sum to the group."""
+    import torch
+    n = 20011
+    c = Cache(H, [n], 2, 128, "f16", seed=3)
+    q = (torch.randn((1, 16, 128), generator=torch.Generator().manual_seed(1)) * 2).to(torch.float16)
+    scores = torch.full((1, 1, 2, n), float("nan")).cuda()
+    attn = H.ScoredDecodeAttention(c.pool, q.cuda(), c.dev_tables, c.dev_lens, scores, n, decay=0.0)
+    out = attn.enqueue(0)
+    (want, w, vmax), = c.attention(0, q, attn.sm_scale)
+    out_close(out[0], want, vmax, False)
+    w = w.view(2, 8, n).sum(dim=1)
+    scores_close(scores[0, 0], w, torch.zeros_like(w))
+    assert abs(float(scores.double().sum()) - 16.0) < 16 * 1e-5
+    again = scores.clone()
+    attn.enqueue(0)
+    assert torch.equal(scores, again)                                 # no atomics: the same bits every time
+
+
+def test_scored_attention_more_sequences_than_a_cta_caches(H):
+    """1 500 sequences of 0 to 40 tokens: more than a CTA keeps the ranges of, several to one share, many empty."""
+    import torch
+    lens = [(s * 7919) % 41 if s % 3 else 0 for s in range(1500)]
+    c = Cache(H, lens, 2, 64, "f16", seed=4)
+    q = torch.randn((1500, 4, 64), generator=torch.Generator().manual_seed(2)).to(torch.float16)
+    scores = torch.zeros((1, 1500, 2, 48)).cuda()
+    attn = H.ScoredDecodeAttention(c.pool, q.cuda(), c.dev_tables, c.dev_lens, scores, 48)
+    out = attn.enqueue(0)
+    assert int(attn.status.item()) == 0
+    for s, (want, w, vmax) in enumerate(c.attention(0, q, attn.sm_scale)):
+        out_close(out[s], want, vmax, False)
+        if lens[s]:
+            w = w.view(2, 2, lens[s]).sum(dim=1)
+            scores_close(scores[0, s, :, : lens[s]], w, torch.zeros_like(w))
+    for s, t in enumerate(lens):
+        assert (scores[0, s, :, t:] == 0).all()
+
+
+def test_scored_attention_in_a_graph_and_on_another_stream(H):
+    """Captured once, replayed after lengths, q and scores changed in place; a call on another stream than the tensors' own."""
+    import torch
+    lens = [70, 200]
+    c = Cache(H, lens, 4, 64, "e4m3", seed=6)
+    q = torch.randn((2, 32, 64), generator=torch.Generator().manual_seed(9)).to(torch.float16)
+    dq, scores = q.cuda(), torch.zeros((1, 2, 4, 256)).cuda()
+    attn = H.ScoredDecodeAttention(c.pool, dq, c.dev_tables, c.dev_lens, scores, 256 - 48)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        attn.enqueue(0)
+    torch.cuda.current_stream().wait_stream(side)
+    first, first_scores = attn.out.clone(), scores.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attn.enqueue(0)
+    scores.zero_()
+    graph.replay()
+    assert torch.equal(attn.out, first) and torch.equal(scores, first_scores)
+    c.dev_lens.copy_(torch.tensor([33, 0], dtype=torch.int32))
+    c.lens = [33, 0]
+    scores.zero_()
+    graph.replay()
+    (want, w, vmax), (zero, _, _) = c.attention(0, q, attn.sm_scale)
+    out_close(attn.out[0], want, vmax, False)
+    assert (attn.out[1] == 0).all()
+    assert (scores[0, 1] == 0).all() and (scores[0, 0, :, 33:] == 0).all()
+
+
+def test_scored_attention_reports_bad_lengths_and_blocks(H):
+    import torch
+    c = Cache(H, [40, 90], 2, 64, "f16", seed=8)
+    q = torch.randn((2, 4, 64)).to(torch.float16).cuda()
+    scores = torch.zeros((1, 2, 2, 128)).cuda()
+    attn = H.ScoredDecodeAttention(c.pool, q, c.dev_tables, torch.tensor([40, 100000], dtype=torch.int32).cuda(), scores, 90)
+    attn.enqueue(0)
+    assert int(attn.status.item()) == N.ERR_INVALID_CONFIG
+    assert (scores[0, 1, :, 90:] == 0).all()                           # clamped
+    bad = c.dev_tables.clone()
+    bad[1, 2] = 1 << 20
+    attn = H.ScoredDecodeAttention(c.pool, q, bad, c.dev_lens, scores, 90)
+    attn.enqueue(0)
+    assert int(attn.status.item()) == N.ERR_INVALID_CONFIG
+
+
+def test_scored_attention_masked_rows_and_extreme_scores(H):
+    """Scores of +-6e4 (far outside exp's range) and equal scores: the maximum is subtracted, ties share."""
+    import torch
+    c = Cache(H, [50], 1, 64, "f16", seed=2)
+    c.pool.blocks(0, False).zero_()
+    k = torch.zeros((50, 64), dtype=torch.float16)
+    k[:, 0] = torch.linspace(-200, 200, 50).to(torch.float16)
+    k[30:, 0] = 200.0
+    for t in range(50):
+        c.pool.blocks(0, False)[int(c.tables[0, t // BS]), t % BS, 0] = k[t].cuda()
+    q = torch.zeros((1, 2, 64), dtype=torch.float16)
+    q[0, 0, 0] = 300.0
+    scores = torch.zeros((1, 1, 1, 64)).cuda()
+    attn = H.ScoredDecodeAttention(c.pool, q.cuda(), c.dev_tables, c.dev_lens, scores, 50, sm_scale=1.0)
+    out = attn.enqueue(0).double().cpu()
+    v = c.rows(0, True, 0)[:, 0]
+    assert torch.allclose(out[0, 0], v[30:].mean(dim=0), atol=2e-3)    # head 0: the twenty equal maxima
+    assert torch.allclose(out[0, 1], v.mean(dim=0), atol=2e-3)         # head 1: q = 0, all tokens alike
+    want = torch.full((50,), 1 / 50, dtype=torch.float64)
+    want[30:] += 1 / 20
+    assert torch.allclose(scores[0, 0, 0, :50].double().cpu(), want, rtol=1e-6)
+
+
+def test_scored_attention_refusals(H):
+    import torch
+    c = Cache(H, [40], 2, 64, "f16", seed=1)
+    q = torch.zeros((1, 4, 64), dtype=torch.float16).cuda()
+    scores = torch.zeros((1, 1, 2, 64)).cuda()
+
+    def code(change, **kw):
+        attn = H.ScoredDecodeAttention(c.pool, q, c.dev_tables, c.dev_lens, scores, 40, **kw)
+        args = attn._mk(0)
+        for name, value in change.items():
+            setattr(args, name, value)
+        import ctypes
+        rc = N.lib().tkv_scored_attn_enqueue(ctypes.byref(attn._pool_c), ctypes.byref(args), None)
+        return rc
+    assert code({}) == 0
+    assert code({"n_seqs": 0}) == 0
+    for change in ({"layer": 1}, {"q": 0}, {"out": 0}, {"tables": 0}, {"kv_lens": 0}, {"scores": 0}, {"q_dtype": N.DTYPE_E4M3}, {"decay": 1.5},
+                   {"decay": float("nan")}, {"sm_scale": float("inf")}, {"q": q.data_ptr() + 2}, {"scores": scores.data_ptr() + 2}):
+        assert code(change) == N.ERR_INVALID_CONFIG, change
+    for change in ({"n_q_heads": 3}, {"n_q_heads": 18}, {"table_stride": 2}, {"score_stride": 39}, {"scratch_bytes": 100}, {"scratch": 0}):
+        assert code(change) == N.ERR_DIMENSION_MISMATCH, change
