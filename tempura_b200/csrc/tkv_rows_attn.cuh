@@ -7,18 +7,27 @@
 // and (m, l, O) of a token range is one partial result; ranges are joined by a second kernel.
 //
 // Bound: every cached K and V byte is read once, 2 x head_dim multiply-adds per query head and byte pair, so HBM sets the pace and
-// what matters is bytes in flight and few instructions per byte.  A warp works alone: one kv head, one contiguous share of the
-// batch's cached blocks, an 8 KB x 3 ring of its own that its lanes fill with 16-byte cp.async and read back lane by lane (every
-// lane copies the pieces that its own MMA fragments need, so the ring needs no barrier and no swizzle).  The eight warps of a CTA
-// are eight kv heads of the same tokens where the pool has eight, so the copies of a CTA cover whole pool rows.  The order of the
-// dims inside a contraction is free, which is what lets a lane's fragment be a 16-byte run of a row: the four lanes of a token take
-// neighbouring 16-byte pieces of K (64-byte runs), the eight lanes of four tokens neighbouring pieces of V (128-byte runs).
+// what matters is bytes in flight, large copies, and few instructions per byte.  A stream is a run of up to eight kv heads over a
+// contiguous share of the batch's cached blocks: a producer warp keeps a ring of whole blocks in flight with bulk copies, and
+// consumer warps, one kv head each, read their fragments out of the stage and hand it back.  A CTA holds 8 / heads streams, so
+// pools with few kv heads keep as many warps busy.  A block arrives as four runs of four tokens, 32 bytes apart from a multiple of 128
+// in shared memory (one copy per token cost 50 ns each: 1.6 us per block against 0.7 us that HBM needs for an E4M3 block; one copy
+// per block leaves four-way bank conflicts).  With token(j, i) = 4 * (i odd ? j ^ 2 : j) + i as the i-th token of the four lanes j, the
+// 16-byte fragment reads of K (four lanes side by side in each of two tokens) and of V (two lanes side by side in each of four tokens)
+// are free of bank conflicts.  The order of the dims inside a contraction is free too: a lane's fragment is a 16-byte run.
 // Both contractions run on mma.sync m16n8k16 with the tokens (K) or the dims (V) as the 16 rows and the query heads as the 8
 // columns; the maximum is only raised, for all lanes at once after a vote, when a score exceeds it by 2^6, so the common step has
-// no shuffle in it.
+// no shuffle in it.  Probabilities are used as two F16 terms (22 bits): with up to four query heads per kv head the second term
+// rides in the four spare columns of the same MMAs, else it is a second set of them.
+//
+// A block costs a consumer a chain of dependent steps (wait, fragments, eight MMAs, exp2, transposes, eight MMAs).  For an F16 block the
+// chain is shorter than the time in which HBM delivers the block; for an E4M3 block, with half the bytes and a conversion in the
+// chain, it is longer, so two consumers take its blocks in turns, each with its own partial result (F32 operands need the registers
+// of both).  Stages then come in pairs: a stage always belongs to the same consumer, whose wait for a barrier's phase would otherwise
+// be answered by the phase before the one that its partner waits for.
 //
 // Work split: the batch's blocks, sequence after sequence, are cut into `parts` equal shares that may span sequences; part p and
-// sequence s meet in partial slot p + s, which is unique because both only grow along the batch.
+// sequence s meet in partial slot p + s (subs_of results each), which is unique because both only grow along the batch.
 #pragma once
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -28,9 +37,13 @@
 namespace tkv_rows {
 
 constexpr int BS = 16;                       // tokens per block
-constexpr int WARPS = 8;
-constexpr int STAGES = 3;
-constexpr int STAGE_DATA = 8192, STAGE_BYTES = STAGE_DATA + 64;
+constexpr int WARPS = 8;                     // consumer warps of a share of the blocks
+// consumers of a kv head, on alternate blocks: partial results per slot
+__host__ __device__ constexpr int subs_of(bool fp8, bool f32) { return fp8 && !f32 ? 2 : 1; }
+__host__ __device__ constexpr int threads_of(bool fp8, bool f32) { return (WARPS * subs_of(fp8, f32) + 1) * 32; }   // and the producer
+constexpr int MAX_STAGES = 8;
+constexpr uint32_t PAD = 32;                 // bytes between runs of four tokens
+constexpr uint32_t RING_BYTES = 208 * 1024;  // of all streams of a CTA
 constexpr uint32_t SEQ_CACHE = 1024;         // sequences whose ranges a CTA keeps in shared memory (more are looked up again)
 constexpr float RAISE = 6.0f;                // log2: probabilities reach 2^6, far inside F16
 
@@ -40,13 +53,14 @@ struct Args {
     const void* q;                           // f16 or f32 [n_seqs][n_q_heads][D]
     const uint32_t *tables, *kv_lens;
     const uint32_t *group_starts, *prefix_lens;   // shared-prefix groups, or null: ranges begin at token 0
-    float *part_o, *part_ml;                 // [slot][n_q_heads][D], [slot][n_q_heads][2]
+    float *part_o, *part_ml;                 // [slot][sub][n_q_heads][D], [slot][sub][n_q_heads][2]
     float* logits;                           // [n_seqs][n_q_heads][logit_stride], or null
     uint32_t* plan;                          // [0] blocks per part, [1 + s] blocks before sequence s (n_seqs + 1 entries)
     uint32_t* status;
     uint64_t block_stride;
     uint32_t row_stride, n_seqs, n_groups, n_q_heads, n_kv_heads, group, table_stride, max_kv_len, max_prefix_len, total_blocks, parts, min_share,
         logit_stride;
+    uint32_t heads, streams, head_groups, stages;   // kv heads per stream, streams per CTA, streams per part, ring depth
     float scale_log2;
 };
 
@@ -74,10 +88,27 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool ok) {   // zeros where !ok
-    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16u : 0u) : "memory");
-    if (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(ok ? 8u : 0u) : "memory");
-    if (BYTES == 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4u : 0u) : "memory");
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// bounded: gives up after 2^17 polls (a few seconds: a poll may sleep for some 45 us), or as soon as another warp of the CTA has recorded a failure
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, const volatile uint32_t* fail) {
+    for (uint32_t it = 0; it < (1u << 17); it++) {
+        if (bar_test(bar, parity)) return true;
+        if ((it & 15u) == 15u && *fail) return false;
+    }
+    return false;
+}
+
+__device__ __forceinline__ void shared_read16(uint32_t at, uint32_t (&w)[4]) {
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
+}
+__device__ __forceinline__ void shared_read8(uint32_t at, uint32_t (&w)[4]) {
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at));
 }
 
 // The group table is device memory that the host has not seen: it is used only if its starts ascend and end inside the batch and
@@ -115,35 +146,34 @@ __device__ __forceinline__ uint2 own_range(const Args& a, uint32_t s) {
 __device__ __forceinline__ uint32_t blocks_of(uint2 r) { return (r.y + BS - 1) / BS - r.x / BS; }
 
 template <int D, bool FP8> struct Shape {
-    static constexpr int ES = FP8 ? 1 : 2;
-    static constexpr int KB = D / 4 * ES, VB = D / 8 * ES;     // bytes of a K token per lane (4 lanes share it), of a V token (8 lanes)
-    static constexpr int KP = KB / 16;                          // 16-byte pieces of a K token per lane
-    static constexpr int VPB = VB >= 16 ? 16 : 8, VP = VB / VPB;
-    static constexpr int LANE_BLOCK = 2 * KB + 4 * VB;          // a lane holds 2 tokens of K and 4 of V
-    static constexpr int NB = STAGE_DATA / 32 / LANE_BLOCK;     // blocks per stage: 1 (F16, 128 dims) .. 4 (E4M3, 64 dims)
+    static constexpr int ES = FP8 ? 1 : 2, ROW = D * ES;       // bytes of one kv head's row
+    static constexpr int KP = ROW / 64;                         // 16-byte pieces of a K token per lane (4 lanes share it)
+    static constexpr int VB = ROW / 8, VPB = VB >= 16 ? 16 : 8, VP = VB / VPB;   // bytes of a V token per lane (8 lanes), and its pieces
     static constexpr int KS = D / 16, MT = D / 16;              // k-steps of Q.K, row tiles of V^T.P
 };
 
-// a position in a part's stream of blocks
+// a position in a part's run of blocks
 struct Cursor {
     uint32_t seq, block, left;                                  // block of the sequence; blocks left in it for this part
     uint32_t len;                                               // tokens of the sequence
     uint32_t rest;                                              // blocks left for this part behind this sequence
 };
 
-// F32: q and out are F32, q is used as two F16 terms (22 bits) and the probabilities too; else q and out are F16 and a probability is
-// one F16 (2^-12 of its own value at most, below the rounding of the output).
-template <int D, bool FP8, bool F32>
-__global__ void __launch_bounds__(WARPS * 32, 1) rows_attn(const Args a) {
+// F32: q and out are F32 and q is used as two F16 terms (22 bits); else both are F16.
+// WIDE: more than four query heads per kv head (the second term of the probabilities then takes MMAs of its own).
+template <int D, bool FP8, bool F32, bool WIDE>
+__global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args a) {
     using S = Shape<D, FP8>;
-    constexpr int NB = S::NB, KS = S::KS, MT = S::MT;
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, grp = lane >> 2, j = lane & 3u;
-    extern __shared__ __align__(128) unsigned char smem[];
-    uint2* seq_info = reinterpret_cast<uint2*>(smem + WARPS * STAGES * STAGE_BYTES);            // [SEQ_CACHE]
-    __shared__ uint32_t cum[WARPS * 32 + 1], warp_sum[WARPS];
+    constexpr int THREADS = threads_of(FP8, F32), NWARPS = THREADS / 32;
+    constexpr int KS = S::KS, MT = S::MT;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    extern __shared__ __align__(128) unsigned char ring[];
+    __shared__ uint2 seq_info[SEQ_CACHE];
+    __shared__ uint32_t cum[THREADS + 1], warp_sum[NWARPS], fail;
+    __shared__ uint64_t full[WARPS][MAX_STAGES], empty[WARPS][MAX_STAGES];   // [stream][stage]
 
     if (a.group_starts) {
-        const bool bad = groups_bad(a.group_starts, a.prefix_lens, a.n_groups, a.n_seqs, a.max_prefix_len, tid, WARPS * 32);
+        const bool bad = groups_bad(a.group_starts, a.prefix_lens, a.n_groups, a.n_seqs, a.max_prefix_len, tid, THREADS);
         if (__syncthreads_or(bad)) {
             if (tid == 0) {
                 report(a.status, 2u);
@@ -153,7 +183,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) rows_attn(const Args a) {
         }
     }
     // ---- blocks before every run of `per` sequences ----
-    const uint32_t per = (a.n_seqs + WARPS * 32 - 1) / (WARPS * 32);
+    const uint32_t per = (a.n_seqs + THREADS - 1) / THREADS;
     uint32_t mine = 0;
     for (uint32_t i = 0; i < per; i++) {
         const uint32_t s = tid * per + i;
@@ -171,14 +201,23 @@ __global__ void __launch_bounds__(WARPS * 32, 1) rows_attn(const Args a) {
         if (lane >= (uint32_t)o) incl += v;
     }
     if (lane == 31) warp_sum[warp] = incl;
+    if (tid < WARPS) {                                          // the streams' barriers; the last run of heads may be short
+        const uint32_t hg = (blockIdx.x * a.streams + tid) % a.head_groups, n = min(a.heads, a.n_kv_heads - hg * a.heads);
+        for (uint32_t i = 0; i < (uint32_t)MAX_STAGES; i++) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_addr(&full[tid][i])));
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(&empty[tid][i])), "r"(n));
+        }
+        if (tid == 0) fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     __syncthreads();
     uint32_t before = 0;
 #pragma unroll
-    for (int w = 0; w < WARPS; w++) before += w < (int)warp ? warp_sum[w] : 0u;
+    for (int w = 0; w < NWARPS; w++) before += w < (int)warp ? warp_sum[w] : 0u;
     cum[tid] = before + incl - mine;
-    if (tid == WARPS * 32 - 1) cum[WARPS * 32] = before + incl;
+    if (tid == THREADS - 1) cum[THREADS] = before + incl;
     __syncthreads();
-    const uint32_t total = cum[WARPS * 32];
+    const uint32_t total = cum[THREADS];
     const uint32_t share = max((total + a.parts - 1) / a.parts, a.min_share);
     auto range_of = [&](uint32_t s) { return s < SEQ_CACHE ? seq_info[s] : own_range(a, s); };
     if (blockIdx.x == 0) {                                      // the joining kernel finds a sequence's parts from these
@@ -195,14 +234,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) rows_attn(const Args a) {
             a.plan[1 + a.n_seqs] = total;
         }
     }
-    const uint32_t stream = blockIdx.x * WARPS + warp, kvh = stream % a.n_kv_heads, part = stream / a.n_kv_heads;
-    if (part >= a.parts || (uint64_t)part * share >= total) return;
-    const uint32_t first = part * share, n_mine = min(share, total - first);
-
-    // ---- the first sequence of this part ----
-    Cursor c;
-    {
-        uint32_t lo = 0, hi = WARPS * 32;                       // cum[lo] <= first < cum[hi]
+    // blocks of part p, and where it starts
+    auto part_blocks = [&](uint32_t p) -> uint32_t { return p < a.parts && (uint64_t)p * share < total ? min(share, total - p * share) : 0u; };
+    auto part_start = [&](uint32_t p, uint32_t n) -> Cursor {
+        const uint32_t first = p * share;
+        uint32_t lo = 0, hi = THREADS;                          // cum[lo] <= first < cum[hi]
         while (hi - lo > 1) {
             const uint32_t mid = (lo + hi) >> 1;
             if (cum[mid] <= first) lo = mid;
@@ -214,12 +250,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) rows_attn(const Args a) {
             at += blocks_of(r);
             r = range_of(++s);
         }
+        Cursor c;
         c.seq = s;
         c.block = r.x / BS + (first - at);
-        c.left = min(blocks_of(r) - (first - at), n_mine);
+        c.left = min(blocks_of(r) - (first - at), n);
         c.len = r.y;
-        c.rest = n_mine - c.left;
-    }
+        c.rest = n - c.left;
+        return c;
+    };
     auto next_sequence = [&](Cursor& x) {                       // called with left == 0 and rest > 0: a later sequence has blocks
         uint2 r;
         do r = range_of(++x.seq);
@@ -229,123 +267,194 @@ __global__ void __launch_bounds__(WARPS * 32, 1) rows_attn(const Args a) {
         x.len = r.y;
         x.rest -= x.left;
     };
-
-    // ---- the ring ----
-    unsigned char* ring = smem + (size_t)warp * STAGES * STAGE_BYTES;
-    const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
-    const size_t head_off = (size_t)kvh * D * S::ES;
-    Cursor f = c;                                               // what is fetched next
-    bool f_done = false;
-    auto ids_at = [&](const Cursor& x, bool done) -> uint32_t { // lane b: block id of block b of the stage at x
-        uint32_t id = 0;
-        if (!done && lane < (uint32_t)NB && lane < x.left) {
-            id = __ldg(a.tables + (size_t)x.seq * a.table_stride + x.block + lane);
-            if (id >= a.total_blocks) {                         // never dereferenced: block 0 is read instead and the launch reports it
-                report(a.status, 2u);
-                id = 0;
-            }
-        }
-        return id;
+    auto block_id = [&](const Cursor& x, uint32_t i) -> uint32_t {
+        const uint32_t id = __ldg(a.tables + (size_t)x.seq * a.table_stride + x.block + i);
+        if (id < a.total_blocks) return id;
+        report(a.status, 2u);                                   // never dereferenced: block 0 is read instead and the launch reports it
+        return 0u;
     };
-    uint32_t ids = ids_at(f, false);
-    auto fetch = [&](uint32_t slot) {
-        if (!f_done) {
-            const uint32_t base = ring_addr + slot * STAGE_BYTES;
-            const uint32_t n = min(f.left, (uint32_t)NB);
+    const uint32_t row_smem = a.heads * S::ROW, run_smem = 4 * row_smem + PAD, plane = 4 * run_smem, stage_bytes = 2 * plane;
+
+    if (warp == NWARPS - 1) {
+        // ---- producer: the streams in step, block k of each; lane x keeps the place in stream x.  A run of tokens is one copy where the
+        // stream has all heads of the pool, else its tokens are copied one by one: lane 16 * (V) + token, lanes without a copy idle ----
+        const uint32_t stream = blockIdx.x * a.streams + lane, hg_l = stream % a.head_groups;
+        const uint32_t n_l = lane < a.streams ? part_blocks(stream / a.head_groups) : 0u;
+        Cursor f{};
+        if (n_l) f = part_start(stream / a.head_groups, n_l);
+        bool done = n_l == 0;
+        uint32_t id[4], live[4], id_next[4], live_next[4];
+        auto look_up = [&](uint32_t (&ids)[4], uint32_t (&lives)[4]) {    // the next four blocks of lane x's stream
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                const uint32_t id = __shfl_sync(0xFFFFFFFFu, ids, b);
-                const uint32_t t0 = (f.block + b) * BS;
-                const uint32_t live = b < (int)n ? min((uint32_t)BS, f.len - t0) : 0u;
-                const char* kb = a.k_base + (uint64_t)id * a.block_stride + head_off;
-                const char* vb = a.v_base + (uint64_t)id * a.block_stride + head_off;
-                const uint32_t kd = base + b * (S::LANE_BLOCK * 32) + lane * 16, vd = base + b * (S::LANE_BLOCK * 32) + 2 * S::KB * 32 + lane * S::VPB;
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const uint32_t tok = grp + 8 * h;
-                    const bool ok = tok < live;
-                    const char* row = kb + (size_t)(ok ? tok : 0u) * a.row_stride + j * 16;
-#pragma unroll
-                    for (int i = 0; i < S::KP; i++) copy_async<16>(kd + (h * S::KP + i) * 512, row + i * 64, ok);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint32_t tok = 2 * j + (i & 1) + 8 * (i >> 1);
-                    const bool ok = tok < live;
-                    const char* row = vb + (size_t)(ok ? tok : 0u) * a.row_stride + grp * S::VPB;
-#pragma unroll
-                    for (int p = 0; p < S::VP; p++) copy_async<S::VPB>(vd + (i * S::VP + p) * (32 * S::VPB), row + p * 128, ok);
+            for (int u = 0; u < 4; u++) {
+                ids[u] = lives[u] = 0;
+                if (!done) {
+                    ids[u] = block_id(f, 0);
+                    lives[u] = min((uint32_t)BS, f.len - f.block * BS);
+                    f.block++;
+                    if (--f.left == 0) {
+                        if (f.rest) next_sequence(f);
+                        else done = true;
+                    }
                 }
             }
-            if (FP8 && a.k_scales) {                            // lane 2b: K scale of block b, lane 2b + 1: V scale
-                const uint32_t id = __shfl_sync(0xFFFFFFFFu, ids, (lane >> 1) & (NB - 1));
-                if (lane < 2u * NB) copy_async<4>(base + STAGE_DATA + lane * 4, ((lane & 1u) ? a.v_scales : a.k_scales) + (size_t)id * a.n_kv_heads + kvh, true);
-            }
-            f.block += n;
-            f.left -= n;
-            if (f.left == 0) {
-                if (f.rest) next_sequence(f);
-                else f_done = true;
-            }
-            ids = ids_at(f, f_done);
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");   // one group per step, empty past the end
-    };
+        };
+        look_up(id, live);
+        const uint32_t n_max = __reduce_max_sync(0xFFFFFFFFu, n_l);
+        const bool whole = a.heads == a.n_kv_heads;
+        const uint32_t row = lane & 15u, per_copy = whole ? 4u : 1u;
+        const bool copies = row % per_copy == 0;
+        const char* base = ((lane >> 4) ? a.v_base : a.k_base) + (size_t)row * a.row_stride;
+        const uint32_t dst0 = smem_addr(ring) + (lane >> 4) * plane + (row >> 2) * run_smem + (row & 3u) * row_smem;
+        uint32_t issued = 0;                                    // lane x: blocks of stream x asked for
+        uint32_t slot = 0, phase = 1;                           // phase of `empty` that block k waits for; the first round waits for nothing
+        bool ok = true;
+        for (uint32_t k0 = 0; k0 < n_max && ok; k0 += 4) {
+            look_up(id_next, live_next);
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; i++) fetch(i);
-
-    uint32_t q_hi[KS][2], q_lo[F32 ? KS : 1][2];
-    auto load_q = [&](uint32_t seq) {
-        const size_t at = ((size_t)seq * a.n_q_heads + kvh * a.group + (grp < a.group ? grp : 0u)) * D;
-        const bool live = grp < a.group;
+            for (int u = 0; u < 4; u++) {
+                if (k0 + u < n_max && ok) {
+                    for (uint32_t x = 0; x < a.streams; x++) {
+                        const uint32_t block = __shfl_sync(0xFFFFFFFFu, id[u], x), rows = __shfl_sync(0xFFFFFFFFu, live[u], x);
+                        const uint32_t hg = __shfl_sync(0xFFFFFFFFu, hg_l, x);
+                        if (rows == 0 || !ok) continue;         // this stream has ended
+                        if (k0 + u >= a.stages) ok = bar_wait(smem_addr(&empty[x][slot]), phase, &fail);
+                        ok = __all_sync(0xFFFFFFFFu, ok);
+                        if (!ok) continue;
+                        const uint32_t bytes = min(a.heads, a.n_kv_heads - hg * a.heads) * S::ROW, bar = smem_addr(&full[x][slot]);
+                        if (lane == 0)
+                            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(2u * rows * bytes) : "memory");
+                        __syncwarp();
+                        if (lane == x) issued++;
+                        if (copies && row < rows)
+                            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                                         ::"r"(dst0 + (x * a.stages + slot) * stage_bytes),
+                                         "l"(base + (uint64_t)block * a.block_stride + (size_t)hg * a.heads * S::ROW), "r"(bytes * min(per_copy, rows - row)),
+                                         "r"(bar) : "memory");
+                    }
+                    if (++slot == a.stages) {
+                        slot = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
-            const int dim = FP8 ? (4 * (s >> 2) + (int)j) * 16 + (s & 3) * 4 : (4 * (s >> 1) + (int)j) * 8 + (s & 1) * 4;
-            if (F32) {
-                const float4 x = live ? *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.q) + at + dim) : make_float4(0, 0, 0, 0);
-                const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(x.z, x.w);
-                const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
-                q_hi[s][0] = h2_bits(h0);
-                q_hi[s][1] = h2_bits(h1);
-                q_lo[F32 ? s : 0][0] = h2_bits(__floats2half2_rn(x.x - f0.x, x.y - f0.y));
-                q_lo[F32 ? s : 0][1] = h2_bits(__floats2half2_rn(x.z - f1.x, x.w - f1.y));
-            } else {
-                const uint2 x = live ? *reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(a.q) + at + dim) : make_uint2(0, 0);
-                q_hi[s][0] = x.x;
-                q_hi[s][1] = x.y;
+            for (int u = 0; u < 4; u++) {
+                id[u] = id_next[u];
+                live[u] = live_next[u];
             }
         }
-    };
+        if (!ok && lane == 0) {
+            atomicCAS(&fail, 0u, 4u);
+            report(a.status, 4u);
+        }
+        // Whatever happens to the consumers, no copy is in flight when the CTA's shared memory goes: the last copy into every stage is waited for.
+        for (uint32_t x = 0; x < a.streams; x++) {
+            const uint32_t n = __shfl_sync(0xFFFFFFFFu, issued, x);
+            for (uint32_t k = n > a.stages ? n - a.stages : 0u; k < n; k++)
+                for (uint32_t it = 0; it < (1u << 17); it++)
+                    if (bar_test(smem_addr(&full[x][k % a.stages]), (k / a.stages) & 1u)) break;
+        }
+        return;
+    }
 
-    float o[MT][4], m2[2], l2[2], v_ref, v_inv;                // o[t]: dims 2t, 2t + 1 of this lane's run, query heads 2j, 2j + 1; in units of v_ref
-    auto begin_sequence = [&](uint32_t seq) {
-        load_q(seq);
+    // ---- consumer: one kv head of one stream, every block or every second one ----
+    constexpr uint32_t STEP = subs_of(FP8, F32);
+    const uint32_t sub = warp / WARPS, x_stream = (warp % WARPS) / a.heads, h = (warp % WARPS) % a.heads, stream = blockIdx.x * a.streams + x_stream;
+    const uint32_t part = stream / a.head_groups, kvh = (stream % a.head_groups) * a.heads + h;
+    if (x_stream >= a.streams || kvh >= a.n_kv_heads) return;
+    const uint32_t n_mine = part_blocks(part);
+    if (n_mine == 0) return;
+    const uint32_t grp = lane >> 2, j = lane & 3u;
+    Cursor c = part_start(part, n_mine);
+    const uint32_t run_k = (grp & 1u) ? (grp >> 1) ^ 2u : grp >> 1, tok_k = 4 * run_k + (grp & 1u);   // tokens of MMA rows grp, grp + 8: tok_k, tok_k + 2
+    const uint32_t tok_v0 = 4 * j, tok_v1 = 4 * (j ^ 2u) + 1;   // of k indices 2j, 2j + 1; of 2j + 8, 2j + 9: two more
+
+    // block scales: lane i holds those of block i of the batch at hand; the next batch's loads are already under way
+    const bool scaled = FP8 && a.k_scales != nullptr;
+    float ks_l = 1.0f, vs_l = 1.0f, ks_n = 1.0f, vs_n = 1.0f;
+    uint32_t next_n = 0;
+    Cursor look = c;
+    auto look_ahead = [&]() {                                   // loads the scales of up to 32 blocks at `look`, which moves on
+        next_n = min(look.left, 32u);
+        if (lane < next_n) {
+            const size_t at = (size_t)block_id(look, lane) * a.n_kv_heads + kvh;
+            ks_n = __ldg(a.k_scales + at);
+            vs_n = __ldg(a.v_scales + at);
+        }
+        look.block += next_n;
+        look.left -= next_n;
+        if (look.left == 0 && look.rest) next_sequence(look);
+    };
+    if (scaled) look_ahead();
+
+    uint32_t slot = sub, phase = 0;                             // ring stage of this consumer's next block
+    uint32_t turn = sub;                                        // blocks until it, counted from c.block
+    const uint32_t ring_base = smem_addr(ring) + x_stream * a.stages * stage_bytes;
+    const uint32_t k_off = ring_base + h * S::ROW + run_k * run_smem + (grp & 1u) * row_smem + j * 16, half = 2 * row_smem;
+    const uint32_t v_off = ring_base + plane + h * S::ROW + grp * S::VPB;
+    const uint32_t v_at0 = v_off + j * run_smem, v_at1 = v_off + (j ^ 2u) * run_smem + row_smem;
+    const bool col0 = 2 * j < a.group, col1 = 2 * j + 1 < a.group;
+
+    for (;;) {                                                  // the sequences of this part
+        uint32_t q_hi[KS][2], q_lo[F32 ? KS : 1][2];
+        {
+            const uint32_t head = WIDE ? grp : (grp & 3u);      // columns 4..7 repeat heads 0..3 where the spare columns carry second terms
+            const bool in = head < a.group;
+            const size_t at = ((size_t)c.seq * a.n_q_heads + kvh * a.group + (in ? head : 0u)) * D;
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                const int dim = FP8 ? (4 * (s >> 2) + (int)j) * 16 + (s & 3) * 4 : (4 * (s >> 1) + (int)j) * 8 + (s & 1) * 4;
+                if (F32) {
+                    const float4 v = in ? *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.q) + at + dim) : make_float4(0, 0, 0, 0);
+                    const __half2 h0 = __floats2half2_rn(v.x, v.y), h1 = __floats2half2_rn(v.z, v.w);
+                    const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+                    q_hi[s][0] = h2_bits(h0);
+                    q_hi[s][1] = h2_bits(h1);
+                    q_lo[F32 ? s : 0][0] = h2_bits(__floats2half2_rn(v.x - f0.x, v.y - f0.y));
+                    q_lo[F32 ? s : 0][1] = h2_bits(__floats2half2_rn(v.z - f1.x, v.w - f1.y));
+                } else {
+                    const uint2 v = in ? *reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(a.q) + at + dim) : make_uint2(0, 0);
+                    q_hi[s][0] = v.x;
+                    q_hi[s][1] = v.y;
+                }
+            }
+        }
+        float o[MT][4], m2[2] = {-INFINITY, -INFINITY}, l2[2] = {0.0f, 0.0f};   // o[t]: dims 2t, 2t + 1 of this lane's run, columns 2j, 2j + 1
 #pragma unroll
         for (int t = 0; t < MT; t++) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
-        m2[0] = m2[1] = -INFINITY;
-        l2[0] = l2[1] = 0.0f;
-        v_ref = FP8 ? 0x1p-100f : 1.0f;                         // a power of two above every V scale met so far: P x scale / v_ref stays in F16's range
-        v_inv = FP8 ? 0x1p+100f : 1.0f;
-    };
-    begin_sequence(c.seq);
+        float v_ref = FP8 ? 0x1p-100f : 1.0f, v_inv = FP8 ? 0x1p+100f : 1.0f;   // a power of two above every V scale met so far: O is in units of
+                                                                // it, and P x scale / v_ref stays in F16's range
+        float* lg = a.logits ? a.logits + ((size_t)c.seq * a.n_q_heads + kvh * a.group + 2 * j) * a.logit_stride + c.block * BS + tok_k : nullptr;
+        uint32_t batch_at = 0, batch_n = 0;                     // blocks [batch_at, batch_at + batch_n) of this sequence: the scales at hand
+        auto next_batch = [&]() {
+            ks_l = ks_n;
+            vs_l = vs_n;
+            batch_at += batch_n;
+            batch_n = next_n;
+            if (look.left) look_ahead();
+            else next_n = 0;
+        };
+        const uint32_t n = c.left;
+        for (; turn < n; turn += STEP) {
+            if (!bar_wait(smem_addr(&full[x_stream][slot]), phase, &fail)) {
+                if (lane == 0) {
+                    atomicCAS(&fail, 0u, 4u);
+                    report(a.status, 4u);
+                }
+                return;
+            }
+            __syncwarp();
+            const uint32_t stage = slot * stage_bytes;
+            const uint32_t live = min((uint32_t)BS, c.len - (c.block + turn) * BS);
 
-    for (uint32_t step = 0;; step++) {
-        fetch((step + STAGES - 1) % STAGES);                    // into the stage that the step before this one has read
-        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-        __syncwarp();
-        const unsigned char* stage = ring + (step % STAGES) * STAGE_BYTES;
-        const uint32_t n = min(c.left, (uint32_t)NB);
-
-        // scores
-        float x[NB][4], vs[NB];
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            const uint4* kp = reinterpret_cast<const uint4*>(stage + b * (S::LANE_BLOCK * 32)) + lane;
+            // scores
             float even[4] = {0.0f, 0.0f, 0.0f, 0.0f}, odd[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // two chains
 #pragma unroll
             for (int i = 0; i < S::KP; i++) {
-                const uint4 lo = kp[i * 32], hi = kp[(S::KP + i) * 32];
-                const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+                uint32_t wl[4], wh[4];
+                shared_read16(stage + k_off + i * 64, wl);
+                shared_read16(stage + k_off + half + i * 64, wh);
 #pragma unroll
                 for (int u = 0; u < (FP8 ? 4 : 2); u++) {
                     const int s = FP8 ? 4 * i + u : 2 * i + u;
@@ -356,113 +465,108 @@ __global__ void __launch_bounds__(WARPS * 32, 1) rows_attn(const Args a) {
                         a1 = e4m3x2_h2(wh[u] & 0xFFFFu);
                         a3 = e4m3x2_h2(wh[u] >> 16);
                     } else {
-                        a0 = wl[2 * u];
-                        a2 = wl[2 * u + 1];
-                        a1 = wh[2 * u];
-                        a3 = wh[2 * u + 1];
+                        a0 = wl[2 * (u & 1)];
+                        a2 = wl[2 * (u & 1) + 1];
+                        a1 = wh[2 * (u & 1)];
+                        a3 = wh[2 * (u & 1) + 1];
                     }
                     mma16816((u & 1) ? odd : even, a0, a1, a2, a3, q_hi[s][0], q_hi[s][1]);
                     if (F32) mma16816((u & 1) ? odd : even, a0, a1, a2, a3, q_lo[F32 ? s : 0][0], q_lo[F32 ? s : 0][1]);
                 }
             }
-            float ks = a.scale_log2;
-            vs[b] = 1.0f;
-            if (FP8 && a.k_scales) {
-                const float2 sc = *reinterpret_cast<const float2*>(stage + STAGE_DATA + b * 8);
-                ks *= sc.x;
-                vs[b] = b < (int)n ? sc.y : 0.0f;
+            float ks = a.scale_log2, vs = 1.0f;
+            if (scaled) {
+                while (turn >= batch_at + batch_n) next_batch();
+                ks *= __shfl_sync(0xFFFFFFFFu, ks_l, turn - batch_at);
+                vs = __shfl_sync(0xFFFFFFFFu, vs_l, turn - batch_at);
             }
-            const uint32_t live = b < (int)n ? min((uint32_t)BS, c.len - (c.block + b) * BS) : 0u;
+            float x[4];                                         // x[2 * (token half) + column]
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[b][i] = grp + 8 * (i >> 1) < live ? (even[i] + odd[i]) * ks : -INFINITY;   // x[b][2 * (token half) + head]
-            if (a.logits) {
+            for (int i = 0; i < 4; i++) x[i] = (even[i] + odd[i]) * ks;
+            if (live < (uint32_t)BS) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint32_t head = 2 * j + (i & 1), tok = grp + 8 * (i >> 1);
-                    if (head < a.group && tok < live)
-                        a.logits[((size_t)c.seq * a.n_q_heads + kvh * a.group + head) * a.logit_stride + (c.block + b) * BS + tok] = x[b][i];
+                for (int i = 0; i < 4; i++) x[i] = tok_k + 2 * (i >> 1) < live ? x[i] : -INFINITY;
+            }
+            if (lg) {
+                float* at = lg + turn * BS;
+                const bool lo = tok_k < live, hi = tok_k + 2 < live;
+                if (col0 && lo) at[0] = x[0];
+                if (col0 && hi) at[2] = x[2];
+                at += a.logit_stride;
+                if (col1 && lo) at[0] = x[1];
+                if (col1 && hi) at[2] = x[3];
+            }
+            // the maxima in use are raised, for all lanes together, once a score is 2^6 above
+            const bool over = fmaxf(x[0], x[2]) > m2[0] + RAISE || fmaxf(x[1], x[3]) > m2[1] + RAISE;
+            if (__any_sync(0xFFFFFFFFu, over)) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float mx = fmaxf(m2[e], fmaxf(x[e], x[2 + e]));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
+                    const float keep = m2[e] == -INFINITY ? 0.0f : exp2_fast(m2[e] - mx);
+                    m2[e] = mx;
+                    l2[e] *= keep;
+#pragma unroll
+                    for (int t = 0; t < MT; t++) {
+                        o[t][e] *= keep;
+                        o[t][2 + e] *= keep;
+                    }
                 }
             }
-        }
-        // the maxima in use are raised, for all lanes together, once a score is 2^6 above
-        bool over = false;
-        float v_top = 0.0f;
+            if (FP8 && vs > v_ref) {                            // the same in every lane
+                const float up = __uint_as_float(min((__float_as_uint(vs) >> 23) + 1u, 253u) << 23);
+                const float keep = v_ref / up;
+                v_ref = up;
+                v_inv = 1.0f / up;
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
+                for (int t = 0; t < MT; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) over |= x[b][i] > m2[i & 1] + RAISE;
-            v_top = fmaxf(v_top, vs[b]);
-        }
-        if (__any_sync(0xFFFFFFFFu, over)) {
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                float mx = m2[h];
-#pragma unroll
-                for (int b = 0; b < NB; b++) mx = fmaxf(mx, fmaxf(x[b][h], x[b][2 + h]));
-                mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
-                mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
-                mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
-                const float keep = m2[h] == -INFINITY ? 0.0f : exp2_fast(m2[h] - mx);
-                m2[h] = mx;
-                l2[h] *= keep;
-#pragma unroll
-                for (int t = 0; t < MT; t++) {
-                    o[t][h] *= keep;
-                    o[t][2 + h] *= keep;
-                }
+                    for (int i = 0; i < 4; i++) o[t][i] *= keep;
             }
-        }
-        if (FP8 && v_top > v_ref) {                             // the same in every lane
-            const float up = __uint_as_float(min((__float_as_uint(v_top) >> 23) + 1u, 253u) << 23);
-            const float keep = v_ref / up;
-            v_ref = up;
-            v_inv = 1.0f / up;
-#pragma unroll
-            for (int t = 0; t < MT; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) o[t][i] *= keep;
-        }
-        const float sub0 = m2[0] == -INFINITY ? 0.0f : m2[0], sub1 = m2[1] == -INFINITY ? 0.0f : m2[1];
-        // probabilities and O += V^T P
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
+            const float sub0 = m2[0] == -INFINITY ? 0.0f : m2[0], sub1 = m2[1] == -INFINITY ? 0.0f : m2[1];
+            // probabilities, and O += V^T P
             float p[4];
-            p[0] = exp2_fast(x[b][0] - sub0);
-            p[1] = exp2_fast(x[b][1] - sub1);
-            p[2] = exp2_fast(x[b][2] - sub0);
-            p[3] = exp2_fast(x[b][3] - sub1);
+            p[0] = exp2_fast(x[0] - sub0);
+            p[1] = exp2_fast(x[1] - sub1);
+            p[2] = exp2_fast(x[2] - sub0);
+            p[3] = exp2_fast(x[3] - sub1);
             l2[0] += p[0] + p[2];
             l2[1] += p[1] + p[3];
             if (FP8) {
-                const float vn = vs[b] * v_inv;
+                const float vn = vs * v_inv;
 #pragma unroll
                 for (int i = 0; i < 4; i++) p[i] *= vn;
             }
-            const __half2 pl = __floats2half2_rn(p[0], p[1]), ph = __floats2half2_rn(p[2], p[3]);
-            const uint32_t b0 = transpose8(h2_bits(pl)), b1 = transpose8(h2_bits(ph));   // rows: tokens 2j, 2j + 1 (+ 8); column: head grp
-            uint32_t c0 = 0, c1 = 0;
-            if (F32) {
-                const float2 fl = __half22float2(pl), fh = __half22float2(ph);
-                c0 = transpose8(h2_bits(__floats2half2_rn(p[0] - fl.x, p[1] - fl.y)));
-                c1 = transpose8(h2_bits(__floats2half2_rn(p[2] - fh.x, p[3] - fh.y)));
+            __half2 pl = __floats2half2_rn(p[0], p[1]), ph = __floats2half2_rn(p[2], p[3]);
+            const float2 fl = __half22float2(pl), fh = __half22float2(ph);
+            const __half2 rl = __floats2half2_rn(p[0] - fl.x, p[1] - fl.y), rh = __floats2half2_rn(p[2] - fh.x, p[3] - fh.y);
+            if (!WIDE && j >= 2) {                              // columns 4..7: the second terms of heads 0..3
+                pl = rl;
+                ph = rh;
             }
-            const unsigned char* vp = stage + b * (S::LANE_BLOCK * 32) + 2 * S::KB * 32 + lane * S::VPB;
+            const uint32_t b0 = transpose8(h2_bits(pl)), b1 = transpose8(h2_bits(ph));   // rows: k indices 2j, 2j + 1 (+ 8); column grp
+            uint32_t c0 = 0, c1 = 0;
+            if (WIDE) {
+                c0 = transpose8(h2_bits(rl));
+                c1 = transpose8(h2_bits(rh));
+            }
 #pragma unroll
             for (int pc = 0; pc < S::VP; pc++) {
-                uint32_t w[4][S::VPB / 4];
+                uint32_t w[4][4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const unsigned char* at = vp + (i * S::VP + pc) * (32 * S::VPB);
-                    if (S::VPB == 16) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(at);
-                        w[i][0] = v.x;
-                        w[i][1] = v.y;
-                        w[i][S::VPB / 4 - 2] = v.z;
-                        w[i][S::VPB / 4 - 1] = v.w;
-                    } else {
-                        const uint2 v = *reinterpret_cast<const uint2*>(at);
-                        w[i][0] = v.x;
-                        w[i][1] = v.y;
+                    const uint32_t at = stage + ((i & 1) ? v_at1 : v_at0) + (i >> 1) * half + pc * 128;
+                    if (S::VPB == 16) shared_read16(at, w[i]);
+                    else shared_read8(at, w[i]);
+                }
+                if (live < (uint32_t)BS) {                      // rows that were not copied hold an older block's bytes: 0 x NaN must not reach O
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t tok = ((i & 1) ? tok_v1 : tok_v0) + 2 * (i >> 1);
+#pragma unroll
+                        for (int e = 0; e < S::VPB / 4; e++) w[i][e] = tok < live ? w[i][e] : 0u;
                     }
                 }
                 constexpr int TILES = S::VPB / S::ES / 2;       // two dims of the run per row tile
@@ -482,74 +586,99 @@ __global__ void __launch_bounds__(WARPS * 32, 1) rows_attn(const Args a) {
                         a3 = __byte_perm(w[2][t], w[3][t], 0x7632u);
                     }
                     mma16816(o[pc * TILES + t], a0, a1, a2, a3, b0, b1);
-                    if (F32) mma16816(o[pc * TILES + t], a0, a1, a2, a3, c0, c1);
+                    if (WIDE) mma16816(o[pc * TILES + t], a0, a1, a2, a3, c0, c1);
                 }
             }
+            __syncwarp();                                       // every lane's reads of the stage are done
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&empty[x_stream][slot])) : "memory");
+            slot += STEP;
+            if (slot >= a.stages) {
+                slot -= a.stages;
+                phase ^= 1u;
+            }
         }
-        c.block += n;
-        c.left -= n;
-        if (c.left) continue;
+        turn -= n;
+        if (scaled)
+            while (batch_at + batch_n < n) next_batch();        // blocks of this sequence that were the other consumer's
 
-        // ---- the sequence's blocks of this part are done ----
-        const uint32_t slot = part + c.seq;
+        // ---- partial results of (part, sequence); a consumer that had no block says so with an empty sum ----
+        const size_t at_slot = ((size_t)part + c.seq) * STEP + sub;
+        if (!WIDE) {                                            // first and second terms of a head together
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            float l = l2[h];
+            for (int t = 0; t < MT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[t][i] += __shfl_xor_sync(0xFFFFFFFFu, o[t][i], 2);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            float l = l2[e];
             l += __shfl_xor_sync(0xFFFFFFFFu, l, 4);
             l += __shfl_xor_sync(0xFFFFFFFFu, l, 8);
             l += __shfl_xor_sync(0xFFFFFFFFu, l, 16);
-            const uint32_t head = 2 * j + h;
+            const uint32_t head = 2 * j + e;
             if (head < a.group) {
-                const size_t row = (size_t)slot * a.n_q_heads + kvh * a.group + head;
-                if (grp == 0) *reinterpret_cast<float2*>(a.part_ml + row * 2) = make_float2(m2[h], l);
+                const size_t row = at_slot * a.n_q_heads + kvh * a.group + head;
+                if (grp == 0) *reinterpret_cast<float2*>(a.part_ml + row * 2) = make_float2(m2[e], l);
                 float* dst = a.part_o + row * D;
 #pragma unroll
                 for (int t = 0; t < MT; t++) {
                     constexpr int RUN = S::VPB / S::ES;         // dims of a piece
-                    const int e = 2 * t, dim = (e / RUN) * (8 * RUN) + (int)grp * RUN + e % RUN;
-                    *reinterpret_cast<float2*>(dst + dim) = make_float2(o[t][h] * v_ref, o[t][2 + h] * v_ref);
+                    const int i = 2 * t, dim = (i / RUN) * (8 * RUN) + (int)grp * RUN + i % RUN;
+                    *reinterpret_cast<float2*>(dst + dim) = make_float2(o[t][e] * v_ref, o[t][2 + e] * v_ref);
                 }
             }
         }
         if (!c.rest) break;
         next_sequence(c);
-        begin_sequence(c.seq);
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------------
 struct Split {
+    uint32_t heads, streams, head_groups;    // of a stream, of a CTA, of a part
     uint32_t parts, min_share, grid;
 };
-// Parts for a batch of at most `blocks` cached blocks: one warp per part and kv head, one CTA per SM, and no part shorter than
-// MIN_SHARE blocks (a part costs the joining kernel a partial result per query head).
+// Streams of at most eight kv heads, as even as they come; parts for a batch of at most `blocks` cached blocks: one CTA per SM, and no
+// part shorter than MIN_SHARE blocks (a part costs the joining kernel a partial result per query head).
 constexpr uint32_t MIN_SHARE = 4;
-inline Split split_for(uint64_t blocks, uint32_t n_kv_heads, uint32_t sms) {
+inline Split split_for(uint64_t blocks, uint32_t n_kv_heads, uint32_t ctas) {
     Split s;
+    s.head_groups = (n_kv_heads + WARPS - 1) / WARPS;
+    s.heads = (n_kv_heads + s.head_groups - 1) / s.head_groups;
+    s.head_groups = (n_kv_heads + s.heads - 1) / s.heads;
+    s.streams = WARPS / s.heads;
     s.min_share = MIN_SHARE;
-    const uint64_t most = (uint64_t)sms * WARPS / n_kv_heads, want = (blocks + MIN_SHARE - 1) / MIN_SHARE;
+    const uint64_t most = (uint64_t)ctas * s.streams / s.head_groups, want = (blocks + MIN_SHARE - 1) / MIN_SHARE;
     s.parts = (uint32_t)(most < 1 ? 1 : want < 1 ? 1 : want < most ? want : most);
-    s.grid = (uint32_t)(((uint64_t)s.parts * n_kv_heads + WARPS - 1) / WARPS);
+    s.grid = (uint32_t)(((uint64_t)s.parts * s.head_groups + s.streams - 1) / s.streams);
     return s;
 }
-constexpr size_t SMEM_BYTES = (size_t)WARPS * STAGES * STAGE_BYTES + SEQ_CACHE * sizeof(uint2);
-static_assert(SMEM_BYTES + 2048 <= 227 * 1024, "shared memory of one CTA");
 
-template <int D, bool FP8, bool F32> cudaError_t launch_one(const Args& a, uint32_t grid, cudaStream_t st) {
-    auto kernel = rows_attn<D, FP8, F32>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
+template <int D, bool FP8, bool F32, bool WIDE> cudaError_t launch_one(Args a, const Split& sp, cudaStream_t st) {
+    using S = Shape<D, FP8>;
+    a.heads = sp.heads;
+    a.streams = sp.streams;
+    a.head_groups = sp.head_groups;
+    a.parts = sp.parts;
+    a.min_share = sp.min_share;
+    const uint32_t stage = 2 * (BS * sp.heads * S::ROW + 4 * PAD), fit = RING_BYTES / (sp.streams * stage);
+    a.stages = (fit < (uint32_t)MAX_STAGES ? fit : (uint32_t)MAX_STAGES) / subs_of(FP8, F32) * subs_of(FP8, F32);   // at least 3 (eight heads of 128
+                                                                                                    // F16 dims: 65 KB each), in pairs for pairs
+    const size_t smem = (size_t)sp.streams * a.stages * stage;
+    auto kernel = rows_attn<D, FP8, F32, WIDE>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RING_BYTES);
     if (e != cudaSuccess) return e;
-    kernel<<<grid, WARPS * 32, SMEM_BYTES, st>>>(a);
+    kernel<<<sp.grid, threads_of(FP8, F32), smem, st>>>(a);
     return cudaGetLastError();
 }
-inline cudaError_t launch_rows(uint32_t head_dim, bool fp8, bool f32, const Args& a, uint32_t grid, cudaStream_t st) {
-    if (head_dim == 128) {
-        if (fp8) return f32 ? launch_one<128, true, true>(a, grid, st) : launch_one<128, true, false>(a, grid, st);
-        return f32 ? launch_one<128, false, true>(a, grid, st) : launch_one<128, false, false>(a, grid, st);
-    }
-    if (fp8) return f32 ? launch_one<64, true, true>(a, grid, st) : launch_one<64, true, false>(a, grid, st);
-    return f32 ? launch_one<64, false, true>(a, grid, st) : launch_one<64, false, false>(a, grid, st);
+template <int D, bool FP8> cudaError_t launch_type(bool f32, const Args& a, const Split& sp, cudaStream_t st) {
+    const bool wide = a.group > 4;
+    if (f32) return wide ? launch_one<D, FP8, true, true>(a, sp, st) : launch_one<D, FP8, true, false>(a, sp, st);
+    return wide ? launch_one<D, FP8, false, true>(a, sp, st) : launch_one<D, FP8, false, false>(a, sp, st);
+}
+inline cudaError_t launch_rows(uint32_t head_dim, bool fp8, bool f32, const Args& a, const Split& sp, cudaStream_t st) {
+    if (head_dim == 128) return fp8 ? launch_type<128, true>(f32, a, sp, st) : launch_type<128, false>(f32, a, sp, st);
+    return fp8 ? launch_type<64, true>(f32, a, sp, st) : launch_type<64, false>(f32, a, sp, st);
 }
 
 }  // namespace tkv_rows

@@ -33,7 +33,7 @@ struct FinishArgs {
     const uint32_t *plan, *kv_lens;
     float* scores;
     void* out;
-    uint32_t n_seqs, n_q_heads, n_kv_heads, group, logit_stride, score_stride, max_kv_len, tasks;
+    uint32_t n_seqs, n_q_heads, n_kv_heads, group, logit_stride, score_stride, max_kv_len, tasks, subs;
     float decay;
 };
 
@@ -46,12 +46,23 @@ template <int D, bool F32> __global__ void __launch_bounds__(256) scored_finish(
     const bool join = task < a.group;
     const uint32_t t0 = join ? 0u : (task - a.group) * CHUNK;
     if (!join && t0 >= len) return;
+    const float* x = a.logits + ((size_t)s * a.n_q_heads + kvh * a.group) * a.logit_stride;
+    float xs[CHUNK / 256][8];                // asked for before the partial results are joined: one latency instead of two
+    if (!join) {
+#pragma unroll
+        for (int i = 0; i < CHUNK / 256; i++) {
+            const uint32_t t = t0 + i * 256 + tid;
+#pragma unroll
+            for (uint32_t g = 0; g < 8; g++) xs[i][g] = g < a.group && t < len ? x[(size_t)g * a.logit_stride + t] : -INFINITY;
+        }
+    }
     const uint32_t share = a.plan[0], lo = a.plan[1 + s], hi = a.plan[2 + s];
-    const uint32_t p0 = hi > lo ? lo / share : 0u, n = hi > lo ? (hi - 1) / share - p0 + 1 : 0u;   // partial results p0 + s .. p0 + s + n - 1
+    const uint32_t p0 = hi > lo ? lo / share : 0u, n = hi > lo ? ((hi - 1) / share - p0 + 1) * a.subs : 0u;
+    const size_t first = (size_t)(p0 + s) * a.subs;     // partial results first .. first + n - 1
     __shared__ float top[8], inv[8];
     if (warp < a.group && (!join || warp == task)) {            // warp g: maximum and sum of query head g
         float m = -INFINITY, l = 0.0f;
-        const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)(p0 + s) * a.n_q_heads + kvh * a.group + warp;
+        const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + first * a.n_q_heads + kvh * a.group + warp;
         for (uint32_t i = lane; i < n; i += 32) {
             const float2 v = ml[(size_t)i * a.n_q_heads];
             const float mm = fmaxf(m, v.x);
@@ -79,10 +90,16 @@ template <int D, bool F32> __global__ void __launch_bounds__(256) scored_finish(
         for (int i = 0; i < PER; i++) acc[i] = 0.0f;
         const float m = top[task];
         for (uint32_t i = warp; i < n; i += 8) {
-            const size_t r = (size_t)(p0 + s + i) * a.n_q_heads + kvh * a.group + task;
-            const float pm = a.part_ml[r * 2], f = pm == -INFINITY ? 0.0f : exp2_fast(pm - m);
+            const size_t r = (first + i) * a.n_q_heads + kvh * a.group + task;
+            const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + r * 2);
+            float v[PER];
 #pragma unroll
-            for (int k = 0; k < PER; k++) acc[k] += f * a.part_o[r * D + k * 32 + lane];
+            for (int k = 0; k < PER; k++) v[k] = a.part_o[r * D + k * 32 + lane];
+            const float f = exp2_fast(ml.x - m);
+            if (ml.x != -INFINITY || ml.y != 0.0f) {            // an empty part's O was never written
+#pragma unroll
+                for (int k = 0; k < PER; k++) acc[k] += f * v[k];
+            }
         }
         __shared__ float part[8][D];
 #pragma unroll
@@ -98,14 +115,15 @@ template <int D, bool F32> __global__ void __launch_bounds__(256) scored_finish(
             else reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(v);
         }
     } else {
-        const float* x = a.logits + ((size_t)s * a.n_q_heads + kvh * a.group) * a.logit_stride;
         float* sc = a.scores + ((size_t)s * a.n_kv_heads + kvh) * a.score_stride;
 #pragma unroll
         for (int i = 0; i < CHUNK / 256; i++) {
             const uint32_t t = t0 + i * 256 + tid;
             if (t < len) {
                 float w = 0.0f;
-                for (uint32_t g = 0; g < a.group; g++) w += exp2_fast(x[(size_t)g * a.logit_stride + t] - top[g]) * inv[g];
+#pragma unroll
+                for (uint32_t g = 0; g < 8; g++)
+                    if (g < a.group) w += exp2_fast(xs[i][g] - top[g]) * inv[g];
                 sc[t] = a.decay == 0.0f ? w : a.decay * sc[t] + w;
             }
         }
@@ -127,7 +145,7 @@ struct Layout {
 Layout layout_of(uint32_t n_seqs, uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t max_kv_len) {
     Layout l;
     l.split = tkv_rows::split_for((uint64_t)n_seqs * ((max_kv_len + 15ull) / 16), n_kv_heads, CTAS);
-    const uint64_t slots = (uint64_t)l.split.parts + n_seqs;
+    const uint64_t slots = ((uint64_t)l.split.parts + n_seqs) * 2;          // an E4M3 pool's slots hold two partial results
     l.logit_stride = (uint32_t)up(max_kv_len, 16);
     l.ml = up(4ull * (n_seqs + 2ull), 256);
     l.o = l.ml + up(slots * n_q_heads * 8ull, 256);
@@ -211,8 +229,6 @@ int32_t tkv_scored_attn_enqueue(const TkvPool* pool, const TkvScoredAttn* p, voi
     a.table_stride = p->table_stride;
     a.max_kv_len = p->max_kv_len;
     a.total_blocks = pool->total_blocks;
-    a.parts = l.split.parts;
-    a.min_share = l.split.min_share;
     a.logit_stride = l.logit_stride;
     a.scale_log2 = p->sm_scale * 1.4426950408889634f;
     FinishArgs f{};
@@ -231,6 +247,7 @@ int32_t tkv_scored_attn_enqueue(const TkvPool* pool, const TkvScoredAttn* p, voi
     f.score_stride = p->score_stride;
     f.max_kv_len = p->max_kv_len;
     f.tasks = tasks;
+    f.subs = tkv_rows::subs_of(es == 1, p->q_dtype == TKV_DTYPE_F32);
     f.decay = p->decay;
 
     int prev = -1;
@@ -239,7 +256,7 @@ int32_t tkv_scored_attn_enqueue(const TkvPool* pool, const TkvScoredAttn* p, voi
     if (e == cudaSuccess) {
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         const bool f32 = p->q_dtype == TKV_DTYPE_F32;
-        e = tkv_rows::launch_rows(pool->head_dim, es == 1, f32, a, l.split.grid, st);
+        e = tkv_rows::launch_rows(pool->head_dim, es == 1, f32, a, l.split, st);
         if (e == cudaSuccess) {
             const unsigned grid = (unsigned)finish_grid;
             if (pool->head_dim == 128) {

@@ -286,3 +286,23 @@ def test_scored_attention_refusals(H):
         assert code(change) == N.ERR_INVALID_CONFIG, change
     for change in ({"n_q_heads": 3}, {"n_q_heads": 18}, {"table_stride": 2}, {"score_stride": 39}, {"scratch_bytes": 100}, {"scratch": 0}):
         assert code(change) == N.ERR_DIMENSION_MISMATCH, change
+
+
+@pytest.mark.parametrize("dtype,kv_heads,head_dim,group", [("f16", 8, 128, 4), ("e4m3", 8, 128, 4), ("e4m3", 7, 128, 2), ("f16", 2, 64, 8), ("e4m3", 1, 64, 4)])
+def test_scored_attention_long_shares(H, dtype, kv_heads, head_dim, group):
+    """Enough blocks that every part walks its ring many times round, across sequences."""
+    import torch
+    lens = [3000 + 531 * s for s in range(9)] + [1, 17]
+    c = Cache(H, lens, kv_heads, head_dim, dtype, seed=11)
+    q = (torch.randn((len(lens), kv_heads * group, head_dim), generator=torch.Generator().manual_seed(3)) * 2).to(torch.float16)
+    scores = torch.zeros((1, len(lens), kv_heads, max(lens))).cuda()
+    attn = H.ScoredDecodeAttention(c.pool, q.cuda(), c.dev_tables, c.dev_lens, scores, max(lens))
+    for rep in range(20):                                            # back to back over one workspace
+        if rep == 19:
+            scores.zero_()
+        out = attn.enqueue(0)
+    assert int(attn.status.item()) == 0
+    for s, (want, w, vmax) in enumerate(c.attention(0, q, attn.sm_scale)):
+        out_close(out[s], want, vmax, False)
+        w = w.view(kv_heads, group, lens[s]).sum(dim=1)
+        scores_close(scores[0, s, :, : lens[s]], w, torch.zeros_like(w))
