@@ -43,6 +43,7 @@ __host__ __device__ constexpr int subs_of(bool fp8, bool f32) { return fp8 && !f
 __host__ __device__ constexpr int threads_of(bool fp8, bool f32) { return (WARPS * subs_of(fp8, f32) + 1) * 32; }   // and the producer
 constexpr int MAX_STAGES = 8;
 constexpr uint32_t PAD = 32;                 // bytes between runs of four tokens
+constexpr uint32_t SCALE_BYTES = 2 * WARPS * 4;
 constexpr uint32_t RING_BYTES = 208 * 1024;  // of all streams of a CTA
 constexpr uint32_t SEQ_CACHE = 1024;         // sequences whose ranges a CTA keeps in shared memory (more are looked up again)
 constexpr float RAISE = 6.0f;                // log2: probabilities reach 2^6, far inside F16
@@ -106,6 +107,11 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, const vo
 
 __device__ __forceinline__ void shared_read16(uint32_t at, uint32_t (&w)[4]) {
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
+}
+__device__ __forceinline__ float shared_read4(uint32_t at) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
+    return v;
 }
 __device__ __forceinline__ void shared_read8(uint32_t at, uint32_t (&w)[4]) {
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at));
@@ -204,7 +210,8 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
     if (tid < WARPS) {                                          // the streams' barriers; the last run of heads may be short
         const uint32_t hg = (blockIdx.x * a.streams + tid) % a.head_groups, n = min(a.heads, a.n_kv_heads - hg * a.heads);
         for (uint32_t i = 0; i < (uint32_t)MAX_STAGES; i++) {
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_addr(&full[tid][i])));
+            // the producer's own arrival and, for scales, one per lane when its copy has landed
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(&full[tid][i])), "r"(FP8 && a.k_scales ? 33u : 1u));
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(&empty[tid][i])), "r"(n));
         }
         if (tid == 0) fail = 0;
@@ -267,13 +274,15 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
         x.len = r.y;
         x.rest -= x.left;
     };
-    auto block_id = [&](const Cursor& x, uint32_t i) -> uint32_t {
-        const uint32_t id = __ldg(a.tables + (size_t)x.seq * a.table_stride + x.block + i);
+    // a table entry; it is checked where it is used, a few blocks later, so that nothing waits for the load here
+    auto table_entry = [&](const Cursor& x, uint32_t i) -> uint32_t { return __ldg(a.tables + (size_t)x.seq * a.table_stride + x.block + i); };
+    auto checked = [&](uint32_t id) -> uint32_t {
         if (id < a.total_blocks) return id;
         report(a.status, 2u);                                   // never dereferenced: block 0 is read instead and the launch reports it
         return 0u;
     };
-    const uint32_t row_smem = a.heads * S::ROW, run_smem = 4 * row_smem + PAD, plane = 4 * run_smem, stage_bytes = 2 * plane;
+    const uint32_t row_smem = a.heads * S::ROW, run_smem = 4 * row_smem + PAD, plane = 4 * run_smem;
+    const uint32_t stage_bytes = 2 * plane + (FP8 ? SCALE_BYTES : 0);    // K, V, scales of K and of V per head
 
     if (warp == NWARPS - 1) {
         // ---- producer: the streams in step, block k of each; lane x keeps the place in stream x.  A run of tokens is one copy where the
@@ -289,7 +298,7 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
             for (int u = 0; u < 4; u++) {
                 ids[u] = lives[u] = 0;
                 if (!done) {
-                    ids[u] = block_id(f, 0);
+                    ids[u] = table_entry(f, 0);
                     lives[u] = min((uint32_t)BS, f.len - f.block * BS);
                     f.block++;
                     if (--f.left == 0) {
@@ -306,6 +315,8 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
         const bool copies = row % per_copy == 0;
         const char* base = ((lane >> 4) ? a.v_base : a.k_base) + (size_t)row * a.row_stride;
         const uint32_t dst0 = smem_addr(ring) + (lane >> 4) * plane + (row >> 2) * run_smem + (row & 3u) * row_smem;
+        uint64_t policy;                                        // read once: the scores and partial results are what L2 should keep
+        asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
         uint32_t issued = 0;                                    // lane x: blocks of stream x asked for
         uint32_t slot = 0, phase = 1;                           // phase of `empty` that block k waits for; the first round waits for nothing
         bool ok = true;
@@ -315,7 +326,7 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
             for (int u = 0; u < 4; u++) {
                 if (k0 + u < n_max && ok) {
                     for (uint32_t x = 0; x < a.streams; x++) {
-                        const uint32_t block = __shfl_sync(0xFFFFFFFFu, id[u], x), rows = __shfl_sync(0xFFFFFFFFu, live[u], x);
+                        const uint32_t entry = __shfl_sync(0xFFFFFFFFu, id[u], x), rows = __shfl_sync(0xFFFFFFFFu, live[u], x);
                         const uint32_t hg = __shfl_sync(0xFFFFFFFFu, hg_l, x);
                         if (rows == 0 || !ok) continue;         // this stream has ended
                         if (k0 + u >= a.stages) ok = bar_wait(smem_addr(&empty[x][slot]), phase, &fail);
@@ -325,12 +336,21 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
                         if (lane == 0)
                             asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(2u * rows * bytes) : "memory");
                         __syncwarp();
+                        const uint32_t block = checked(entry);
                         if (lane == x) issued++;
+                        const uint32_t stage = (x * a.stages + slot) * stage_bytes;
+                        if (FP8 && a.k_scales) {                // 4-byte copies that arrive on the same barrier
+                            const uint32_t head = hg * a.heads + row;
+                            if (row < a.heads && head < a.n_kv_heads)
+                                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(ring) + stage + 2 * plane + ((lane >> 4) * WARPS + row) * 4),
+                                             "l"(((lane >> 4) ? a.v_scales : a.k_scales) + (size_t)block * a.n_kv_heads + head) : "memory");
+                            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+                        }
                         if (copies && row < rows)
-                            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                                         ::"r"(dst0 + (x * a.stages + slot) * stage_bytes),
+                            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
+                                         ::"r"(dst0 + stage),
                                          "l"(base + (uint64_t)block * a.block_stride + (size_t)hg * a.heads * S::ROW), "r"(bytes * min(per_copy, rows - row)),
-                                         "r"(bar) : "memory");
+                                         "r"(bar), "l"(policy) : "memory");
                     }
                     if (++slot == a.stages) {
                         slot = 0;
@@ -348,6 +368,7 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
             atomicCAS(&fail, 0u, 4u);
             report(a.status, 4u);
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         // Whatever happens to the consumers, no copy is in flight when the CTA's shared memory goes: the last copy into every stage is waited for.
         for (uint32_t x = 0; x < a.streams; x++) {
             const uint32_t n = __shfl_sync(0xFFFFFFFFu, issued, x);
@@ -370,30 +391,14 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
     const uint32_t run_k = (grp & 1u) ? (grp >> 1) ^ 2u : grp >> 1, tok_k = 4 * run_k + (grp & 1u);   // tokens of MMA rows grp, grp + 8: tok_k, tok_k + 2
     const uint32_t tok_v0 = 4 * j, tok_v1 = 4 * (j ^ 2u) + 1;   // of k indices 2j, 2j + 1; of 2j + 8, 2j + 9: two more
 
-    // block scales: lane i holds those of block i of the batch at hand; the next batch's loads are already under way
     const bool scaled = FP8 && a.k_scales != nullptr;
-    float ks_l = 1.0f, vs_l = 1.0f, ks_n = 1.0f, vs_n = 1.0f;
-    uint32_t next_n = 0;
-    Cursor look = c;
-    auto look_ahead = [&]() {                                   // loads the scales of up to 32 blocks at `look`, which moves on
-        next_n = min(look.left, 32u);
-        if (lane < next_n) {
-            const size_t at = (size_t)block_id(look, lane) * a.n_kv_heads + kvh;
-            ks_n = __ldg(a.k_scales + at);
-            vs_n = __ldg(a.v_scales + at);
-        }
-        look.block += next_n;
-        look.left -= next_n;
-        if (look.left == 0 && look.rest) next_sequence(look);
-    };
-    if (scaled) look_ahead();
-
     uint32_t slot = sub, phase = 0;                             // ring stage of this consumer's next block
     uint32_t turn = sub;                                        // blocks until it, counted from c.block
     const uint32_t ring_base = smem_addr(ring) + x_stream * a.stages * stage_bytes;
     const uint32_t k_off = ring_base + h * S::ROW + run_k * run_smem + (grp & 1u) * row_smem + j * 16, half = 2 * row_smem;
     const uint32_t v_off = ring_base + plane + h * S::ROW + grp * S::VPB;
     const uint32_t v_at0 = v_off + j * run_smem, v_at1 = v_off + (j ^ 2u) * run_smem + row_smem;
+    const uint32_t sc_off = ring_base + 2 * plane + 4 * h;
     const bool col0 = 2 * j < a.group, col1 = 2 * j + 1 < a.group;
 
     for (;;) {                                                  // the sequences of this part
@@ -426,15 +431,6 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
         float v_ref = FP8 ? 0x1p-100f : 1.0f, v_inv = FP8 ? 0x1p+100f : 1.0f;   // a power of two above every V scale met so far: O is in units of
                                                                 // it, and P x scale / v_ref stays in F16's range
         float* lg = a.logits ? a.logits + ((size_t)c.seq * a.n_q_heads + kvh * a.group + 2 * j) * a.logit_stride + c.block * BS + tok_k : nullptr;
-        uint32_t batch_at = 0, batch_n = 0;                     // blocks [batch_at, batch_at + batch_n) of this sequence: the scales at hand
-        auto next_batch = [&]() {
-            ks_l = ks_n;
-            vs_l = vs_n;
-            batch_at += batch_n;
-            batch_n = next_n;
-            if (look.left) look_ahead();
-            else next_n = 0;
-        };
         const uint32_t n = c.left;
         for (; turn < n; turn += STEP) {
             if (!bar_wait(smem_addr(&full[x_stream][slot]), phase, &fail)) {
@@ -476,9 +472,8 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
             }
             float ks = a.scale_log2, vs = 1.0f;
             if (scaled) {
-                while (turn >= batch_at + batch_n) next_batch();
-                ks *= __shfl_sync(0xFFFFFFFFu, ks_l, turn - batch_at);
-                vs = __shfl_sync(0xFFFFFFFFu, vs_l, turn - batch_at);
+                ks *= shared_read4(stage + sc_off);
+                vs = shared_read4(stage + sc_off + 4 * WARPS);
             }
             float x[4];                                         // x[2 * (token half) + column]
 #pragma unroll
@@ -598,8 +593,6 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
             }
         }
         turn -= n;
-        if (scaled)
-            while (batch_at + batch_n < n) next_batch();        // blocks of this sequence that were the other consumer's
 
         // ---- partial results of (part, sequence); a consumer that had no block says so with an empty sum ----
         const size_t at_slot = ((size_t)part + c.seq) * STEP + sub;
@@ -661,7 +654,7 @@ template <int D, bool FP8, bool F32, bool WIDE> cudaError_t launch_one(Args a, c
     a.head_groups = sp.head_groups;
     a.parts = sp.parts;
     a.min_share = sp.min_share;
-    const uint32_t stage = 2 * (BS * sp.heads * S::ROW + 4 * PAD), fit = RING_BYTES / (sp.streams * stage);
+    const uint32_t stage = 2 * (BS * sp.heads * S::ROW + 4 * PAD) + (FP8 ? SCALE_BYTES : 0), fit = RING_BYTES / (sp.streams * stage);
     a.stages = (fit < (uint32_t)MAX_STAGES ? fit : (uint32_t)MAX_STAGES) / subs_of(FP8, F32) * subs_of(FP8, F32);   // at least 3 (eight heads of 128
                                                                                                     // F16 dims: 65 KB each), in pairs for pairs
     const size_t smem = (size_t)sp.streams * a.stages * stage;

@@ -33,41 +33,50 @@ struct FinishArgs {
     const uint32_t *plan, *kv_lens;
     float* scores;
     void* out;
-    uint32_t n_seqs, n_q_heads, n_kv_heads, group, logit_stride, score_stride, max_kv_len, tasks, subs;
+    uint32_t n_seqs, n_q_heads, n_kv_heads, group, logit_stride, score_stride, max_kv_len, tasks, subs, v4;
     float decay;
 };
 
 // One CTA per (sequence, kv head, task): the first `group` tasks join the partial results of one query head, the others turn the
-// scores of CHUNK tokens into weights.  Bound by L2 and launch: everything it reads was written just before.
-template <int D, bool F32> __global__ void __launch_bounds__(256) scored_finish(const FinishArgs a) {
+// scores of CHUNK tokens into weights, four tokens per thread.  Bound by L2 and launch: everything it reads was written just before,
+// so a thread asks for its scores before it joins the maxima and sums.  V4: rows of scores are 16-byte aligned.
+template <int D, bool F32, int G> __device__ __forceinline__ void finish_body(const FinishArgs& a, bool v4) {
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t task = blockIdx.x % a.tasks, row = blockIdx.x / a.tasks, kvh = row % a.n_kv_heads, s = row / a.n_kv_heads;
     const uint32_t len = min(a.kv_lens[s], a.max_kv_len);
-    const bool join = task < a.group;
-    const uint32_t t0 = join ? 0u : (task - a.group) * CHUNK;
-    if (!join && t0 >= len) return;
-    const float* x = a.logits + ((size_t)s * a.n_q_heads + kvh * a.group) * a.logit_stride;
-    float xs[CHUNK / 256][8];                // asked for before the partial results are joined: one latency instead of two
-    if (!join) {
+    const bool join = task < (uint32_t)G;
+    const uint32_t t = join ? 0u : (task - G) * CHUNK + 4 * tid;
+    if (!join && (task - G) * CHUNK >= len) return;
+    float4 x[G], old = make_float4(0, 0, 0, 0);
+    float* sc = a.scores + ((size_t)s * a.n_kv_heads + kvh) * a.score_stride + t;
+    if (!join && t < len) {                                     // rows of x are padded to 16 tokens: a float4 stays inside
+        const float* src = a.logits + ((size_t)s * a.n_q_heads + kvh * G) * a.logit_stride + t;
 #pragma unroll
-        for (int i = 0; i < CHUNK / 256; i++) {
-            const uint32_t t = t0 + i * 256 + tid;
-#pragma unroll
-            for (uint32_t g = 0; g < 8; g++) xs[i][g] = g < a.group && t < len ? x[(size_t)g * a.logit_stride + t] : -INFINITY;
+        for (int g = 0; g < G; g++) x[g] = *reinterpret_cast<const float4*>(src + (size_t)g * a.logit_stride);
+        if (a.decay != 0.0f) {
+            if (v4 && t + 4 <= len) {
+                old = *reinterpret_cast<const float4*>(sc);
+            } else {
+                old.x = sc[0];
+                if (t + 1 < len) old.y = sc[1];
+                if (t + 2 < len) old.z = sc[2];
+                if (t + 3 < len) old.w = sc[3];
+            }
         }
     }
     const uint32_t share = a.plan[0], lo = a.plan[1 + s], hi = a.plan[2 + s];
     const uint32_t p0 = hi > lo ? lo / share : 0u, n = hi > lo ? ((hi - 1) / share - p0 + 1) * a.subs : 0u;
-    const size_t first = (size_t)(p0 + s) * a.subs;     // partial results first .. first + n - 1
+    const size_t first = (size_t)(p0 + s) * a.subs;             // partial results first .. first + n - 1
+    const bool few = n <= 16;                                   // few partial results: the first task joins all heads, a warp each
+    if (join && few && task) return;
     __shared__ float top[8], inv[8];
-    if (warp < a.group && (!join || warp == task)) {            // warp g: maximum and sum of query head g
+    if (warp < (uint32_t)G && (!join || few || warp == task)) { // warp g: maximum and sum of query head g
         float m = -INFINITY, l = 0.0f;
-        const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + first * a.n_q_heads + kvh * a.group + warp;
+        const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + first * a.n_q_heads + kvh * G + warp;
         for (uint32_t i = lane; i < n; i += 32) {
             const float2 v = ml[(size_t)i * a.n_q_heads];
             const float mm = fmaxf(m, v.x);
-            if (mm != -INFINITY) l = l * exp2_fast(m - mm) + v.y * exp2_fast(v.x - mm);
-            else l += v.y;                                      // a part whose scores are all -inf or NaN says so in its sum
+            l = mm == -INFINITY ? l + v.y : l * exp2_fast(m - mm) + v.y * exp2_fast(v.x - mm);   // a part whose scores are all NaN says so in its sum
             m = mm;
         }
 #pragma unroll
@@ -88,18 +97,31 @@ template <int D, bool F32> __global__ void __launch_bounds__(256) scored_finish(
         float acc[PER];
 #pragma unroll
         for (int i = 0; i < PER; i++) acc[i] = 0.0f;
-        const float m = top[task];
-        for (uint32_t i = warp; i < n; i += 8) {
-            const size_t r = (first + i) * a.n_q_heads + kvh * a.group + task;
+        const uint32_t head = few ? warp : task;
+        if (head >= (uint32_t)G) return;
+        const float m = top[head];
+#pragma unroll 4
+        for (uint32_t i = few ? 0u : warp; i < n; i += few ? 1u : 8u) {
+            const size_t r = (first + i) * a.n_q_heads + kvh * G + head;
             const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + r * 2);
             float v[PER];
 #pragma unroll
             for (int k = 0; k < PER; k++) v[k] = a.part_o[r * D + k * 32 + lane];
             const float f = exp2_fast(ml.x - m);
-            if (ml.x != -INFINITY || ml.y != 0.0f) {            // an empty part's O was never written
+            if (ml.x != -INFINITY || ml.y != 0.0f) {            // an empty part's O counts for nothing
 #pragma unroll
-                for (int k = 0; k < PER; k++) acc[k] += f * v[k];
+                for (int k = 0; k < PER; k++) acc[k] = __fmaf_rn(f, v[k], acc[k]);
             }
+        }
+        const size_t at = ((size_t)s * a.n_q_heads + kvh * G + head) * D;
+        if (few) {
+#pragma unroll
+            for (int k = 0; k < PER; k++) {
+                const float v = acc[k] * inv[head];
+                if (F32) reinterpret_cast<float*>(a.out)[at + k * 32 + lane] = v;
+                else reinterpret_cast<__half*>(a.out)[at + k * 32 + lane] = __float2half_rn(v);
+            }
+            return;
         }
         __shared__ float part[8][D];
 #pragma unroll
@@ -109,24 +131,47 @@ template <int D, bool F32> __global__ void __launch_bounds__(256) scored_finish(
             float v = 0.0f;
 #pragma unroll
             for (int w = 0; w < 8; w++) v += part[w][tid];
-            v *= inv[task];
-            const size_t at = ((size_t)s * a.n_q_heads + kvh * a.group + task) * D + tid;
-            if (F32) reinterpret_cast<float*>(a.out)[at] = v;
-            else reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(v);
+            v *= inv[head];
+            if (F32) reinterpret_cast<float*>(a.out)[at + tid] = v;
+            else reinterpret_cast<__half*>(a.out)[at + tid] = __float2half_rn(v);
         }
-    } else {
-        float* sc = a.scores + ((size_t)s * a.n_kv_heads + kvh) * a.score_stride;
+    } else if (t < len) {
+        float4 w = make_float4(0, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < CHUNK / 256; i++) {
-            const uint32_t t = t0 + i * 256 + tid;
-            if (t < len) {
-                float w = 0.0f;
-#pragma unroll
-                for (uint32_t g = 0; g < 8; g++)
-                    if (g < a.group) w += exp2_fast(xs[i][g] - top[g]) * inv[g];
-                sc[t] = a.decay == 0.0f ? w : a.decay * sc[t] + w;
-            }
+        for (int g = 0; g < G; g++) {
+            const float m = top[g], f = inv[g];
+            w.x = __fmaf_rn(exp2_fast(x[g].x - m), f, w.x);
+            w.y = __fmaf_rn(exp2_fast(x[g].y - m), f, w.y);
+            w.z = __fmaf_rn(exp2_fast(x[g].z - m), f, w.z);
+            w.w = __fmaf_rn(exp2_fast(x[g].w - m), f, w.w);
         }
+        if (a.decay != 0.0f) {
+            w.x = __fmaf_rn(a.decay, old.x, w.x);
+            w.y = __fmaf_rn(a.decay, old.y, w.y);
+            w.z = __fmaf_rn(a.decay, old.z, w.z);
+            w.w = __fmaf_rn(a.decay, old.w, w.w);
+        }
+        if (v4 && t + 4 <= len) {
+            *reinterpret_cast<float4*>(sc) = w;
+        } else {
+            sc[0] = w.x;
+            if (t + 1 < len) sc[1] = w.y;
+            if (t + 2 < len) sc[2] = w.z;
+            if (t + 3 < len) sc[3] = w.w;
+        }
+    }
+}
+template <int D, bool F32> __global__ void __launch_bounds__(256) scored_finish(const FinishArgs a) {
+    const bool v4 = a.v4;
+    switch (a.group) {                                          // the group's scores of four tokens are registers: their number has to be known
+        case 1: return finish_body<D, F32, 1>(a, v4);
+        case 2: return finish_body<D, F32, 2>(a, v4);
+        case 3: return finish_body<D, F32, 3>(a, v4);
+        case 4: return finish_body<D, F32, 4>(a, v4);
+        case 5: return finish_body<D, F32, 5>(a, v4);
+        case 6: return finish_body<D, F32, 6>(a, v4);
+        case 7: return finish_body<D, F32, 7>(a, v4);
+        default: return finish_body<D, F32, 8>(a, v4);
     }
 }
 
@@ -247,6 +292,7 @@ int32_t tkv_scored_attn_enqueue(const TkvPool* pool, const TkvScoredAttn* p, voi
     f.score_stride = p->score_stride;
     f.max_kv_len = p->max_kv_len;
     f.tasks = tasks;
+    f.v4 = p->scores % 16 == 0 && p->score_stride % 4 == 0;
     f.subs = tkv_rows::subs_of(es == 1, p->q_dtype == TKV_DTYPE_F32);
     f.decay = p->decay;
 
