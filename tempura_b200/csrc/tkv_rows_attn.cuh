@@ -34,6 +34,8 @@
 
 #include <stdint.h>
 
+#include <atomic>
+
 namespace tkv_rows {
 
 constexpr int BS = 16;                       // tokens per block
@@ -281,6 +283,7 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
         report(a.status, 2u);                                   // never dereferenced: block 0 is read instead and the launch reports it
         return 0u;
     };
+    asm volatile("griddepcontrol.launch_dependents;");          // the joining kernel may take its place; it waits for this grid's end by itself
     const uint32_t row_smem = a.heads * S::ROW, run_smem = 4 * row_smem + PAD, plane = 4 * run_smem;
     const uint32_t stage_bytes = 2 * plane + (FP8 ? SCALE_BYTES : 0);    // K, V, scales of K and of V per head
 
@@ -659,8 +662,16 @@ template <int D, bool FP8, bool F32, bool WIDE> cudaError_t launch_one(Args a, c
                                                                                                     // F16 dims: 65 KB each), in pairs for pairs
     const size_t smem = (size_t)sp.streams * a.stages * stage;
     auto kernel = rows_attn<D, FP8, F32, WIDE>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RING_BYTES);
+    static std::atomic<uint64_t> granted{0};                    // devices on which this kernel may use the ring's shared memory
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
+    if (!(granted.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RING_BYTES);
+        if (e != cudaSuccess) return e;
+        granted.fetch_or(bit, std::memory_order_relaxed);
+    }
     kernel<<<sp.grid, threads_of(FP8, F32), smem, st>>>(a);
     return cudaGetLastError();
 }

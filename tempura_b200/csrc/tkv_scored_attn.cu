@@ -10,6 +10,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <stdint.h>
@@ -26,7 +27,6 @@ namespace {
 using tkv_rows::exp2_fast;
 
 constexpr uint32_t CTAS = 148;               // one per SM of the part this is built for; partial results are sized by it
-constexpr int CHUNK = 1024;                  // tokens per CTA of the second kernel
 
 struct FinishArgs {
     const float *part_o, *part_ml, *logits;
@@ -37,47 +37,67 @@ struct FinishArgs {
     float decay;
 };
 
-// One CTA per (sequence, kv head, task): the first `group` tasks join the partial results of one query head, the others turn the
-// scores of CHUNK tokens into weights, four tokens per thread.  Bound by L2 and launch: everything it reads was written just before,
-// so a thread asks for its scores before it joins the maxima and sums.  V4: rows of scores are 16-byte aligned.
-template <int D, bool F32, int G> __device__ __forceinline__ void finish_body(const FinishArgs& a, bool v4) {
+// Tokens per thread of the second kernel: their scores of all G query heads wait in registers.
+__host__ __device__ constexpr int tokens_of(int g) { return g > 4 ? 2 : 4; }
+
+// One CTA per (sequence, kv head, task): the first G tasks join the partial results of one query head each (the first one those of all
+// heads, a warp each, when they are few), the others turn the scores of 256 x TOK tokens into weights.  Bound by latency and L2:
+// everything it reads was written just before, so a thread asks for its scores before it joins the maxima and sums, and asks
+// for all of those at once.  V: rows of scores are aligned to a thread's tokens.
+template <int D, bool F32, int G> __global__ void __launch_bounds__(256) scored_finish(const FinishArgs a) {
+    constexpr int TOK = tokens_of(G);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t task = blockIdx.x % a.tasks, row = blockIdx.x / a.tasks, kvh = row % a.n_kv_heads, s = row / a.n_kv_heads;
-    const uint32_t len = min(a.kv_lens[s], a.max_kv_len);
     const bool join = task < (uint32_t)G;
-    const uint32_t t = join ? 0u : (task - G) * CHUNK + 4 * tid;
-    if (!join && (task - G) * CHUNK >= len) return;
-    float4 x[G], old = make_float4(0, 0, 0, 0);
-    float* sc = a.scores + ((size_t)s * a.n_kv_heads + kvh) * a.score_stride + t;
-    if (!join && t < len) {                                     // rows of x are padded to 16 tokens: a float4 stays inside
-        const float* src = a.logits + ((size_t)s * a.n_q_heads + kvh * G) * a.logit_stride + t;
+    constexpr uint32_t RUN = 256 * TOK;
+    const uint32_t skip = (a.tasks - G) * RUN;
+    uint32_t t0 = join ? 0u : (task - G) * RUN;
+    asm volatile("griddepcontrol.wait;" ::: "memory");          // launched ahead of the first kernel's end
+    const uint32_t len = min(a.kv_lens[s], a.max_kv_len);
+    const uint32_t share = a.plan[0], lo = a.plan[1 + s], hi = a.plan[2 + s];
+    const float* src = a.logits + ((size_t)s * a.n_q_heads + kvh * G) * a.logit_stride + TOK * tid;
+    auto read = [&](float (&x)[G][TOK], uint32_t at) {          // rows of x are padded to 16 tokens: a vector stays inside; what lies behind len is not used
+        if (at + TOK * tid < a.logit_stride) {
 #pragma unroll
-        for (int g = 0; g < G; g++) x[g] = *reinterpret_cast<const float4*>(src + (size_t)g * a.logit_stride);
-        if (a.decay != 0.0f) {
-            if (v4 && t + 4 <= len) {
-                old = *reinterpret_cast<const float4*>(sc);
-            } else {
-                old.x = sc[0];
-                if (t + 1 < len) old.y = sc[1];
-                if (t + 2 < len) old.z = sc[2];
-                if (t + 3 < len) old.w = sc[3];
+            for (int g = 0; g < G; g++) {
+                if (TOK == 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(src + (size_t)g * a.logit_stride + at);
+                    x[g][0] = v.x;
+                    x[g][1] = v.y;
+                    x[g][TOK - 2] = v.z;
+                    x[g][TOK - 1] = v.w;
+                } else {
+                    const float2 v = *reinterpret_cast<const float2*>(src + (size_t)g * a.logit_stride + at);
+                    x[g][0] = v.x;
+                    x[g][1] = v.y;
+                }
             }
         }
-    }
-    const uint32_t share = a.plan[0], lo = a.plan[1 + s], hi = a.plan[2 + s];
+    };
+    float x[G][TOK];
+    if (!join) read(x, t0);
+    if (!join && t0 >= len) return;
     const uint32_t p0 = hi > lo ? lo / share : 0u, n = hi > lo ? ((hi - 1) / share - p0 + 1) * a.subs : 0u;
     const size_t first = (size_t)(p0 + s) * a.subs;             // partial results first .. first + n - 1
-    const bool few = n <= 16;                                   // few partial results: the first task joins all heads, a warp each
+    const bool few = n <= 16;
     if (join && few && task) return;
     __shared__ float top[8], inv[8];
     if (warp < (uint32_t)G && (!join || few || warp == task)) { // warp g: maximum and sum of query head g
         float m = -INFINITY, l = 0.0f;
         const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + first * a.n_q_heads + kvh * G + warp;
-        for (uint32_t i = lane; i < n; i += 32) {
-            const float2 v = ml[(size_t)i * a.n_q_heads];
-            const float mm = fmaxf(m, v.x);
-            l = mm == -INFINITY ? l + v.y : l * exp2_fast(m - mm) + v.y * exp2_fast(v.x - mm);   // a part whose scores are all NaN says so in its sum
-            m = mm;
+        for (uint32_t i0 = 0; i0 < n; i0 += 256) {
+            float2 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const uint32_t i = i0 + 32 * k + lane;
+                v[k] = i < n ? ml[(size_t)i * a.n_q_heads] : make_float2(-INFINITY, 0.0f);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float mm = fmaxf(m, v[k].x);
+                l = mm == -INFINITY ? l + v[k].y : l * exp2_fast(m - mm) + v[k].y * exp2_fast(v[k].x - mm);   // scores all NaN: the sum says so
+                m = mm;
+            }
         }
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) {
@@ -100,18 +120,17 @@ template <int D, bool F32, int G> __device__ __forceinline__ void finish_body(co
         const uint32_t head = few ? warp : task;
         if (head >= (uint32_t)G) return;
         const float m = top[head];
-#pragma unroll 4
-        for (uint32_t i = few ? 0u : warp; i < n; i += few ? 1u : 8u) {
+        const uint32_t step = few ? 1u : 8u;
+#pragma unroll 8
+        for (uint32_t i = few ? 0u : warp; i < n; i += step) {
             const size_t r = (first + i) * a.n_q_heads + kvh * G + head;
             const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + r * 2);
             float v[PER];
 #pragma unroll
             for (int k = 0; k < PER; k++) v[k] = a.part_o[r * D + k * 32 + lane];
             const float f = exp2_fast(ml.x - m);
-            if (ml.x != -INFINITY || ml.y != 0.0f) {            // an empty part's O counts for nothing
 #pragma unroll
-                for (int k = 0; k < PER; k++) acc[k] = __fmaf_rn(f, v[k], acc[k]);
-            }
+            for (int k = 0; k < PER; k++) acc[k] = ml.x != -INFINITY || ml.y != 0.0f ? __fmaf_rn(f, v[k], acc[k]) : acc[k];   // an empty part's O counts for nothing
         }
         const size_t at = ((size_t)s * a.n_q_heads + kvh * G + head) * D;
         if (few) {
@@ -130,48 +149,66 @@ template <int D, bool F32, int G> __device__ __forceinline__ void finish_body(co
         if (tid < D) {
             float v = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 8; w++) v += part[w][tid];
+            for (int w8 = 0; w8 < 8; w8++) v += part[w8][tid];
             v *= inv[head];
             if (F32) reinterpret_cast<float*>(a.out)[at + tid] = v;
             else reinterpret_cast<__half*>(a.out)[at + tid] = __float2half_rn(v);
         }
-    } else if (t < len) {
-        float4 w = make_float4(0, 0, 0, 0);
+    } else {
+        float* sc = a.scores + ((size_t)s * a.n_kv_heads + kvh) * a.score_stride + TOK * tid;
+        for (;; t0 += skip) {
+            const uint32_t t = t0 + TOK * tid;
+            float w[TOK], y[G][TOK];
 #pragma unroll
-        for (int g = 0; g < G; g++) {
-            const float m = top[g], f = inv[g];
-            w.x = __fmaf_rn(exp2_fast(x[g].x - m), f, w.x);
-            w.y = __fmaf_rn(exp2_fast(x[g].y - m), f, w.y);
-            w.z = __fmaf_rn(exp2_fast(x[g].z - m), f, w.z);
-            w.w = __fmaf_rn(exp2_fast(x[g].w - m), f, w.w);
-        }
-        if (a.decay != 0.0f) {
-            w.x = __fmaf_rn(a.decay, old.x, w.x);
-            w.y = __fmaf_rn(a.decay, old.y, w.y);
-            w.z = __fmaf_rn(a.decay, old.z, w.z);
-            w.w = __fmaf_rn(a.decay, old.w, w.w);
-        }
-        if (v4 && t + 4 <= len) {
-            *reinterpret_cast<float4*>(sc) = w;
-        } else {
-            sc[0] = w.x;
-            if (t + 1 < len) sc[1] = w.y;
-            if (t + 2 < len) sc[2] = w.z;
-            if (t + 3 < len) sc[3] = w.w;
+            for (int i = 0; i < TOK; i++) w[i] = a.decay != 0.0f && t + i < len ? a.decay * sc[t0 + i] : 0.0f;
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+                for (int i = 0; i < TOK; i++) y[g][i] = x[g][i];
+            const bool more = t0 + skip < len;
+            if (more) read(x, t0 + skip);                       // the next run's, under this run's arithmetic
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                const float m = top[g], f = inv[g];
+#pragma unroll
+                for (int i = 0; i < TOK; i++) w[i] = __fmaf_rn(exp2_fast(y[g][i] - m), f, w[i]);
+            }
+            if (a.v4 && t + TOK <= len) {
+                if (TOK == 4) *reinterpret_cast<float4*>(sc + t0) = make_float4(w[0], w[1], w[TOK - 2], w[TOK - 1]);
+                else *reinterpret_cast<float2*>(sc + t0) = make_float2(w[0], w[1]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < TOK; i++)
+                    if (t + i < len) sc[t0 + i] = w[i];
+            }
+            if (!more) break;
         }
     }
 }
-template <int D, bool F32> __global__ void __launch_bounds__(256) scored_finish(const FinishArgs a) {
-    const bool v4 = a.v4;
-    switch (a.group) {                                          // the group's scores of four tokens are registers: their number has to be known
-        case 1: return finish_body<D, F32, 1>(a, v4);
-        case 2: return finish_body<D, F32, 2>(a, v4);
-        case 3: return finish_body<D, F32, 3>(a, v4);
-        case 4: return finish_body<D, F32, 4>(a, v4);
-        case 5: return finish_body<D, F32, 5>(a, v4);
-        case 6: return finish_body<D, F32, 6>(a, v4);
-        case 7: return finish_body<D, F32, 7>(a, v4);
-        default: return finish_body<D, F32, 8>(a, v4);
+
+template <int D, bool F32, int G> cudaError_t launch_finish_g(const FinishArgs& a, unsigned grid, cudaStream_t st) {
+    // The launch does not wait for the first kernel's end (the kernel itself does): its CTAs are in place when the last partial result is written.
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, scored_finish<D, F32, G>, a);
+}
+template <int D, bool F32> cudaError_t launch_finish(const FinishArgs& a, unsigned grid, cudaStream_t st) {
+    switch (a.group) {
+        case 1: return launch_finish_g<D, F32, 1>(a, grid, st);
+        case 2: return launch_finish_g<D, F32, 2>(a, grid, st);
+        case 3: return launch_finish_g<D, F32, 3>(a, grid, st);
+        case 4: return launch_finish_g<D, F32, 4>(a, grid, st);
+        case 5: return launch_finish_g<D, F32, 5>(a, grid, st);
+        case 6: return launch_finish_g<D, F32, 6>(a, grid, st);
+        case 7: return launch_finish_g<D, F32, 7>(a, grid, st);
+        default: return launch_finish_g<D, F32, 8>(a, grid, st);
     }
 }
 
@@ -246,8 +283,11 @@ int32_t tkv_scored_attn_enqueue(const TkvPool* pool, const TkvScoredAttn* p, voi
     const Layout l = layout_of(p->n_seqs, p->n_q_heads, pool->n_kv_heads, pool->head_dim, p->max_kv_len);
     if (!p->scratch || p->scratch_bytes < l.bytes)
         return fail(TKV_ERR_DIMENSION_MISMATCH, "dimension mismatch: expected %llu, got %llu (scratch bytes)", l.bytes, p->scratch ? p->scratch_bytes : 0);
-    const uint32_t group = p->n_q_heads / pool->n_kv_heads, tasks = group + (p->max_kv_len + CHUNK - 1) / CHUNK;
-    const uint64_t finish_grid = (uint64_t)p->n_seqs * pool->n_kv_heads * tasks;
+    const uint32_t group = p->n_q_heads / pool->n_kv_heads, run = 256 * tokens_of((int)group), runs = (p->max_kv_len + run - 1) / run;
+    // four CTAs per SM turn scores into weights where there are rows and runs for them
+    const uint64_t rows = (uint64_t)p->n_seqs * pool->n_kv_heads;
+    const uint32_t per_row = (uint32_t)std::min<uint64_t>(runs, std::max<uint64_t>(4ull * CTAS / rows, 1ull)), tasks = group + per_row;
+    const uint64_t finish_grid = rows * tasks;
     if (finish_grid > 0x7FFFFFFFull) return fail(TKV_ERR_INVALID_CONFIG, "%llu sequences of %llu tokens: batch too large", p->n_seqs, p->max_kv_len);
 
     tkv_rows::Args a{};
@@ -305,14 +345,8 @@ int32_t tkv_scored_attn_enqueue(const TkvPool* pool, const TkvScoredAttn* p, voi
         e = tkv_rows::launch_rows(pool->head_dim, es == 1, f32, a, l.split, st);
         if (e == cudaSuccess) {
             const unsigned grid = (unsigned)finish_grid;
-            if (pool->head_dim == 128) {
-                if (f32) scored_finish<128, true><<<grid, 256, 0, st>>>(f);
-                else scored_finish<128, false><<<grid, 256, 0, st>>>(f);
-            } else {
-                if (f32) scored_finish<64, true><<<grid, 256, 0, st>>>(f);
-                else scored_finish<64, false><<<grid, 256, 0, st>>>(f);
-            }
-            e = cudaGetLastError();
+            if (pool->head_dim == 128) e = f32 ? launch_finish<128, true>(f, grid, st) : launch_finish<128, false>(f, grid, st);
+            else e = f32 ? launch_finish<64, true>(f, grid, st) : launch_finish<64, false>(f, grid, st);
         }
     }
     if (prev >= 0 && prev != pool->device) cudaSetDevice(prev);
