@@ -442,6 +442,50 @@ typedef struct TkvScoredAttn {
 uint64_t tkv_scored_attn_scratch_bytes(uint32_t n_seqs, uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t max_kv_len);
 int32_t tkv_scored_attn_enqueue(const TkvPool* pool, const TkvScoredAttn* args, void* stream);
 
+/* Eviction: cutting every sequence of a batch to a budget by accumulated attention weight (tkv_scored_attn_enqueue), in two calls.
+ * No counterpart in the reference.
+ * Select: for each (layer, sequence, kv head) row of scores over len = kv_lens[s] tokens, which tokens stay.  The first protect[s]
+ * (a prefix shared with other sequences, attention sinks), the last `recent`, and the highest scores of the others, ties to the
+ * lower index, NaN below every number:
+ *     new_lens[s] = min(len, max(budget, protect[s] + recent));   kept = their indices in ascending order, new_lens[s] of them.
+ * Entries of kept behind new_lens[s] are left alone.  The same number stays in every layer and head, so one length serves all.        */
+typedef struct TkvEvictSelect {
+    int32_t device;               /* CUDA ordinal that owns the memory                                              */
+    uint32_t n_layers, n_seqs, n_kv_heads;
+    uint32_t max_kv_len;          /* bounds kv_lens                                                                 */
+    uint32_t score_stride;        /* floats from one row of scores to the next; at least max_kv_len                 */
+    uint32_t kept_stride;         /* entries from one row of kept to the next; at least budget and recent (unless they are
+                                     max_kv_len or more), and protect[s] + recent of every sequence that is cut; a
+                                     sequence that is not cut gets its indices as far as they fit                    */
+    uint32_t budget, recent, reserved;
+    uint64_t scores;              /* f32 [n_layers][n_seqs][n_kv_heads][score_stride]                               */
+    uint64_t kv_lens;             /* u32 [n_seqs]                                                                   */
+    uint64_t protect;             /* u32 [n_seqs], or 0: nothing protected                                          */
+    uint64_t kept;                /* u32 [n_layers][n_seqs][n_kv_heads][kept_stride]                                */
+    uint64_t new_lens;            /* u32 [n_seqs]                                                                   */
+    uint64_t status;              /* 0, or a device u32 (zero it before the launch): TKV_ERR_INVALID_CONFIG if kv_lens held a value
+                                     above max_kv_len (clamped to it) or kept is too narrow for a sequence, which then is not cut */
+} TkvEvictSelect;
+int32_t tkv_evict_select_enqueue(const TkvEvictSelect* args, void* stream);
+/* Compact: row j of every (layer, sequence, kv head) becomes the row that kept[j] names, for K, V and (if given) scores, in place
+ * through the block tables; scores from new_lens[s] to kv_lens[s] become 0.  Sequences with new_lens[s] == kv_lens[s] and rows with
+ * kept[j] == j are not touched.  Afterwards the caller makes new_lens the lengths and may return the blocks behind them
+ * (tkv_device_page_allocator_free with first = ceil(new_lens / 16), seq_lens = the old lengths).  A block that other
+ * sequences use as well has to lie below protect[s] at selection.  An E4M3 pool with scales: a block's scale becomes the largest of
+ * its new rows' scales; rows that had another one are rounded to E4M3 again at the new scale.  F16 or E4M3 pool, 16-token
+ * blocks, head_dim 64 or 128.                                                                                       */
+typedef struct TkvEvictCompact {
+    uint32_t layer_begin, n_layers, n_seqs, table_stride, max_kv_len, score_stride, kept_stride, reserved;
+    uint64_t tables;              /* u32 [n_seqs][table_stride] block ids                                           */
+    uint64_t kv_lens;             /* u32 [n_seqs] lengths before                                                    */
+    uint64_t kept;                /* u32 [n_layers][n_seqs][n_kv_heads][kept_stride], ascending; kept[j] >= j        */
+    uint64_t new_lens;            /* u32 [n_seqs]                                                                   */
+    uint64_t scores;              /* f32 [n_layers][n_seqs][n_kv_heads][score_stride], or 0                         */
+    uint64_t status;              /* 0, or a device u32: TKV_ERR_INVALID_CONFIG if a length exceeded its bound, kept named a row outside
+                                     the sequence or below its place (that row stays), or a table entry a block outside the pool */
+} TkvEvictCompact;
+int32_t tkv_evict_compact_enqueue(const TkvPool* pool, const TkvEvictCompact* args, void* stream);
+
 /* Device self-check of the tcgen05 path's operand plumbing (tensor-map copy with the 128-byte swizzle,
  * shared-memory and instruction descriptors, tensor-memory reads) on operands of small dyadic values whose
  * products and sums are exact: mismatches[0..3] count wrong accumulators for E4M3 K-major, E4M3 x E5M2

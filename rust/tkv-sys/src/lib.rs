@@ -229,6 +229,46 @@ pub struct TkvScoredAttn {
 
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
+pub struct TkvEvictSelect {
+    pub device: i32,
+    pub n_layers: u32,
+    pub n_seqs: u32,
+    pub n_kv_heads: u32,
+    pub max_kv_len: u32,
+    pub score_stride: u32,
+    pub kept_stride: u32,
+    pub budget: u32,
+    pub recent: u32,
+    pub reserved: u32,
+    pub scores: u64,
+    pub kv_lens: u64,
+    pub protect: u64,
+    pub kept: u64,
+    pub new_lens: u64,
+    pub status: u64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct TkvEvictCompact {
+    pub layer_begin: u32,
+    pub n_layers: u32,
+    pub n_seqs: u32,
+    pub table_stride: u32,
+    pub max_kv_len: u32,
+    pub score_stride: u32,
+    pub kept_stride: u32,
+    pub reserved: u32,
+    pub tables: u64,
+    pub kv_lens: u64,
+    pub kept: u64,
+    pub new_lens: u64,
+    pub scores: u64,
+    pub status: u64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
 pub struct TkvSessionHeader {
     pub position: u64,
     pub seed: u64,
@@ -388,6 +428,8 @@ extern "C" {
     pub fn tkv_prefill_attn_enqueue(pool: *const TkvPool, args: *const TkvPrefillAttn, stream: *mut c_void) -> i32;
     pub fn tkv_scored_attn_scratch_bytes(n_seqs: u32, n_q_heads: u32, n_kv_heads: u32, head_dim: u32, max_kv_len: u32) -> u64;
     pub fn tkv_scored_attn_enqueue(pool: *const TkvPool, args: *const TkvScoredAttn, stream: *mut c_void) -> i32;
+    pub fn tkv_evict_select_enqueue(args: *const TkvEvictSelect, stream: *mut c_void) -> i32;
+    pub fn tkv_evict_compact_enqueue(pool: *const TkvPool, args: *const TkvEvictCompact, stream: *mut c_void) -> i32;
     pub fn tkv_selfcheck_tensor_cores(mismatches: *mut u64) -> i32;
     pub fn tkv_session_wire_size(h: *const TkvSessionHeader) -> usize;
     pub fn tkv_session_pack(h: *const TkvSessionHeader, blocks: *const u32, logits: *const f32, out: *mut u8, cap: usize, written: *mut usize) -> i32;

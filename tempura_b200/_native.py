@@ -69,6 +69,17 @@ class TkvScoredAttn(C.Structure):
         (n, C.c_uint64) for n in ("q", "out", "tables", "kv_lens", "scores", "scratch", "scratch_bytes", "status")]
 
 
+class TkvEvictSelect(C.Structure):
+    _fields_ = [("device", C.c_int32)] + [(n, C.c_uint32) for n in (
+        "n_layers", "n_seqs", "n_kv_heads", "max_kv_len", "score_stride", "kept_stride", "budget", "recent", "reserved")] + [
+        (n, C.c_uint64) for n in ("scores", "kv_lens", "protect", "kept", "new_lens", "status")]
+
+
+class TkvEvictCompact(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("layer_begin", "n_layers", "n_seqs", "table_stride", "max_kv_len", "score_stride", "kept_stride",
+                                          "reserved")] + [(n, C.c_uint64) for n in ("tables", "kv_lens", "kept", "new_lens", "scores", "status")]
+
+
 class TkvPrefixBatch(C.Structure):
     _fields_ = [(n, C.c_uint32) for n in ("n_seqs", "stride", "page_stride", "reserved")] + [
         (n, C.c_uint64) for n in ("tokens", "lens", "pages", "page_lens")]
@@ -174,6 +185,8 @@ SIGNATURES = {
     "tkv_decode_attn_enqueue": (_i32, [C.POINTER(TkvPool), C.POINTER(TkvDecodeAttn), _vp]),
     "tkv_scored_attn_scratch_bytes": (_u64, [_u32, _u32, _u32, _u32, _u32]),
     "tkv_scored_attn_enqueue": (_i32, [C.POINTER(TkvPool), C.POINTER(TkvScoredAttn), _vp]),
+    "tkv_evict_select_enqueue": (_i32, [C.POINTER(TkvEvictSelect), _vp]),
+    "tkv_evict_compact_enqueue": (_i32, [C.POINTER(TkvPool), C.POINTER(TkvEvictCompact), _vp]),
     "tkv_selfcheck_tensor_cores": (_i32, [_u64p]),
     "tkv_session_wire_size": (_sz, [C.POINTER(TkvSessionHeader)]),
     "tkv_session_pack": (_i32, [C.POINTER(TkvSessionHeader), _u32p, C.POINTER(C.c_float), _u8p, _sz, _szp]),

@@ -494,6 +494,71 @@ class ScoredDecodeAttention:
         return self.out
 
 
+class CacheEviction:
+    """Cuts the sequences of a batch to ``budget`` cached tokens by their accumulated attention weights
+    (:class:`ScoredDecodeAttention`).  ``select`` chooses, per layer, sequence and kv head, the tokens that stay -- the first
+    ``protect[s]``, the last ``recent`` and the best-scored others, ``min(len, max(budget, protect[s] + recent))`` in all -- into
+    ``kept`` (ascending indices) and ``new_lens``; ``compact`` moves their K, V and score rows to the front of the sequence's blocks,
+    in place.  ``evict`` does both and makes ``new_lens`` the batch's ``kv_lens``.  Blocks behind the new length can then go back:
+    ``DevicePageAllocator.free(tables, first=ceil(new_lens / 16), seq_lens=old_lens)``.
+
+    ``scores`` is f32 ``[n_layers, n_seqs, n_kv_heads, score_stride]``, ``kv_lens`` int32 ``[n_seqs]`` (at most ``score_stride``),
+    ``tables`` int32 ``[n_seqs, table_stride]``, ``protect`` int32 ``[n_seqs]`` or None.  A prefix that other sequences share has to
+    be protected.  ``kept`` int32 ``[n_layers, n_seqs, n_kv_heads, n]`` and ``new_lens`` are made here unless given; a sequence whose
+    protected and recent tokens exceed both ``budget`` and ``n`` is not cut and sets ``status``.  ``pool`` and ``tables`` may be None
+    for ``select`` alone."""
+
+    def __init__(self, pool: Optional[Pool], tables: Optional[torch.Tensor], kv_lens: torch.Tensor, scores: torch.Tensor, budget: int, recent: int,
+                 protect: Optional[torch.Tensor] = None, kept: Optional[torch.Tensor] = None, new_lens: Optional[torch.Tensor] = None):
+        assert scores.is_cuda and scores.dtype == torch.float32 and scores.is_contiguous() and scores.dim() == 4
+        n_layers, n_seqs, n_kv_heads, stride = scores.shape
+        dev = scores.device
+        if kept is None:
+            kept = torch.zeros((n_layers, n_seqs, n_kv_heads, min(stride, max(budget, recent))), dtype=torch.int32, device=dev)
+        if new_lens is None:
+            new_lens = torch.zeros(n_seqs, dtype=torch.int32, device=dev)
+        for t in (kv_lens, protect, new_lens):
+            assert t is None or (t.dtype == torch.int32 and t.is_contiguous() and t.device == dev and t.numel() == n_seqs)
+        assert kept.dtype == torch.int32 and kept.is_contiguous() and kept.device == dev and kept.shape[:3] == scores.shape[:3]
+        assert tables is None or (tables.dtype == torch.int32 and tables.is_contiguous() and tables.device == dev and tables.shape[0] == n_seqs)
+        assert pool is None or (pool.device == dev.index and pool.n_layers == n_layers and pool.n_kv_heads == n_kv_heads)
+        self.pool, self.tables, self.kv_lens, self.scores, self.protect = pool, tables, kv_lens, scores, protect
+        self.kept, self.new_lens = kept, new_lens
+        self.status = torch.zeros(1, dtype=torch.int32, device=dev)
+        self._device = dev.index
+        self._select = N.TkvEvictSelect(dev.index, n_layers, n_seqs, n_kv_heads, stride, stride, kept.shape[3], budget, recent, 0, scores.data_ptr(),
+                                        kv_lens.data_ptr(), protect.data_ptr() if protect is not None else 0, kept.data_ptr(), new_lens.data_ptr(),
+                                        self.status.data_ptr())
+        if pool is not None and tables is not None:
+            self._pool_c = pool.c_struct()
+            bound = min(stride, tables.shape[1] * pool.block_size)
+            self._compact = N.TkvEvictCompact(0, n_layers, n_seqs, tables.shape[1], bound, stride, kept.shape[3], 0, tables.data_ptr(),
+                                              kv_lens.data_ptr(), kept.data_ptr(), new_lens.data_ptr(), scores.data_ptr(), self.status.data_ptr())
+
+    def _stream(self, stream):
+        return C.c_void_p((stream or torch.cuda.current_stream(self._device)).cuda_stream)
+
+    def select(self, stream: Optional[torch.cuda.Stream] = None):
+        """Fills and returns ``(kept, new_lens)``."""
+        check(lib().tkv_evict_select_enqueue(C.byref(self._select), self._stream(stream)))
+        return self.kept, self.new_lens
+
+    def compact(self, stream: Optional[torch.cuda.Stream] = None) -> None:
+        """Moves the rows that ``kept`` names; ``kv_lens`` still holds the lengths before."""
+        if self.pool is None or self.tables is None:
+            raise TkvError(N.ERR_INVALID_CONFIG, "compact needs the pool and its block tables")
+        check(lib().tkv_evict_compact_enqueue(C.byref(self._pool_c), C.byref(self._compact), self._stream(stream)))
+
+    def evict(self, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+        """``select``, ``compact``, and ``kv_lens`` becomes ``new_lens``, which is returned."""
+        stream = stream or torch.cuda.current_stream(self._device)
+        self.select(stream)
+        self.compact(stream)
+        with torch.cuda.stream(stream):
+            self.kv_lens.copy_(self.new_lens)
+        return self.new_lens
+
+
 class PrefixIndex:
     """Device-resident ``RadixTree`` (engine/src/prefix_cache.rs:17-149): insert / lookup / release /
     evict_lru over a batch of token sequences, one launch per call, all state in HBM.  Sequences are
