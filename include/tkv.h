@@ -442,6 +442,37 @@ typedef struct TkvScoredAttn {
 uint64_t tkv_scored_attn_scratch_bytes(uint32_t n_seqs, uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t max_kv_len);
 int32_t tkv_scored_attn_enqueue(const TkvPool* pool, const TkvScoredAttn* args, void* stream);
 
+/* Decode attention of a batch in which groups of sequences share a prefix (what tkv_prefix_index_lookup found resident, say): the
+ * shared tokens' K and V are read and attended to once per group, on the tcgen05 tensor cores, instead of once per sequence; the
+ * tokens behind them as in tkv_decode_attn_enqueue.  Sequences group_starts[g] .. group_starts[g + 1] - 1 are group g; their first
+ * prefix_lens[g] tokens (whole blocks) are those that the table row of the group's FIRST sequence names.  The result is that of
+ * attending every sequence to its own kv_lens[s] tokens; a sequence shorter than its group's prefix attends to as much of it.
+ * Sequences outside [group_starts[0], group_starts[n_groups]) are not computed and their rows of out are left as they were (a padded
+ * batch); a sequence of length 0 inside gets zeros.  No counterpart in the reference.  F16 or E4M3 pool (per-block scales applied),
+ * F16 q and out, 16-token blocks, head_dim 64 or 128, 1..8 query heads per kv head.  Lengths and groups are device memory read when the
+ * kernels run.  Calls that share scratch have to be ordered, two graphs that were captured with the same scratch included.            */
+typedef struct TkvPrefixAttn {
+    uint32_t n_seqs, n_groups, n_q_heads, table_stride, layer;
+    uint32_t max_kv_len;          /* bounds kv_lens                                                                */
+    uint32_t max_prefix_len;      /* bounds prefix_lens                                                            */
+    float sm_scale;               /* usually 1 / sqrt(head_dim)                                                    */
+    uint64_t q;                   /* f16 [n_seqs][n_q_heads][head_dim]                                             */
+    uint64_t out;                 /* f16, same shape                                                               */
+    uint64_t tables;              /* u32 [n_seqs][table_stride] block ids, prefix blocks first                     */
+    uint64_t kv_lens;             /* u32 [n_seqs] tokens, the prefix included                                      */
+    uint64_t group_starts;        /* u32 [n_groups + 1], ascending, at most n_seqs                                 */
+    uint64_t prefix_lens;         /* u32 [n_groups], multiples of 16                                               */
+    uint64_t scratch;             /* tkv_prefix_attn_scratch_bytes(...) bytes of device memory, 256-byte aligned   */
+    uint64_t scratch_bytes;
+    uint64_t status;              /* 0, or a device u32 (zero it before the launch): TKV_ERR_TIMEOUT if a bounded wait gave up,
+                                     TKV_ERR_INVALID_CONFIG if the groups do not ascend, a prefix is no whole number of blocks or above
+                                     its bound (nothing is computed then), a length is above its bound (clamped) or a table entry
+                                     names a block outside the pool (never read); out is then not valid            */
+} TkvPrefixAttn;
+uint64_t tkv_prefix_attn_scratch_bytes(uint32_t n_seqs, uint32_t n_groups, uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                                       uint32_t max_kv_len, uint32_t max_prefix_len);
+int32_t tkv_prefix_attn_enqueue(const TkvPool* pool, const TkvPrefixAttn* args, void* stream);
+
 /* Eviction: cutting every sequence of a batch to a budget by accumulated attention weight (tkv_scored_attn_enqueue), in two calls.
  * No counterpart in the reference.
  * Select: for each (layer, sequence, kv head) row of scores over len = kv_lens[s] tokens, which tokens stay.  The first protect[s]

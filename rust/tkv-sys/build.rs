@@ -11,6 +11,7 @@ const SOURCES: &[&str] = &[
     "tkv_attention_tc.cu",
     "tkv_prefill_tc.cu",
     "tkv_scored_attn.cu",
+    "tkv_prefix_attn.cu",
     "tkv_evict.cu",
     "tkv_prefix_index.cu",
     "tkv_hostobj.cpp",

@@ -229,6 +229,28 @@ pub struct TkvScoredAttn {
 
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
+pub struct TkvPrefixAttn {
+    pub n_seqs: u32,
+    pub n_groups: u32,
+    pub n_q_heads: u32,
+    pub table_stride: u32,
+    pub layer: u32,
+    pub max_kv_len: u32,
+    pub max_prefix_len: u32,
+    pub sm_scale: f32,
+    pub q: u64,
+    pub out: u64,
+    pub tables: u64,
+    pub kv_lens: u64,
+    pub group_starts: u64,
+    pub prefix_lens: u64,
+    pub scratch: u64,
+    pub scratch_bytes: u64,
+    pub status: u64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
 pub struct TkvEvictSelect {
     pub device: i32,
     pub n_layers: u32,
@@ -428,6 +450,8 @@ extern "C" {
     pub fn tkv_prefill_attn_enqueue(pool: *const TkvPool, args: *const TkvPrefillAttn, stream: *mut c_void) -> i32;
     pub fn tkv_scored_attn_scratch_bytes(n_seqs: u32, n_q_heads: u32, n_kv_heads: u32, head_dim: u32, max_kv_len: u32) -> u64;
     pub fn tkv_scored_attn_enqueue(pool: *const TkvPool, args: *const TkvScoredAttn, stream: *mut c_void) -> i32;
+    pub fn tkv_prefix_attn_scratch_bytes(n_seqs: u32, n_groups: u32, n_q_heads: u32, n_kv_heads: u32, head_dim: u32, max_kv_len: u32, max_prefix_len: u32) -> u64;
+    pub fn tkv_prefix_attn_enqueue(pool: *const TkvPool, args: *const TkvPrefixAttn, stream: *mut c_void) -> i32;
     pub fn tkv_evict_select_enqueue(args: *const TkvEvictSelect, stream: *mut c_void) -> i32;
     pub fn tkv_evict_compact_enqueue(pool: *const TkvPool, args: *const TkvEvictCompact, stream: *mut c_void) -> i32;
     pub fn tkv_selfcheck_tensor_cores(mismatches: *mut u64) -> i32;

@@ -69,6 +69,12 @@ class TkvScoredAttn(C.Structure):
         (n, C.c_uint64) for n in ("q", "out", "tables", "kv_lens", "scores", "scratch", "scratch_bytes", "status")]
 
 
+class TkvPrefixAttn(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("n_seqs", "n_groups", "n_q_heads", "table_stride", "layer", "max_kv_len", "max_prefix_len")] + [
+        ("sm_scale", C.c_float)] + [(n, C.c_uint64) for n in (
+            "q", "out", "tables", "kv_lens", "group_starts", "prefix_lens", "scratch", "scratch_bytes", "status")]
+
+
 class TkvEvictSelect(C.Structure):
     _fields_ = [("device", C.c_int32)] + [(n, C.c_uint32) for n in (
         "n_layers", "n_seqs", "n_kv_heads", "max_kv_len", "score_stride", "kept_stride", "budget", "recent", "reserved")] + [
@@ -185,6 +191,8 @@ SIGNATURES = {
     "tkv_decode_attn_enqueue": (_i32, [C.POINTER(TkvPool), C.POINTER(TkvDecodeAttn), _vp]),
     "tkv_scored_attn_scratch_bytes": (_u64, [_u32, _u32, _u32, _u32, _u32]),
     "tkv_scored_attn_enqueue": (_i32, [C.POINTER(TkvPool), C.POINTER(TkvScoredAttn), _vp]),
+    "tkv_prefix_attn_scratch_bytes": (_u64, [_u32, _u32, _u32, _u32, _u32, _u32, _u32]),
+    "tkv_prefix_attn_enqueue": (_i32, [C.POINTER(TkvPool), C.POINTER(TkvPrefixAttn), _vp]),
     "tkv_evict_select_enqueue": (_i32, [C.POINTER(TkvEvictSelect), _vp]),
     "tkv_evict_compact_enqueue": (_i32, [C.POINTER(TkvPool), C.POINTER(TkvEvictCompact), _vp]),
     "tkv_selfcheck_tensor_cores": (_i32, [_u64p]),

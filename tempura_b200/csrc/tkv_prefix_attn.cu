@@ -1,0 +1,895 @@
+// Decode attention of a batch whose sequences share prefixes: the shared tokens of a group are attended to once for all its members.
+//
+// Over the prefix every (member, query head) of a group and kv head is one row of a matrix product, so
+//
+//     S[rows][128 tokens] = Q . K_tile^T,   P = 2^(scale * S - m),   O[rows][dims] += P . V_tile
+//
+// runs on the fifth-generation tensor cores (tcgen05, accumulators in tensor memory) and K and V of the prefix are read once
+// per group instead of once per sequence.  The tokens behind the prefix go through rows_attn, and a third kernel joins the partial
+// results (m, l, O) of both: out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.
+//
+// A CTA works on up to 256 rows of one (group, kv head) as two streams of 128 with their own S, P and O: with more than 128 rows
+// the streams are two row tiles that read the same cached tiles; with fewer they are the same rows on alternate cached tiles (two
+// partial results).  While the softmax of one stream runs, the tensor cores work for the other.  A softmax thread owns a row: no
+// exchange between threads.  P goes back to tensor memory, over the S it was made from, as the A operand of the second product, so
+// shared memory holds Q and the K and V tiles only.  The row maximum in use is raised, and O rescaled, only when a score exceeds it by 2^6.
+// An F16 pool's tiles arrive as tensor-map boxes, in the 128-byte swizzle the MMA reads.  An E4M3 pool's tiles are widened to F16
+// on the way by four warps (exact); K's block scale multiplies the scores, V's the probabilities, in units of a power of two above every
+// scale met so far.  Both operands of both products are then F16 and the products exact; a probability is rounded to F16 once (2^-11 of
+// its value at most, like the output itself).
+//
+// Work split: the cached tiles of all (group, kv head, row block) items, one after another, in equal shares, one per CTA; a share may
+// begin and end inside an item.  The partial rows of item i and share c start at 2 * (rows before item i) + 512 * c, which keeps them
+// apart because both only grow along the work.
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <cstdio>
+#include <stdint.h>
+#include <type_traits>
+
+#include "../../include/tkv.h"
+#include "tkv_rows_attn.cuh"
+#include "tkv_tc_common.cuh"
+
+namespace tkv_internal {
+int32_t set_error(int32_t code, int32_t cuda_code, const char* text);
+}
+
+namespace {
+
+using namespace tkv_tc;
+using tkv_rows::bar_wait;
+
+constexpr uint32_t CTAS = 148;               // one per SM of the part this is built for; partial results are sized by it
+constexpr int BS = 16, KT = 128;             // tokens of a block, of a cached tile
+constexpr int GROUP_BYTES = 128 * 128;       // a [128 rows][128 B] swizzled column group of an operand tile
+constexpr float RAISE = 6.0f;
+constexpr uint32_t MIN_SHARE = 2;            // cached tiles
+
+struct Args {
+    const uint32_t *tables, *kv_lens, *group_starts, *prefix_lens;
+    const __half* q;
+    const char *k8, *v8;                     // layer tensors of an E4M3 pool
+    const float *k_scales, *v_scales;
+    float *part_o, *part_ml;                 // [row][D], [row][2]
+    uint32_t *plan, *status;                 // [0] cached tiles per share, [1 + g] tiles before group g (n_groups + 1 entries)
+    uint64_t block_stride;
+    uint32_t row_stride, n_seqs, n_groups, n_q_heads, n_kv_heads, group, table_stride, max_kv_len, max_prefix_len, total_blocks, parts;
+    uint32_t q_sign;                         // 0x80008000 for a negative scale: its sign is moved to q
+    float scale_log2;                        // not negative
+};
+
+__host__ __device__ constexpr int softmax_warps() { return 8; }
+__host__ __device__ constexpr int feed_warps(bool fp8) { return fp8 ? 4 : 1; }
+__host__ __device__ constexpr int threads_of(bool fp8) { return (softmax_warps() + feed_warps(fp8) + 1) * 32; }
+
+struct Control {
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+    uint64_t q_ready[2], s_full[2], p_full[2], pv_done[2], drained;
+    uint32_t tmem, fail;
+    float scales[4][16];                     // per cached tile (mod 4): K scales of its 8 blocks, V scales
+};
+constexpr uint32_t CTRL_BYTES = 1024;
+static_assert(sizeof(Control) <= CTRL_BYTES, "control block");
+
+// one tile of one item
+struct Item {
+    uint32_t first_seq, rows, row0, block_rows;   // of the group: first sequence, rows; of the row block: first row, rows (at most 256)
+    uint32_t kvh, prefix, tile, n_tiles;          // tiles [tile, tile + n_tiles) of the prefix
+    uint64_t out_row;                             // first partial row
+};
+__device__ __forceinline__ uint32_t row_blocks(uint32_t rows) { return (rows + 255) / 256; }
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) { mma<false>(d, a, b, idesc, acc); }
+// A operand from tensor memory: lane = row, two F16 of the row per column
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+
+template <int D, bool FP8>
+__global__ void __launch_bounds__(threads_of(FP8), 1)
+prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Args a) {
+    constexpr int NCG = D / 64;                                 // column groups of 64 F16 dims
+    constexpr int TILE = NCG * GROUP_BYTES;                     // Q, K or V tile of 128 rows
+    constexpr int KSTEPS = D / 16;
+    constexpr int THREADS = threads_of(FP8), SM = softmax_warps(), FEED = feed_warps(FP8);
+    constexpr uint32_t IDESC_QK = instr_desc2(0u, 0u, 0u, 0u, 128u), IDESC_PV = instr_desc2(0u, 0u, 0u, 1u, (uint32_t)D);   // B = V, MN-major
+    constexpr uint64_t DESC_HI = ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+    constexpr uint64_t DESC_K = DESC_HI | ((uint64_t)1u << 16);
+    constexpr uint64_t DESC_V = DESC_HI | ((uint64_t)(GROUP_BYTES >> 4) << 16);        // the second 64 dims one column group further
+    constexpr uint32_t TM_S = 0, TM_O = 256;                    // tensor memory columns: S (and P over it) of stream x at 128 x, O at 256 + 128 x
+
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    Control* c = reinterpret_cast<Control*>(smem);
+    unsigned char* q_tile = smem + CTRL_BYTES;                  // two
+    unsigned char* k_ring = q_tile + 2 * TILE;                  // two
+    unsigned char* v_ring = k_ring + 2 * TILE;                  // two
+    const volatile uint32_t* fail = &c->fail;
+    __shared__ uint32_t cum[THREADS + 1], warp_sum[THREADS / 32];
+
+    if (__syncthreads_or(tkv_rows::groups_bad(a.group_starts, a.prefix_lens, a.n_groups, a.n_seqs, a.max_prefix_len, tid, THREADS))) {
+        if (tid == 0) {
+            tkv_rows::report(a.status, 2u);
+            if (blockIdx.x == 0) a.plan[0] = 0;                 // nothing was computed
+        }
+        return;
+    }
+    // ---- cached tiles before every run of `per` groups ----
+    auto tiles_of = [&](uint32_t g) -> uint32_t {               // a group's tiles times its (kv head, row block) items
+        const uint32_t rows = (a.group_starts[g + 1] - a.group_starts[g]) * a.group;
+        return row_blocks(rows) * a.n_kv_heads * ((a.prefix_lens[g] + KT - 1) / KT);
+    };
+    const uint32_t per = (a.n_groups + THREADS - 1) / THREADS;
+    uint32_t mine = 0;
+    for (uint32_t i = 0; i < per; i++)
+        if (tid * per + i < a.n_groups) mine += tiles_of(tid * per + i);
+    uint32_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+        if (lane >= (uint32_t)o) incl += v;
+    }
+    if (lane == 31) warp_sum[warp] = incl;
+    if (tid == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(c->k_full + i, FP8 ? FEED : 1);
+            mbar_init(c->v_full + i, FP8 ? FEED : 1);
+            mbar_init(c->k_empty + i, 1);
+            mbar_init(c->v_empty + i, 1);
+            mbar_init(c->q_ready + i, SM / 2);
+            mbar_init(c->s_full + i, 1);
+            mbar_init(c->p_full + i, SM / 2);
+            mbar_init(c->pv_done + i, 1);
+        }
+        mbar_init(&c->drained, 1);
+        c->fail = (smem_u32(smem) & 1023u) ? 2u : 0u;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    uint32_t before = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; w++) before += w < (int)warp ? warp_sum[w] : 0u;
+    cum[tid] = before + incl - mine;
+    if (tid == THREADS - 1) cum[THREADS] = before + incl;
+    __syncthreads();
+    const uint32_t total = cum[THREADS], share = max((total + a.parts - 1) / a.parts, MIN_SHARE);
+    if (blockIdx.x == 0) {
+        uint32_t at = cum[tid];
+        for (uint32_t i = 0; i < per; i++)
+            if (tid * per + i < a.n_groups) {
+                a.plan[1 + tid * per + i] = at;
+                at += tiles_of(tid * per + i);
+            }
+        if (tid == 0) {
+            a.plan[0] = share;
+            a.plan[1 + a.n_groups] = total;
+        }
+    }
+    if ((uint64_t)blockIdx.x * share >= total) return;
+    const uint32_t u_begin = blockIdx.x * share, u_end = min(total, u_begin + share);
+
+    if (warp == SM + FEED) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&c->tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = c->tmem;
+
+    // ---- the group of the first tile ----
+    uint32_t g, at;                                             // tiles before group g
+    {
+        uint32_t lo = 0, hi = THREADS;                          // cum[lo] <= u_begin < cum[hi]
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if (cum[mid] <= u_begin) lo = mid;
+            else hi = mid;
+        }
+        g = lo * per;
+        at = cum[lo];
+    }
+    uint32_t tiles_done = 0;                                    // cached tiles of this CTA before the item at hand: places in the rings
+    uint32_t n_pv[2] = {0, 0};                                  // products P.V of each stream so far: phases of its barriers
+    uint32_t issued[2] = {0, 0};                                // F16 producer: tiles of K, of V asked for
+    bool ok = true;
+    for (uint32_t u = u_begin, item_no = 0; u < u_end; item_no++) {
+        while (at + tiles_of(g) <= u) at += tiles_of(g++);
+        Item it;
+        {
+            it.first_seq = a.group_starts[g];
+            it.rows = (a.group_starts[g + 1] - it.first_seq) * a.group;
+            it.prefix = a.prefix_lens[g];
+            const uint32_t nt = (it.prefix + KT - 1) / KT, rbs = row_blocks(it.rows), item = (u - at) / nt;
+            it.kvh = item / rbs;
+            it.row0 = (item % rbs) * 256;
+            it.block_rows = min(256u, it.rows - it.row0);
+            it.tile = (u - at) % nt;
+            it.n_tiles = min(nt - it.tile, u_end - u);
+            it.out_row = 2ull * ((uint64_t)(it.first_seq - a.group_starts[0]) * a.group * a.n_kv_heads + (uint64_t)it.kvh * it.rows + it.row0) + 512ull * blockIdx.x;
+        }
+        const bool same_rows = it.block_rows <= 128;            // both streams the same rows, alternate tiles
+        const uint32_t* table = a.tables + (size_t)it.first_seq * a.table_stride;
+        const uint32_t n_blocks = it.prefix / BS;
+        auto blocks_in = [&](uint32_t i) { return min(8u, n_blocks - (it.tile + i) * 8u); };   // of the item's i-th tile
+        uint32_t n_of[2];                                       // tiles of each stream
+        n_of[0] = same_rows ? (it.n_tiles + 1) / 2 : it.n_tiles;
+        n_of[1] = same_rows ? it.n_tiles / 2 : it.n_tiles;
+
+        if (warp == SM + FEED) {
+            // ---- MMA issuer: whichever stream is ready goes next ----
+            if (lane == 0) {
+                const uint32_t q_lo = smem_u32(q_tile) >> 4, k_lo = smem_u32(k_ring) >> 4, v_lo = smem_u32(v_ring) >> 4;
+                uint32_t jq[2] = {0, 0}, jp[2] = {0, 0}, k_left[2] = {0, 0}, v_left[2] = {0, 0}, idle = 0;
+                const uint32_t readers = same_rows ? 1u : 2u;
+                for (int x = 0; x < 2 && ok; x++) ok = bar_wait(smem_u32(c->q_ready + x), item_no & 1u, fail);
+                while (ok && (jp[0] < n_of[0] || jp[1] < n_of[1])) {
+                    bool did = false;
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        const uint32_t i = same_rows ? 2 * jq[x] + x : jq[x];
+                        if (jq[x] == jp[x] && jq[x] < n_of[x]) {
+                            const uint32_t t = tiles_done + i, st = t & 1u, total_pv = n_pv[x] + jp[x];
+                            // S of this stream is free when the product that read P over it is done
+                            if (mbar_test(c->k_full + st, (t >> 1) & 1u) && (total_pv == 0 || mbar_test(c->pv_done + x, (total_pv - 1) & 1u))) {
+                                tc_fence_after();
+#pragma unroll
+                                for (int ks = 0; ks < KSTEPS; ks++) {
+                                    const uint32_t off = (ks / 4) * (GROUP_BYTES >> 4) + (ks % 4) * 2;
+                                    mma_ss(tmem + TM_S + x * 128, DESC_K | (q_lo + x * (TILE >> 4) + off), DESC_K | (k_lo + st * (TILE >> 4) + off), IDESC_QK,
+                                           ks > 0 ? 1u : 0u);
+                                }
+                                tc_commit(c->s_full + x);
+                                if (++k_left[st] == readers) {
+                                    tc_commit(c->k_empty + st);
+                                    k_left[st] = 0;
+                                }
+                                jq[x]++;
+                                did = true;
+                            }
+                        } else if (jq[x] == jp[x] + 1) {
+                            const uint32_t ip = same_rows ? 2 * jp[x] + x : jp[x], t = tiles_done + ip, st = t & 1u, total_pv = n_pv[x] + jp[x];
+                            if (mbar_test(c->p_full + x, total_pv & 1u) && mbar_test(c->v_full + st, (t >> 1) & 1u)) {
+                                tc_fence_after();
+                                const uint32_t nb = blocks_in(ip);       // a block is one k-step: blocks behind the prefix are left out
+                                for (uint32_t ks = 0; ks < nb; ks++)
+                                    mma_ts(tmem + TM_O + x * 128, tmem + TM_S + x * 128 + ks * 8, DESC_V | (v_lo + st * (TILE >> 4) + ks * (2048u >> 4)), IDESC_PV,
+                                           (jp[x] > 0 || ks > 0) ? 1u : 0u);
+                                tc_commit(c->pv_done + x);
+                                if (++v_left[st] == readers) {
+                                    tc_commit(c->v_empty + st);
+                                    v_left[st] = 0;
+                                }
+                                jp[x]++;
+                                did = true;
+                            }
+                        }
+                    }
+                    if (did) {
+                        idle = 0;
+                    } else {
+                        if (++idle > (1u << 24) || ((idle & 63u) == 0 && *fail)) ok = false;    // bounded: a stuck barrier ends the CTA, not the GPU
+                        __nanosleep(20);
+                    }
+                }
+                if (!ok) atomicCAS(&c->fail, 0u, 4u);
+            }
+            __syncwarp();
+        } else if (warp >= SM) {
+            if (!FP8) {
+                // ---- producer: eight lanes, a block each ----
+                for (uint32_t i = 0; i < it.n_tiles && ok; i++) {
+                    const uint32_t t = tiles_done + i, st = t & 1u, nb = blocks_in(i);
+                    uint32_t blk = 0;
+                    if (lane < nb) blk = table[(it.tile + i) * 8u + lane];
+                    if (__any_sync(0xFFFFFFFFu, blk >= a.total_blocks)) {          // a stale or foreign id is never turned into an address
+                        if (lane == 0) atomicCAS(&c->fail, 0u, 2u);
+                        ok = false;
+                        break;
+                    }
+#pragma unroll
+                    for (int kv = 0; kv < 2; kv++) {
+                        uint64_t* full = (kv ? c->v_full : c->k_full) + st;
+                        if (t >= 2) ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32((kv ? c->v_empty : c->k_empty) + st), ((t >> 1) - 1u) & 1u, fail));
+                        if (!ok) break;
+                        issued[kv] = t + 1;
+                        if (lane == 0) mbar_expect_tx(full, nb * BS * 128u * NCG);
+                        __syncwarp();
+                        if (lane < nb) {
+                            const uint32_t dst = smem_u32((kv ? v_ring : k_ring) + st * TILE) + lane * (BS * 128u);
+#pragma unroll
+                            for (int cg = 0; cg < NCG; cg++)
+                                tma_head_rows(dst + cg * GROUP_BYTES, kv ? &map_v : &map_k, cg * 128, (int32_t)it.kvh, (int32_t)(blk * BS), full);
+                        }
+                    }
+                }
+                if (!ok) {
+                    if (lane == 0) atomicCAS(&c->fail, 0u, 4u);
+                    // no copy is in flight when the CTA's shared memory goes: the last two of each ring are waited for
+#pragma unroll
+                    for (int kv = 0; kv < 2; kv++)
+                        for (uint32_t t = issued[kv] > 2 ? issued[kv] - 2 : 0u; t < issued[kv]; t++)
+                            for (uint32_t n = 0; n < (1u << 20) && !mbar_test((kv ? c->v_full : c->k_full) + (t & 1u), (t >> 1) & 1u); n++) {}
+                }
+            } else {
+                // ---- widening: 128 threads, 16 bytes of a token at a time, a tile ahead in registers ----
+                constexpr int CPR = D / 16, PER = 128 * CPR / 128;             // 16-byte pieces of a row; per thread and tile
+                const uint32_t t128 = tid - SM * 32;
+                uint4 kr[PER], vr[PER];
+                float sc = 0.0f;
+                auto piece = [&](int e, uint32_t& row, uint32_t& ch) {          // a warp's 32 pieces: whole rows
+                    const uint32_t n = e * 128 + t128;
+                    row = n / CPR;
+                    ch = n % CPR;
+                };
+                auto load = [&](uint4 (&r)[PER], const char* base, uint32_t i) {
+                    const uint32_t nb = blocks_in(i);
+#pragma unroll
+                    for (int e = 0; e < PER; e++) {
+                        uint32_t row, ch;
+                        piece(e, row, ch);
+                        r[e] = make_uint4(0, 0, 0, 0);
+                        if (row / BS < nb) {
+                            const uint32_t blk = table[(it.tile + i) * 8u + row / BS];
+                            if (blk < a.total_blocks)
+                                r[e] = __ldg(reinterpret_cast<const uint4*>(base + (uint64_t)blk * a.block_stride + (size_t)(row % BS) * a.row_stride + (size_t)it.kvh * D + ch * 16));
+                            else atomicCAS(&c->fail, 0u, 2u);
+                        }
+                    }
+                };
+                auto load_scales = [&](uint32_t i) {
+                    sc = 1.0f;
+                    if (t128 < 16 && a.k_scales) {
+                        sc = 0.0f;
+                        if ((t128 & 7u) < blocks_in(i)) {
+                            const uint32_t blk = table[(it.tile + i) * 8u + (t128 & 7u)];
+                            if (blk < a.total_blocks) sc = __ldg((t128 < 8 ? a.k_scales : a.v_scales) + (size_t)blk * a.n_kv_heads + it.kvh);
+                        }
+                    }
+                };
+                auto widen = [&](unsigned char* tile, const uint4 (&r)[PER]) {
+#pragma unroll
+                    for (int e = 0; e < PER; e++) {
+                        uint32_t row, ch;
+                        piece(e, row, ch);
+                        const uint32_t w[4] = {r[e].x, r[e].y, r[e].z, r[e].w};
+                        uint32_t h[8];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            h[2 * k] = tkv_rows::e4m3x2_h2(w[k] & 0xFFFFu);
+                            h[2 * k + 1] = tkv_rows::e4m3x2_h2(w[k] >> 16);
+                        }
+                        unsigned char* base = tile + (ch / 4) * GROUP_BYTES;   // 16 dims = two 16-byte chunks of F16
+                        *reinterpret_cast<uint4*>(base + swz(row, (ch % 4) * 2)) = make_uint4(h[0], h[1], h[2], h[3]);
+                        *reinterpret_cast<uint4*>(base + swz(row, (ch % 4) * 2 + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                };
+                load_scales(0);
+                load(kr, a.k8, 0);
+                load(vr, a.v8, 0);
+                for (uint32_t i = 0; i < it.n_tiles && ok; i++) {
+                    const uint32_t t = tiles_done + i, st = t & 1u;
+                    if (t >= 2) ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(c->k_empty + st), ((t >> 1) - 1u) & 1u, fail));
+                    if (!ok) break;
+                    if (t128 < 16) c->scales[t & 3u][t128] = sc;
+                    widen(k_ring + st * TILE, kr);
+                    if (lane == 0) mbar_arrive(c->k_full + st);
+                    if (i + 1 < it.n_tiles) {
+                        load_scales(i + 1);
+                        load(kr, a.k8, i + 1);
+                    }
+                    if (t >= 2) ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(c->v_empty + st), ((t >> 1) - 1u) & 1u, fail));
+                    if (!ok) break;
+                    widen(v_ring + st * TILE, vr);
+                    if (lane == 0) mbar_arrive(c->v_full + st);
+                    if (i + 1 < it.n_tiles) load(vr, a.v8, i + 1);
+                    if (*fail) ok = false;
+                }
+                if (!ok && lane == 0) atomicCAS(&c->fail, 0u, 4u);
+            }
+        } else {
+            // ---- softmax: one row per thread ----
+            const uint32_t x = warp >> 2, n_x = x ? n_of[1] : n_of[0], pv_x = x ? n_pv[1] : n_pv[0], r = (warp & 3u) * 32u + lane, row = it.row0 + (same_rows ? 0u : x * 128u) + r;   // of the group and kv head
+            const bool live = row < it.rows && (same_rows ? r < it.block_rows : x * 128u + r < it.block_rows);
+            const bool warp_live = __any_sync(0xFFFFFFFFu, live);
+            const uint32_t seq = it.first_seq + (live ? row / a.group : 0u), head = it.kvh * a.group + (live ? row % a.group : 0u);
+            const uint32_t limit = live ? min(min(a.kv_lens[seq], a.max_kv_len), it.prefix) : 0u;
+            {
+                const uint4* src = reinterpret_cast<const uint4*>(a.q + ((size_t)seq * a.n_q_heads + head) * D);
+                unsigned char* qt = q_tile + x * TILE;
+#pragma unroll
+                for (int ch = 0; ch < D / 8; ch++) {
+                    uint4 v = live ? __ldg(src + ch) : make_uint4(0, 0, 0, 0);
+                    v = make_uint4(v.x ^ a.q_sign, v.y ^ a.q_sign, v.z ^ a.q_sign, v.w ^ a.q_sign);
+                    *reinterpret_cast<uint4*>(qt + (ch / 8) * GROUP_BYTES + swz(r, ch % 8)) = v;
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(c->q_ready + x);
+            }
+            const uint32_t lanes = ((warp & 3u) * 32u) << 16, ts = tmem + TM_S + x * 128 + lanes, to = tmem + TM_O + x * 128 + lanes;
+            float m = -INFINITY, l = 0.0f, v_ref = FP8 ? 0x1p-100f : 1.0f, v_inv = FP8 ? 0x1p+100f : 1.0f;
+            for (uint32_t j = 0; j < n_x && ok; j++) {
+                const uint32_t i = same_rows ? 2 * j + x : j, t0 = (it.tile + i) * KT, slot = (tiles_done + i) & 3u;
+                ok = bar_wait(smem_u32(c->s_full + x), (pv_x + j) & 1u, fail);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) break;
+                if (warp_live) {
+                    tc_fence_after();
+                    constexpr int CH = FP8 ? 64 : 128;          // scores held in registers; an E4M3 pool's are read twice
+                    const int left = (int)min(limit > t0 ? limit - t0 : 0u, (uint32_t)KT);   // tokens of the tile that the row attends to
+                    auto tile = [&](auto masked_type) {
+                    constexpr bool MASKED = decltype(masked_type)::value;
+                    uint32_t v[CH / 32][32];
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int c0 = 0; c0 < KT; c0 += CH) {
+#pragma unroll
+                        for (int k = 0; k < CH; k += 32) tmem_ld32(ts + c0 + k, v[k / 32]);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int b = 0; b < CH / 16; b++) {
+                            float top = -INFINITY;              // neither scale is negative: the maximum commutes with them
+#pragma unroll
+                            for (int k = 0; k < 16; k++)
+                                top = fmaxf(top, MASKED && c0 + b * 16 + k >= left ? -INFINITY : __uint_as_float(v[b / 2][(b & 1) * 16 + k]));
+                            mx = fmaxf(mx, top == -INFINITY ? top : top * (FP8 ? a.scale_log2 * c->scales[slot][c0 / 16 + b] : a.scale_log2));
+                        }
+                    }
+                    // ---- a raised maximum or V scale rescales the row of O; the previous product is done, or S would not be here ----
+                    float factor = 1.0f;
+                    if (mx > m + RAISE) {
+                        factor = m == -INFINITY ? 0.0f : fast_exp2(m - mx);
+                        m = mx;
+                        l *= factor;
+                    }
+                    if (FP8) {
+                        float top = 0.0f;
+#pragma unroll
+                        for (int b = 0; b < 8; b++) top = fmaxf(top, c->scales[slot][8 + b]);
+                        if (top > v_ref) {                      // the same in every thread
+                            const float up = __uint_as_float(min((__float_as_uint(top) >> 23) + 1u, 253u) << 23);
+                            factor *= v_ref / up;
+                            v_ref = up;
+                            v_inv = 1.0f / up;
+                        }
+                    }
+                    if (j > 0 && __any_sync(0xFFFFFFFFu, factor != 1.0f)) {
+#pragma unroll 1
+                        for (uint32_t c0 = 0; c0 < (uint32_t)D; c0 += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(to + c0, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
+                            tmem_st16(to + c0, o);
+                        }
+                        tmem_wait_st();
+                    }
+                    // ---- probabilities, as F16 pairs over the scores ----
+                    const float sub = m == -INFINITY ? 0.0f : m;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int c0 = 0; c0 < KT; c0 += CH) {       // P of tokens [c0, c0 + CH) goes to columns [c0 / 2, (c0 + CH) / 2): scores already read
+                        if (CH < KT) {
+#pragma unroll
+                            for (int k = 0; k < CH; k += 32) tmem_ld32(ts + c0 + k, v[k / 32]);
+                            tmem_wait_ld();
+                        }
+#pragma unroll
+                        for (int b = 0; b < CH / 16; b++) {
+                            const float ks = FP8 ? a.scale_log2 * c->scales[slot][c0 / 16 + b] : a.scale_log2;
+                            const float vn = FP8 ? c->scales[slot][8 + c0 / 16 + b] * v_inv : 1.0f;
+#pragma unroll
+                            for (int k = 0; k < 16; k += 2) {
+                                float p0 = fast_exp2(__fmaf_rn(__uint_as_float(v[b / 2][(b & 1) * 16 + k]), ks, -sub));
+                                float p1 = fast_exp2(__fmaf_rn(__uint_as_float(v[b / 2][(b & 1) * 16 + k + 1]), ks, -sub));
+                                if (MASKED) {
+                                    p0 = c0 + b * 16 + k < left ? p0 : 0.0f;
+                                    p1 = c0 + b * 16 + k + 1 < left ? p1 : 0.0f;
+                                }
+                                sum += p0 + p1;
+                                if (FP8) {
+                                    p0 *= vn;
+                                    p1 *= vn;
+                                }
+                                const __half2 h = __floats2half2_rn(p0, p1);
+                                v[b / 4][((b & 3) * 16 + k) / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < CH / 2; k += 32) tmem_st32(ts + c0 / 2 + k, v[k / 32]);
+                    }
+                    tmem_wait_st();
+                    l += sum;
+                    };
+                    if (__any_sync(0xFFFFFFFFu, left < KT)) tile(std::true_type{});
+                    else tile(std::false_type{});
+                    tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(c->p_full + x);
+            }
+            // ---- partial result of the row ----
+            const uint32_t n = n_x;
+            const uint64_t dst = it.out_row + (same_rows ? x * it.block_rows + r : x * 128u + r);
+            if (ok && n) {
+                ok = bar_wait(smem_u32(c->pv_done + x), (pv_x + n - 1) & 1u, fail);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+            }
+            if (ok && warp_live) {
+                tc_fence_after();
+                if (live) *reinterpret_cast<float2*>(a.part_ml + dst * 2) = n ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
+                if (n) {
+#pragma unroll 1
+                    for (uint32_t c0 = 0; c0 < (uint32_t)D; c0 += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(to + c0, o);
+                        tmem_wait_ld();
+                        if (live) {
+#pragma unroll
+                            for (int k = 0; k < 32; k += 4)
+                                *reinterpret_cast<float4*>(a.part_o + dst * D + c0 + k) =
+                                    make_float4(__uint_as_float(o[k]) * v_ref, __uint_as_float(o[k + 1]) * v_ref, __uint_as_float(o[k + 2]) * v_ref,
+                                                __uint_as_float(o[k + 3]) * v_ref);
+                        }
+                    }
+                }
+            }
+            if (!ok && lane == 0) atomicCAS(&c->fail, 0u, 4u);
+            tc_fence_before();
+        }
+        __syncthreads();                                        // the next item's Q overwrites this one's
+        tc_fence_after();
+        if (*fail) break;                                       // the same for all threads: nobody writes it between the two barriers
+        __syncthreads();
+        tiles_done += it.n_tiles;
+        n_pv[0] += n_of[0];
+        n_pv[1] += n_of[1];
+        u += it.n_tiles;
+    }
+    if (warp == SM + FEED) {
+        if (lane == 0) {                                        // whatever ended the loop, no product is under way when tensor memory is given back
+            tc_commit(&c->drained);
+            for (uint32_t i = 0; i < (1u << 22) && !mbar_test(&c->drained, 0u); i++) {}
+        }
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+    if (tid == 0 && c->fail) tkv_rows::report(a.status, c->fail);
+}
+
+// ---- joining ----------------------------------------------------------------------------------------------------------------------
+struct JoinArgs {
+    const float *pre_o, *pre_ml, *own_o, *own_ml;   // partial results over the prefixes, over the tokens behind them
+    const uint32_t *pre_plan, *own_plan, *kv_lens, *group_starts, *prefix_lens;
+    __half* out;
+    uint32_t n_seqs, n_groups, n_q_heads, n_kv_heads, group, subs;
+};
+
+// WPR warps join the partial results of one (sequence, query head): one where there are rows enough to fill the machine, eight where
+// few rows have many parts.  Bound by latency and L2.
+template <int D, int WPR> __global__ void __launch_bounds__(256) prefix_join(const JoinArgs a) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");          // launched ahead of the second kernel's end
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint64_t row = WPR == 1 ? (uint64_t)blockIdx.x * 8 + warp : blockIdx.x;
+    const bool in = row < (uint64_t)a.n_seqs * a.n_q_heads;
+    const uint32_t s = in ? (uint32_t)(row / a.n_q_heads) : 0u, head = in ? (uint32_t)(row % a.n_q_heads) : 0u;
+    const uint32_t share_t = a.pre_plan[0], share_b = a.own_plan[0];
+    const uint32_t g = tkv_rows::group_of(a.group_starts, a.n_groups, s);
+    if (!in || share_t == 0 || share_b == 0 || g == a.n_groups) return;   // (all warps of a row alike) refused, or a row behind the last sequence
+    // parts of the prefix
+    const uint32_t s0 = a.group_starts[g], rows = (a.group_starts[g + 1] - s0) * a.group, kvh = head / a.group, r = (s - s0) * a.group + head % a.group;
+    const uint32_t rb = r / 256, block_rows = min(256u, rows - rb * 256), nt = (a.prefix_lens[g] + KT - 1) / KT;
+    const bool same_rows = block_rows <= 128;
+    const uint32_t t0 = a.pre_plan[1 + g] + (kvh * row_blocks(rows) + rb) * nt, c0 = nt ? t0 / share_t : 0u, k = same_rows ? 2u : 1u;
+    const uint32_t n_pre = nt ? ((t0 + nt - 1) / share_t - c0 + 1) * k : 0u;
+    const uint64_t first = 2ull * ((uint64_t)(s0 - a.group_starts[0]) * a.group * a.n_kv_heads + (uint64_t)kvh * rows + rb * 256) + 512ull * c0 + r % 256;
+    // parts of the tokens behind it
+    const uint32_t lo = a.own_plan[1 + s], hi = a.own_plan[2 + s], p0 = hi > lo ? lo / share_b : 0u;
+    const uint32_t n_own = hi > lo ? ((hi - 1) / share_b - p0 + 1) * a.subs : 0u, n = n_pre + n_own;
+    auto part = [&](uint32_t i, const float*& o, const float*& ml) {
+        if (i < n_pre) {
+            const uint64_t at = first + (i / k) * 512ull + (i % k) * block_rows;
+            o = a.pre_o + at * D;
+            ml = a.pre_ml + at * 2;
+        } else {
+            const uint64_t at = ((uint64_t)(p0 + s) * a.subs + (i - n_pre)) * a.n_q_heads + head;
+            o = a.own_o + at * D;
+            ml = a.own_ml + at * 2;
+        }
+    };
+    // maximum and sum of the row, every warp by itself
+    float m = -INFINITY, l = 0.0f;
+    for (uint32_t i0 = 0; i0 < n; i0 += 128) {
+        float2 v[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const uint32_t i = i0 + 32 * q + lane;
+            v[q] = make_float2(-INFINITY, 0.0f);
+            if (i < n) {
+                const float *o, *ml;
+                part(i, o, ml);
+                v[q] = *reinterpret_cast<const float2*>(ml);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const float mm = fmaxf(m, v[q].x);
+            l = mm == -INFINITY ? l + v[q].y : l * fast_exp2(m - mm) + v[q].y * fast_exp2(v[q].x - mm);
+            m = mm;
+        }
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        const float m_o = __shfl_xor_sync(0xFFFFFFFFu, m, off), l_o = __shfl_xor_sync(0xFFFFFFFFu, l, off);
+        const float mm = fmaxf(m, m_o);
+        l = mm == -INFINITY ? l + l_o : l * fast_exp2(m - mm) + l_o * fast_exp2(m_o - mm);
+        m = mm;
+    }
+    const float top = m == -INFINITY ? 0.0f : m, inv = l == 0.0f ? 0.0f : 1.0f / l;   // an empty row: 0
+    constexpr int PER = D / 32;
+    float acc[PER];
+#pragma unroll
+    for (int d = 0; d < PER; d++) acc[d] = 0.0f;
+#pragma unroll 8
+    for (uint32_t i = WPR == 1 ? 0u : warp; i < n; i += WPR) {
+        const float *o, *ml;
+        part(i, o, ml);
+        const float2 v = *reinterpret_cast<const float2*>(ml);
+        const float f = fast_exp2(v.x - top);
+        float x[PER];
+#pragma unroll
+        for (int d = 0; d < PER; d++) x[d] = o[d * 32 + lane];
+#pragma unroll
+        for (int d = 0; d < PER; d++) acc[d] = v.x != -INFINITY || v.y != 0.0f ? __fmaf_rn(f, x[d], acc[d]) : acc[d];   // an empty part's O counts for nothing
+    }
+    __half* out = a.out + row * D;
+    if (WPR == 1) {
+#pragma unroll
+        for (int d = 0; d < PER; d++) out[d * 32 + lane] = __float2half_rn(acc[d] * inv);
+    } else {
+        __shared__ float sum[8][D];
+#pragma unroll
+        for (int d = 0; d < PER; d++) sum[warp][d * 32 + lane] = acc[d];
+        __syncthreads();
+        if (threadIdx.x < D) {
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 8; w++) v += sum[w][threadIdx.x];
+            out[threadIdx.x] = __float2half_rn(v * inv);
+        }
+    }
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------------------------
+int32_t fail(int32_t code, const char* fmt, unsigned long long x = 0, unsigned long long y = 0) {
+    char buf[256];
+    snprintf(buf, sizeof buf, fmt, x, y);
+    return tkv_internal::set_error(code, 0, buf);
+}
+uint64_t up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
+
+// An F16 layer tensor as bytes [token][kv head][2 D], boxes of [16 tokens][1 head][128 B]: one column group of a head's rows of a block.
+bool make_map(CUtensorMap* map, uint64_t base, uint32_t total_blocks, uint32_t n_kv_heads, uint32_t head_dim) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {2ull * head_dim, n_kv_heads, (cuuint64_t)total_blocks * BS};
+    const cuuint64_t strides[2] = {2ull * head_dim, 2ull * head_dim * n_kv_heads};
+    const cuuint32_t box[3] = {128u, 1u, (cuuint32_t)BS}, elem[3] = {1u, 1u, 1u};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, reinterpret_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Layout {
+    tkv_rows::Split own;                     // of the tokens behind the prefixes
+    uint32_t parts;                          // of the prefixes
+    uint64_t pre_ml, pre_o, own_plan, own_ml, own_o, bytes;   // offsets; the prefixes' plan is at 0
+};
+Layout layout_of(uint32_t n_seqs, uint32_t n_groups, uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t max_kv_len, uint32_t max_prefix_len) {
+    Layout l;
+    const uint64_t group = n_q_heads / n_kv_heads, nt = (max_prefix_len + KT - 1ull) / KT;
+    const uint64_t tiles = (n_groups + (uint64_t)n_seqs * group / 256) * n_kv_heads * nt;      // at most: every group ends in a row block of its own
+    l.parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(CTAS, (tiles + MIN_SHARE - 1) / MIN_SHARE));
+    l.own = tkv_rows::split_for((uint64_t)n_seqs * ((max_kv_len + 15ull) / 16), n_kv_heads, CTAS);
+    const uint64_t rows = 2ull * n_seqs * n_q_heads + 512ull * l.parts, slots = ((uint64_t)l.own.parts + n_seqs) * 2;   // two results per slot of an E4M3 pool
+    l.pre_ml = up(4ull * (n_groups + 2ull), 256);
+    l.pre_o = l.pre_ml + up(rows * 8, 256);
+    l.own_plan = l.pre_o + up(rows * head_dim * 4, 256);
+    l.own_ml = l.own_plan + up(4ull * (n_seqs + 2ull), 256);
+    l.own_o = l.own_ml + up(slots * n_q_heads * 8, 256);
+    l.bytes = l.own_o + slots * n_q_heads * head_dim * 4;
+    return l;
+}
+
+template <int D, bool FP8> cudaError_t launch_prefix(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, cudaStream_t st) {
+    constexpr size_t smem = CTRL_BYTES + 6 * (size_t)(D / 64) * GROUP_BYTES;
+    static_assert(smem + 4096 <= 227 * 1024, "shared memory of one CTA");
+    auto kernel = prefix_attn_tc<D, FP8>;
+    static std::atomic<uint64_t> granted{0};                    // devices on which this kernel may use that much shared memory
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
+    if (!(granted.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+        granted.fetch_or(bit, std::memory_order_relaxed);
+    }
+    kernel<<<a.parts, threads_of(FP8), smem, st>>>(mk, mv, a);
+    return cudaGetLastError();
+}
+template <int D> cudaError_t launch_join(const JoinArgs& a, cudaStream_t st) {
+    const uint64_t rows = (uint64_t)a.n_seqs * a.n_q_heads;
+    const bool few = rows <= 8ull * CTAS;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(few ? rows : (rows + 7) / 8));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return few ? cudaLaunchKernelEx(&cfg, prefix_join<D, 8>, a) : cudaLaunchKernelEx(&cfg, prefix_join<D, 1>, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t tkv_prefix_attn_scratch_bytes(uint32_t n_seqs, uint32_t n_groups, uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t max_kv_len,
+                                       uint32_t max_prefix_len) {
+    if (!n_seqs || !n_groups || !n_kv_heads || n_q_heads < n_kv_heads || max_kv_len > 0xFFFFFFF0u || max_prefix_len > 0xFFFFFFF0u) return 0;
+    return layout_of(n_seqs, n_groups, n_q_heads, n_kv_heads, head_dim, max_kv_len, max_prefix_len).bytes;
+}
+
+int32_t tkv_prefix_attn_enqueue(const TkvPool* pool, const TkvPrefixAttn* p, void* stream) {
+    if (!pool || !p) return fail(TKV_ERR_INVALID_CONFIG, "NULL argument");
+    if (pool->dtype != TKV_DTYPE_F16 && pool->dtype != TKV_DTYPE_E4M3)
+        return fail(TKV_ERR_INVALID_CONFIG, "shared-prefix attention reads F16 or E4M3 pools (dtype %llu)", (unsigned long long)pool->dtype);
+    if (pool->head_dim != 64 && pool->head_dim != 128)
+        return fail(TKV_ERR_DIMENSION_MISMATCH, "dimension mismatch: expected %llu, got %llu (shared-prefix attention is built for head_dim 64 and 128)", 128,
+                    pool->head_dim);
+    if (pool->block_size != BS)
+        return fail(TKV_ERR_DIMENSION_MISMATCH, "dimension mismatch: expected %llu, got %llu (tokens per block)", BS, pool->block_size);
+    if (p->layer >= pool->n_layers) return fail(TKV_ERR_INVALID_CONFIG, "layer %llu outside the pool (%llu layers)", p->layer, pool->n_layers);
+    if (!pool->n_kv_heads || !p->n_q_heads || p->n_q_heads % pool->n_kv_heads || p->n_q_heads / pool->n_kv_heads > 8)
+        return fail(TKV_ERR_DIMENSION_MISMATCH, "dimension mismatch: expected %llu, got %llu (query heads must be 1..8 times the kv heads)",
+                    pool->n_kv_heads, p->n_q_heads);
+    if (pool->n_kv_heads > CTAS * tkv_rows::WARPS) return fail(TKV_ERR_INVALID_CONFIG, "at most %llu kv heads (%llu)", CTAS * tkv_rows::WARPS, pool->n_kv_heads);
+    if ((pool->k_scales == 0) != (pool->v_scales == 0)) return fail(TKV_ERR_INVALID_CONFIG, "k_scales and v_scales must both be set or both be 0");
+    if (pool->k_scales && pool->dtype != TKV_DTYPE_E4M3) return fail(TKV_ERR_INVALID_CONFIG, "only an E4M3 pool carries scales");
+    if (!std::isfinite(p->sm_scale)) return fail(TKV_ERR_INVALID_CONFIG, "sm_scale is not finite");
+    if (p->n_seqs == 0 || p->n_groups == 0) return TKV_OK;
+    if (!p->q || !p->out || !p->tables || !p->kv_lens || !p->group_starts || !p->prefix_lens || !pool->k_layer_ptrs || !pool->v_layer_ptrs || !pool->total_blocks)
+        return fail(TKV_ERR_INVALID_CONFIG, "NULL buffer");
+    if (p->max_kv_len > 0xFFFFFFF0u || p->max_prefix_len > 0xFFFFFFF0u) return fail(TKV_ERR_INVALID_CONFIG, "length bounds above 2^32 - 16");
+    const uint64_t own_blocks = (uint64_t)p->n_seqs * ((p->max_kv_len + 15ull) / 16), group = p->n_q_heads / pool->n_kv_heads;
+    const uint64_t tiles = (p->n_groups + (uint64_t)p->n_seqs * group / 256) * pool->n_kv_heads * ((p->max_prefix_len + KT - 1ull) / KT);
+    if (own_blocks >= 0x7FFFFFFFull || tiles >= 0x7FFFFFFFull || (uint64_t)p->n_seqs * p->n_q_heads >= 0x7FFFFFFFull)
+        return fail(TKV_ERR_INVALID_CONFIG, "%llu sequences of %llu tokens: batch too large", p->n_seqs, p->max_kv_len);
+    if (std::max((p->max_kv_len + 15ull) / 16, (p->max_prefix_len + 15ull) / 16) > p->table_stride)
+        return fail(TKV_ERR_DIMENSION_MISMATCH, "dimension mismatch: expected %llu, got %llu (table_stride below the blocks of max_kv_len or max_prefix_len)",
+                    std::max((p->max_kv_len + 15ull) / 16, (p->max_prefix_len + 15ull) / 16), p->table_stride);
+    const bool fp8 = pool->dtype == TKV_DTYPE_E4M3;
+    if (!fp8 && (uint64_t)pool->total_blocks * BS >= 0x7FFFFFFFull) return fail(TKV_ERR_INVALID_CONFIG, "an F16 pool of %llu blocks is too large", pool->total_blocks);
+    const uint64_t kp = pool->k_layer_ptrs[p->layer], vp = pool->v_layer_ptrs[p->layer];
+    if (!kp || !vp) return fail(TKV_ERR_INVALID_CONFIG, "NULL buffer");
+    if ((kp | vp | p->q | p->out) % 16 || p->scratch % 256) return fail(TKV_ERR_INVALID_CONFIG, "layer tensors, q and out must be 16-byte aligned, scratch 256-byte");
+    if ((p->tables | p->kv_lens | p->group_starts | p->prefix_lens | p->status | pool->k_scales | pool->v_scales) % 4)
+        return fail(TKV_ERR_INVALID_CONFIG, "tables, lengths, groups, scales and status must be 4-byte aligned");
+    const Layout l = layout_of(p->n_seqs, p->n_groups, p->n_q_heads, pool->n_kv_heads, pool->head_dim, p->max_kv_len, p->max_prefix_len);
+    if (!p->scratch || p->scratch_bytes < l.bytes)
+        return fail(TKV_ERR_DIMENSION_MISMATCH, "dimension mismatch: expected %llu, got %llu (scratch bytes)", l.bytes, p->scratch ? p->scratch_bytes : 0);
+
+    const uint32_t es = fp8 ? 1u : 2u;
+    const size_t layer_scales = (size_t)p->layer * pool->total_blocks * pool->n_kv_heads;
+    const float scale_log2 = p->sm_scale * 1.4426950408889634f;
+    Args a{};
+    a.tables = reinterpret_cast<const uint32_t*>(p->tables);
+    a.kv_lens = reinterpret_cast<const uint32_t*>(p->kv_lens);
+    a.group_starts = reinterpret_cast<const uint32_t*>(p->group_starts);
+    a.prefix_lens = reinterpret_cast<const uint32_t*>(p->prefix_lens);
+    a.q = reinterpret_cast<const __half*>(p->q);
+    a.k8 = reinterpret_cast<const char*>(kp);
+    a.v8 = reinterpret_cast<const char*>(vp);
+    a.k_scales = pool->k_scales ? reinterpret_cast<const float*>(pool->k_scales) + layer_scales : nullptr;
+    a.v_scales = pool->v_scales ? reinterpret_cast<const float*>(pool->v_scales) + layer_scales : nullptr;
+    a.plan = reinterpret_cast<uint32_t*>(p->scratch);
+    a.part_ml = reinterpret_cast<float*>(p->scratch + l.pre_ml);
+    a.part_o = reinterpret_cast<float*>(p->scratch + l.pre_o);
+    a.status = reinterpret_cast<uint32_t*>(p->status);
+    a.row_stride = pool->n_kv_heads * pool->head_dim * es;
+    a.block_stride = (uint64_t)BS * a.row_stride;
+    a.n_seqs = p->n_seqs;
+    a.n_groups = p->n_groups;
+    a.n_q_heads = p->n_q_heads;
+    a.n_kv_heads = pool->n_kv_heads;
+    a.group = (uint32_t)group;
+    a.table_stride = p->table_stride;
+    a.max_kv_len = p->max_kv_len;
+    a.max_prefix_len = p->max_prefix_len;
+    a.total_blocks = pool->total_blocks;
+    a.parts = l.parts;
+    a.q_sign = scale_log2 < 0.0f ? 0x80008000u : 0u;
+    a.scale_log2 = std::fabs(scale_log2);
+
+    tkv_rows::Args r{};
+    r.k_base = a.k8;
+    r.v_base = a.v8;
+    r.k_scales = a.k_scales;
+    r.v_scales = a.v_scales;
+    r.q = a.q;
+    r.tables = a.tables;
+    r.kv_lens = a.kv_lens;
+    r.group_starts = a.group_starts;
+    r.prefix_lens = a.prefix_lens;
+    r.plan = reinterpret_cast<uint32_t*>(p->scratch + l.own_plan);
+    r.part_ml = reinterpret_cast<float*>(p->scratch + l.own_ml);
+    r.part_o = reinterpret_cast<float*>(p->scratch + l.own_o);
+    r.status = a.status;
+    r.block_stride = a.block_stride;
+    r.row_stride = a.row_stride;
+    r.n_seqs = a.n_seqs;
+    r.n_groups = a.n_groups;
+    r.n_q_heads = a.n_q_heads;
+    r.n_kv_heads = a.n_kv_heads;
+    r.group = a.group;
+    r.table_stride = a.table_stride;
+    r.max_kv_len = a.max_kv_len;
+    r.max_prefix_len = a.max_prefix_len;
+    r.total_blocks = a.total_blocks;
+    r.scale_log2 = scale_log2;
+
+    JoinArgs j{};
+    j.pre_o = a.part_o;
+    j.pre_ml = a.part_ml;
+    j.own_o = r.part_o;
+    j.own_ml = r.part_ml;
+    j.pre_plan = a.plan;
+    j.own_plan = r.plan;
+    j.kv_lens = a.kv_lens;
+    j.group_starts = a.group_starts;
+    j.prefix_lens = a.prefix_lens;
+    j.out = reinterpret_cast<__half*>(p->out);
+    j.n_seqs = a.n_seqs;
+    j.n_groups = a.n_groups;
+    j.n_q_heads = a.n_q_heads;
+    j.n_kv_heads = a.n_kv_heads;
+    j.group = a.group;
+    j.subs = tkv_rows::subs_of(fp8, false);
+
+    CUtensorMap mk{}, mv{};
+    if (!fp8 && (!make_map(&mk, kp, pool->total_blocks, pool->n_kv_heads, pool->head_dim) || !make_map(&mv, vp, pool->total_blocks, pool->n_kv_heads, pool->head_dim)))
+        return fail(TKV_ERR_CUDA, "shared-prefix attention: cannot describe the layer tensors to the copy engine");
+    int prev = -1;
+    cudaError_t e = cudaGetDevice(&prev);
+    if (e == cudaSuccess && prev != pool->device) e = cudaSetDevice(pool->device);
+    if (e == cudaSuccess) {
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (pool->head_dim == 128) e = fp8 ? launch_prefix<128, true>(mk, mv, a, st) : launch_prefix<128, false>(mk, mv, a, st);
+        else e = fp8 ? launch_prefix<64, true>(mk, mv, a, st) : launch_prefix<64, false>(mk, mv, a, st);
+        if (e == cudaSuccess) e = tkv_rows::launch_rows(pool->head_dim, fp8, false, r, l.own, st);
+        if (e == cudaSuccess) e = pool->head_dim == 128 ? launch_join<128>(j, st) : launch_join<64>(j, st);
+    }
+    if (prev >= 0 && prev != pool->device) cudaSetDevice(prev);
+    if (e != cudaSuccess) {
+        char buf[256];
+        snprintf(buf, sizeof buf, "shared-prefix attention launch: %s (cuda error %d)", cudaGetErrorString(e), (int)e);
+        return tkv_internal::set_error(TKV_ERR_CUDA, (int32_t)e, buf);
+    }
+    return TKV_OK;
+}
+
+}  // extern "C"

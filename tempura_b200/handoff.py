@@ -494,6 +494,46 @@ class ScoredDecodeAttention:
         return self.out
 
 
+class PrefixAttention:
+    """Decode attention of a batch in which groups of sequences share a prefix: the prefix's K and V are read once per group.
+    Sequences ``group_starts[g] .. group_starts[g + 1] - 1`` are group ``g``; their first ``prefix_lens[g]`` tokens (a multiple of the
+    block size) are in the blocks at the head of their table rows, the same for all of them.  ``kv_lens`` counts the prefix.  Rows of
+    ``out`` behind the last group are left alone (a padded batch).  ``q`` is f16 ``[n_seqs, n_q_heads, head_dim]``, ``tables`` int32
+    ``[n_seqs, table_stride]``, ``kv_lens`` int32 ``[n_seqs]``, ``group_starts`` int32 ``[n_groups + 1]``, ``prefix_lens`` int32
+    ``[n_groups]``, all on the pool's device and read when the kernels run.  Output and workspace are made once; enqueues of one
+    handle share the workspace and have to be ordered."""
+
+    def __init__(self, pool: Pool, q: torch.Tensor, tables: torch.Tensor, kv_lens: torch.Tensor, group_starts: torch.Tensor,
+                 prefix_lens: torch.Tensor, max_kv_len: int, max_prefix_len: int, sm_scale: Optional[float] = None):
+        _check_batch(pool, q, tables, kv_lens)
+        assert q.dtype == torch.float16
+        for t in (group_starts, prefix_lens):
+            assert t.dtype == torch.int32 and t.is_contiguous() and t.device == q.device
+        assert group_starts.numel() == prefix_lens.numel() + 1
+        n_seqs, n_q_heads, head_dim = q.shape
+        n_groups = prefix_lens.numel()
+        self.pool, self.q, self.tables, self.kv_lens, self.group_starts, self.prefix_lens = pool, q, tables, kv_lens, group_starts, prefix_lens
+        self.sm_scale = 1.0 / float(head_dim) ** 0.5 if sm_scale is None else sm_scale
+        self.out = torch.empty_like(q)
+        need = int(lib().tkv_prefix_attn_scratch_bytes(n_seqs, n_groups, n_q_heads, pool.n_kv_heads, head_dim, max_kv_len, max_prefix_len))
+        self.scratch = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=q.device)
+        self._pool_c = pool.c_struct()
+        self._args = {}
+        self._mk = lambda layer: N.TkvPrefixAttn(n_seqs, n_groups, n_q_heads, tables.shape[1], layer, max_kv_len, max_prefix_len, self.sm_scale,
+                                                 q.data_ptr(), self.out.data_ptr(), tables.data_ptr(), kv_lens.data_ptr(), group_starts.data_ptr(),
+                                                 prefix_lens.data_ptr(), self.scratch.data_ptr(), need, self.status.data_ptr())
+
+    def enqueue(self, layer: int, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+        if stream is None:
+            stream = torch.cuda.current_stream(self.pool.device)
+        args = self._args.get(layer)
+        if args is None:
+            args = self._args[layer] = C.byref(self._mk(layer))
+        check(lib().tkv_prefix_attn_enqueue(C.byref(self._pool_c), args, C.c_void_p(stream.cuda_stream)))
+        return self.out
+
+
 class CacheEviction:
     """Cuts the sequences of a batch to ``budget`` cached tokens by their accumulated attention weights
     (:class:`ScoredDecodeAttention`).  ``select`` chooses, per layer, sequence and kv head, the tokens that stay -- the first

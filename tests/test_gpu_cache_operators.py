@@ -306,3 +306,175 @@ def test_scored_attention_long_shares(H, dtype, kv_heads, head_dim, group):
         out_close(out[s], want, vmax, False)
         w = w.view(kv_heads, group, lens[s]).sum(dim=1)
         scores_close(scores[0, s, :, : lens[s]], w, torch.zeros_like(w))
+
+
+# ---- shared-prefix attention --------------------------------------------------------------------------------------------------------
+def grouped(sizes, prefixes, suffixes):
+    """(starts, prefix lengths, per-sequence (group, prefix blocks), lengths) of a batch; suffixes go round."""
+    starts, shared, lens = [0], [], []
+    for g, (n, p) in enumerate(zip(sizes, prefixes)):
+        for i in range(n):
+            shared.append((g, p // BS))
+            lens.append(max(0, p + suffixes[len(lens) % len(suffixes)]))
+        starts.append(starts[-1] + n)
+    return starts, shared, lens
+
+
+def prefix_case(H, dtype, kv_heads, head_dim, group, sizes, prefixes, suffixes, seed=0, pad=0, gain=2.0):
+    import torch
+    starts, shared, lens = grouped(sizes, prefixes, suffixes)
+    c = Cache(H, lens + [40] * pad, kv_heads, head_dim, dtype, layers=1, seed=seed, shared=shared + [None] * pad)
+    n = len(lens) + pad
+    q = (torch.randn((n, kv_heads * group, head_dim), generator=torch.Generator().manual_seed(seed + 1)) * gain).to(torch.float16)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+    width = max(c.tables.shape[1], max(prefixes) // BS)
+    tables = torch.full((n, width), -1, dtype=torch.int32)
+    tables[:, : c.tables.shape[1]] = c.tables
+    first = {}
+    for s, (g, blocks) in enumerate(shared):                          # a group's first row names the whole prefix, however short the member
+        first.setdefault(g, s)
+        longest = max((t for t in range(n - pad) if shared[t][0] == g), key=lambda t: lens[t])
+        if s == first[g]:
+            tables[s, :blocks] = c.tables[longest, :blocks]
+    attn = H.PrefixAttention(c.pool, q.cuda(), tables.cuda(), c.dev_lens, i32(starts), i32(prefixes), max(lens + [40]), max(prefixes))
+    return c, q, attn, lens
+
+
+@pytest.mark.parametrize("dtype", ["f16", "e4m3", "e4m3 unscaled"])
+@pytest.mark.parametrize("kv_heads,head_dim,group", [(8, 128, 4), (4, 64, 8), (1, 128, 1), (5, 128, 3), (3, 64, 2), (2, 128, 8), (2, 64, 7)])
+@pytest.mark.parametrize("sizes,prefixes,suffixes", [
+    ([3], [48], [1, 20, 5]),                                          # one short tile
+    ([1, 5, 2, 40], [16, 400, 0, 1040], [0, 7, 33, 100, 1]),          # uneven groups, one without a prefix, sequences with nothing of their own
+    ([70], [272], [17, 0, 3]),                                        # several row blocks for larger groups of heads
+    ([2, 2], [128, 256], [16, 64]),                                   # whole tiles
+])
+def test_prefix_attention(H, dtype, kv_heads, head_dim, group, sizes, prefixes, suffixes):
+    import torch
+    c, q, attn, lens = prefix_case(H, dtype, kv_heads, head_dim, group, sizes, prefixes, suffixes, seed=kv_heads + head_dim + len(sizes))
+    attn.out.fill_(float("nan"))
+    out = attn.enqueue(0)
+    assert int(attn.status.item()) == 0
+    for s, (want, _, vmax) in enumerate(c.attention(0, q, attn.sm_scale)):
+        out_close(out[s], want, vmax, False)
+    again = out.clone()
+    attn.enqueue(0)
+    assert torch.equal(attn.out, again)                               # no atomics: the same bits every time
+
+
+@pytest.mark.parametrize("dtype", ["f16", "e4m3"])
+def test_prefix_attention_long_prefix(H, dtype):
+    """More cached tiles than CTAs, shares that begin and end inside items, two row blocks of which the second is short."""
+    c, q, attn, lens = prefix_case(H, dtype, 2, 128, 8, [40, 3], [9008, 4096], [40, 0, 100], seed=3)
+    out = attn.enqueue(0)
+    assert int(attn.status.item()) == 0
+    for s, (want, _, vmax) in enumerate(c.attention(0, q, attn.sm_scale)):
+        out_close(out[s], want, vmax, False)
+
+
+def test_prefix_attention_leaves_padded_rows_and_serves_short_members(H):
+    """Rows behind the last group stay as they were; a member shorter than its group's prefix, or empty, gets its own tokens only."""
+    import torch
+    starts, shared, lens = grouped([4], [64], [10])
+    lens = [74, 40, 0, 64]
+    c = Cache(H, lens + [40, 40], 2, 64, "f16", seed=4, shared=shared + [None, None])
+    q = torch.randn((6, 8, 64), generator=torch.Generator().manual_seed(1)).to(torch.float16)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+    attn = H.PrefixAttention(c.pool, q.cuda(), c.dev_tables, c.dev_lens, i32([0, 4]), i32([64]), 74, 64)
+    attn.out.fill_(7.5)
+    out = attn.enqueue(0)
+    assert int(attn.status.item()) == 0
+    assert (out[4:] == 7.5).all()
+    for s, (want, _, vmax) in enumerate(c.attention(0, q, attn.sm_scale)[:4]):
+        out_close(out[s], want, vmax, False)
+    assert (out[2] == 0).all()
+
+
+def test_prefix_attention_equals_decode_attention_without_groups_of_more_than_one(H):
+    """Every sequence its own group: what the plain decode attention computes, to both kernels' rounding."""
+    import torch
+    c, q, attn, lens = prefix_case(H, "f16", 8, 128, 4, [1] * 9, [16 * (s % 5) for s in range(9)], [30, 5], seed=6)
+    out = attn.enqueue(0).float()
+    ref = H.decode_attention(c.pool, 0, q.float().cuda(), c.dev_tables, c.dev_lens)
+    for s, (want, _, vmax) in enumerate(c.attention(0, q, attn.sm_scale)):
+        out_close(out[s], want, vmax, False)
+    assert (out - ref).abs().max() < 2e-2
+
+
+def test_prefix_attention_in_a_graph_with_changing_groups(H):
+    """Captured once; lengths, groups and prefixes change in place between replays."""
+    import torch
+    c, q, attn, lens = prefix_case(H, "f16", 4, 64, 4, [3, 4], [96, 64], [20, 9], seed=8)
+    attn.enqueue(0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attn.enqueue(0)
+    attn.out.zero_()
+    graph.replay()
+    for s, (want, _, vmax) in enumerate(c.attention(0, q, attn.sm_scale)):
+        out_close(attn.out[s], want, vmax, False)
+    attn.prefix_lens.copy_(torch.tensor([48, 0], dtype=torch.int32))  # a shorter shared part is as right
+    attn.group_starts.copy_(torch.tensor([0, 3, 6], dtype=torch.int32))
+    attn.out.fill_(3.0)
+    graph.replay()
+    for s, (want, _, vmax) in enumerate(c.attention(0, q, attn.sm_scale)[:6]):
+        out_close(attn.out[s], want, vmax, False)
+    assert (attn.out[6] == 3.0).all()
+
+
+def test_prefix_attention_negative_scale_and_equal_scores(H):
+    import torch
+    c, q, attn, lens = prefix_case(H, "f16", 2, 64, 2, [3], [160], [5], seed=9)
+    neg = H.PrefixAttention(c.pool, attn.q, attn.tables, attn.kv_lens, attn.group_starts, attn.prefix_lens, max(lens), 160, sm_scale=-0.2)
+    out = neg.enqueue(0)
+    for s, (want, _, vmax) in enumerate(c.attention(0, q, -0.2)):
+        out_close(out[s], want, vmax, False)
+    flat = H.PrefixAttention(c.pool, attn.q, attn.tables, attn.kv_lens, attn.group_starts, attn.prefix_lens, max(lens), 160, sm_scale=0.0)
+    out = flat.enqueue(0)
+    for s, (want, _, vmax) in enumerate(c.attention(0, q, 0.0)):
+        out_close(out[s], want, vmax, False)
+
+
+def test_prefix_attention_reports_what_it_cannot_trust(H):
+    import torch
+    c, q, attn, lens = prefix_case(H, "f16", 2, 64, 2, [2, 2], [64, 32], [9], seed=10)
+    good = attn.enqueue(0).clone()
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+
+    def run(**kw):
+        args = dict(tables=attn.tables, kv_lens=attn.kv_lens, group_starts=attn.group_starts, prefix_lens=attn.prefix_lens)
+        args.update(kw)
+        a = H.PrefixAttention(c.pool, attn.q, args["tables"], args["kv_lens"], args["group_starts"], args["prefix_lens"], max(lens), 64)
+        a.out.fill_(5.0)
+        a.enqueue(0)
+        return int(a.status.item()), a.out
+    assert run()[0] == 0
+    for kw in ({"group_starts": i32([0, 3, 2])}, {"group_starts": i32([0, 2, 5])}, {"prefix_lens": i32([64, 40])}, {"prefix_lens": i32([80, 32])}):
+        code, out = run(**kw)
+        assert code == N.ERR_INVALID_CONFIG and (out == 5.0).all(), kw     # nothing is computed
+    bad = attn.tables.clone()
+    bad[0, 1] = 1 << 24                                                # a prefix block outside the pool
+    assert run(tables=bad)[0] == N.ERR_INVALID_CONFIG
+    bad = attn.tables.clone()
+    bad[3, 2] = -5                                                     # one behind the prefix
+    assert run(tables=bad)[0] == N.ERR_INVALID_CONFIG
+    code, out = run(kv_lens=i32([lens[0], 100000, lens[2], lens[3]]))
+    assert code == N.ERR_INVALID_CONFIG
+    assert torch.equal(run()[1], good)                                 # the context is still usable
+
+
+def test_prefix_attention_refusals(H):
+    import ctypes
+    c, q, attn, lens = prefix_case(H, "f16", 2, 64, 2, [2], [32], [9], seed=11)
+
+    def code(change):
+        args = attn._mk(0)
+        for name, value in change.items():
+            setattr(args, name, value)
+        return N.lib().tkv_prefix_attn_enqueue(ctypes.byref(attn._pool_c), ctypes.byref(args), None)
+    assert code({}) == 0 and code({"n_seqs": 0}) == 0 and code({"n_groups": 0}) == 0
+    for change in ({"layer": 1}, {"q": 0}, {"out": 0}, {"tables": 0}, {"kv_lens": 0}, {"group_starts": 0}, {"prefix_lens": 0},
+                   {"sm_scale": float("nan")}, {"q": attn.q.data_ptr() + 8}, {"scratch": attn.scratch.data_ptr() + 16}):
+        assert code(change) == N.ERR_INVALID_CONFIG, change
+    for change in ({"n_q_heads": 3}, {"n_q_heads": 18}, {"table_stride": 2}, {"max_prefix_len": 64}, {"scratch_bytes": 100}, {"scratch": 0}):
+        assert code(change) == N.ERR_DIMENSION_MISMATCH, change
