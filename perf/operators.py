@@ -342,7 +342,7 @@ def _handle(state):
                                 pointers(k), pointers(v), ks, vs)
     if case["op"] == "prefix":
         return H.PrefixAttention(pool, state["q"], state["tables"], state["lens"], state["starts"], state["prefix"], state["max_len"],
-                                 case["prefix_hi"], sm_scale=state["sm_scale"])
+                                 max(state["plan"]["prefix"]), sm_scale=state["sm_scale"])
     if case["op"] == "scored":
         return H.ScoredDecodeAttention(pool, state["q"], state["tables"], state["lens"], state["scores"], state["max_len"],
                                        sm_scale=state["sm_scale"], decay=case["decay"])
