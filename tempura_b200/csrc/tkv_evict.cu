@@ -4,8 +4,8 @@
 // Select.  Of a row of `len` tokens the first `protect`, the last `recent` and the best-scored others stay, together
 //     new_len = min(len, max(budget, protect + recent)),
 // ties to the lower index.  Scores become 32-bit keys that compare like the numbers (NaN below everything, -0 = +0); the key that
-// the last kept token has is found by three histograms over 11, 11 and 10 bits of it, each over the tokens whose higher bits
-// agree with what is known, and a last pass writes the indices in ascending order (ballots inside a warp, prefix sums across warps
+// the last kept token has is found by histograms over 11, 11 and 10 bits of it, each over the tokens whose higher bits
+// agree with what is known; once these are few, one warp finishes bit by bit in registers.  A last pass writes the indices in ascending order (ballots inside a warp, prefix sums across warps
 // and CTAs).  Scores are read once into shared memory; the bound is HBM for many rows and latency for few, so a row is split over a
 // thread-block cluster, whose CTAs add their histograms through distributed shared memory, where there are fewer rows than SMs.
 //
@@ -36,8 +36,8 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int BS = 16;
-constexpr int SEL_THREADS = 512, SEL_WARPS = SEL_THREADS / 32;
 constexpr int BINS = 2048;
+constexpr int FEW = 256;                     // tokens that one warp holds in registers
 constexpr uint32_t STAGE_TOKENS = 49152;     // tokens of a row that a CTA keeps in shared memory; longer slices are read again in every pass
 constexpr uint32_t MAX_CLUSTER = 8;
 
@@ -66,13 +66,16 @@ __device__ __forceinline__ uint32_t key_of(float x) {
     return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
 
-__global__ void __launch_bounds__(SEL_THREADS) evict_select(const SelectArgs a) {
+template <int THREADS> __global__ void __launch_bounds__(THREADS) evict_select(const SelectArgs a) {
+    constexpr int WARPS = THREADS / 32, PER_THREAD = BINS / THREADS;
+    static_assert(BINS % (4 * THREADS) == 0, "every thread clears the same number of bins");
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t parts = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t row = blockIdx.x / parts, s = (row / a.n_kv_heads) % a.n_seqs;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, below = (1u << lane) - 1u;
     extern __shared__ uint32_t keys[];
-    __shared__ uint32_t hist[BINS], warp_sum[SEL_WARPS], chosen[2], n_gt[SEL_WARPS + 1], n_eq[SEL_WARPS + 1];
+    __shared__ __align__(16) uint32_t hist[BINS];
+    __shared__ uint32_t warp_sum[WARPS], chosen[4], n_gt[WARPS + 1], n_eq[WARPS + 1], few[FEW];
 
     uint32_t len = a.kv_lens[s];
     if (len > a.max_kv_len) {
@@ -87,19 +90,17 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select(const SelectArgs a) 
     uint32_t* out = a.kept + (size_t)row * a.kept_stride;
     if (n_new == len) {
         if (!fits && tid == 0) report_bad(a.status);
-        for (uint32_t i = rank * SEL_THREADS + tid; i < min(len, a.kept_stride); i += parts * SEL_THREADS) out[i] = i;
+        for (uint32_t i = rank * THREADS + tid; i < min(len, a.kept_stride); i += parts * THREADS) out[i] = i;
         return;
     }
     const uint32_t lo = protect, n_mid = len - a.recent - protect, need = n_new - protect - a.recent;   // need < n_mid
-    for (uint32_t i = rank * SEL_THREADS + tid; i < protect + a.recent; i += parts * SEL_THREADS)
+    for (uint32_t i = rank * THREADS + tid; i < protect + a.recent; i += parts * THREADS)
         out[i < protect ? i : need + i] = i < protect ? i : len - a.recent + (i - protect);
     if (need == 0) return;
 
     // ---- this CTA's slice of the tokens to choose from ----
     const uint32_t per = (n_mid + parts - 1) / parts, begin = min(n_mid, rank * per), n = min(per, n_mid - begin);
     const float* src = a.scores + (size_t)row * a.score_stride + lo + begin;
-    if (a.staged)
-        for (uint32_t i = tid; i < n; i += SEL_THREADS) keys[i] = key_of(src[i]);
     auto key_at = [&](uint32_t i) { return a.staged ? keys[i] : key_of(src[i]); };
 
     // ---- the key of the last token that stays ----
@@ -107,23 +108,39 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select(const SelectArgs a) 
     for (int pass = 0; pass < 3; pass++) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const uint32_t digit_mask = pass == 2 ? 1023u : 2047u;
-        for (uint32_t i = tid; i < BINS; i += SEL_THREADS) hist[i] = 0;
+#pragma unroll
+        for (int i = 0; i < BINS / 4; i += THREADS) reinterpret_cast<uint4*>(hist)[i + tid] = make_uint4(0, 0, 0, 0);
+        if (tid == 0) chosen[2] = 0;
         __syncthreads();
-        for (uint32_t i = tid; i < n; i += SEL_THREADS) {
-            const uint32_t k = key_at(i);
-            if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & digit_mask], 1u);
+        if (pass == 0) {                                        // the scores are read here
+#pragma unroll 4
+            for (uint32_t i = tid; i < n; i += THREADS) {
+                const uint32_t k = key_of(src[i]);
+                if (a.staged) keys[i] = k;
+                atomicAdd(&hist[k >> 21], 1u);
+            }
+        } else {
+            for (uint32_t i = tid; i < n; i += THREADS) {
+                const uint32_t k = key_at(i);
+                if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & digit_mask], 1u);
+            }
         }
         if (parts > 1) cluster.sync();
         else __syncthreads();
-        // thread t has bins 4t .. 4t + 3 of all CTAs, from the top: bin BINS - 1 - 4t first
-        uint32_t c[4], sum = 0;
+        // thread t has the bins from BINS - 1 - PER_THREAD * t downwards, of all CTAs
+        uint32_t c[PER_THREAD], sum = 0;
+        const uint32_t bin0 = BINS - PER_THREAD * (tid + 1);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t bin = BINS - 1 - (4 * tid + i);
-            c[i] = 0;
-            for (uint32_t r = 0; r < parts; r++) c[i] += parts > 1 ? *cluster.map_shared_rank(&hist[bin], r) : hist[bin];
-            sum += c[i];
+        for (int i = 0; i < PER_THREAD; i++) c[i] = hist[bin0 + PER_THREAD - 1 - i];
+        if (parts > 1) {
+            for (uint32_t r = 1; r < parts; r++) {
+                const uint32_t* other = cluster.map_shared_rank(hist, (rank + r) % parts);
+#pragma unroll
+                for (int i = 0; i < PER_THREAD; i++) c[i] += other[bin0 + PER_THREAD - 1 - i];
+            }
         }
+#pragma unroll
+        for (int i = 0; i < PER_THREAD; i++) sum += c[i];
         uint32_t incl = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -133,65 +150,117 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select(const SelectArgs a) 
         if (lane == 31) warp_sum[warp] = incl;
         __syncthreads();
         uint32_t above = incl - sum;
-        for (uint32_t w = 0; w < warp; w++) above += warp_sum[w];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (above < left && left <= above + c[i]) {         // one bin of one thread
-                chosen[0] = BINS - 1 - (4 * tid + i);
-                chosen[1] = above;
+        for (int w = 0; w < WARPS; w++) above += w < (int)warp ? warp_sum[w] : 0u;
+        if (above < left && left <= above + sum) {              // one thread
+#pragma unroll
+            for (int i = 0; i < PER_THREAD; i++) {
+                if (above < left && left <= above + c[i]) {
+                    chosen[0] = bin0 + PER_THREAD - 1 - i;
+                    chosen[1] = above;
+                    chosen[3] = c[i];
+                }
+                above += c[i];
             }
-            above += c[i];
         }
         if (parts > 1) cluster.sync();                          // nobody reads this histogram any more
         else __syncthreads();
         prefix |= chosen[0] << shift;
         mask |= digit_mask << shift;
         left -= chosen[1];
+        const uint32_t in_bin = chosen[3];
+        if (pass == 2) break;
+        if (parts == 1 && in_bin <= (uint32_t)FEW) {
+            // few tokens share the known bits: they are gathered and one warp finds the rest of the key, bit by bit, in registers
+            for (uint32_t i0 = warp * 32; i0 < n; i0 += THREADS) {
+                const uint32_t i = i0 + lane, k = i < n ? key_at(i) : 0u;
+                const bool hit = i < n && (k & mask) == prefix;
+                const uint32_t m = __ballot_sync(0xFFFFFFFFu, hit);
+                if (m) {
+                    uint32_t at = 0;
+                    if (lane == 0) at = atomicAdd(&chosen[2], (uint32_t)__popc(m));
+                    at = __shfl_sync(0xFFFFFFFFu, at, 0);
+                    if (hit) few[at + __popc(m & below)] = k;
+                }
+            }
+            __syncthreads();
+            if (warp == 0) {
+                uint32_t k[FEW / 32];
+#pragma unroll
+                for (int q = 0; q < FEW / 32; q++) k[q] = q * 32 + lane < in_bin ? few[q * 32 + lane] : ~prefix;   // ~prefix never matches
+                for (int b = shift - 1; b >= 0; b--) {
+                    const uint32_t bit = 1u << b, want = prefix | bit;
+                    mask |= bit;
+                    uint32_t ones = 0;
+#pragma unroll
+                    for (int q = 0; q < FEW / 32; q++) ones += __popc(__ballot_sync(0xFFFFFFFFu, (k[q] & mask) == want));
+                    if (left <= ones) prefix = want;
+                    else left -= ones;
+                }
+                if (lane == 0) {
+                    chosen[0] = prefix;
+                    chosen[1] = left;
+                }
+            }
+            __syncthreads();
+            prefix = chosen[0];
+            left = chosen[1];
+            break;
+        }
         __syncthreads();
     }
 
     // ---- indices in ascending order: keys above `prefix`, and the first `left` that equal it ----
-    const uint32_t seg = ((n + SEL_WARPS - 1) / SEL_WARPS + 31) / 32 * 32, w0 = min(n, warp * seg), w1 = min(n, w0 + seg);
+    const uint32_t seg = ((n + WARPS - 1) / WARPS + 31) / 32 * 32, w0 = min(n, warp * seg), w1 = min(n, w0 + seg);
     uint32_t gt = 0, eq = 0;
-    for (uint32_t i0 = w0; i0 < w1; i0 += 32) {
-        const uint32_t i = i0 + lane, k = i < w1 ? key_at(i) : 0u;
-        gt += __popc(__ballot_sync(0xFFFFFFFFu, i < w1 && k > prefix));
-        eq += __popc(__ballot_sync(0xFFFFFFFFu, i < w1 && k == prefix));
+    for (uint32_t i = w0 + lane; i < w1; i += 32) {
+        const uint32_t k = key_at(i);
+        gt += k > prefix;
+        eq += k == prefix;
     }
+    gt = __reduce_add_sync(0xFFFFFFFFu, gt);
+    eq = __reduce_add_sync(0xFFFFFFFFu, eq);
     if (lane == 0) {
         n_gt[warp] = gt;
         n_eq[warp] = eq;
     }
     __syncthreads();
-    if (tid == 0) {
-        uint32_t g = 0, e = 0;
-        for (int w = 0; w < SEL_WARPS; w++) {
-            g += n_gt[w];
-            e += n_eq[w];
-        }
-        n_gt[SEL_WARPS] = g;
-        n_eq[SEL_WARPS] = e;
-    }
-    if (parts > 1) cluster.sync();
-    else __syncthreads();
     uint32_t gt_before = 0, eq_before = 0;
-    for (uint32_t r = 0; r < rank; r++) {
-        gt_before += *cluster.map_shared_rank(&n_gt[SEL_WARPS], r);
-        eq_before += *cluster.map_shared_rank(&n_eq[SEL_WARPS], r);
+    if (parts > 1) {
+        if (tid == 0) {
+            uint32_t g = 0, e = 0;
+            for (int w = 0; w < WARPS; w++) {
+                g += n_gt[w];
+                e += n_eq[w];
+            }
+            n_gt[WARPS] = g;
+            n_eq[WARPS] = e;
+        }
+        cluster.sync();
+        for (uint32_t r = 0; r < rank; r++) {
+            gt_before += *cluster.map_shared_rank(&n_gt[WARPS], r);
+            eq_before += *cluster.map_shared_rank(&n_eq[WARPS], r);
+        }
     }
-    for (uint32_t w = 0; w < warp; w++) {
-        gt_before += n_gt[w];
-        eq_before += n_eq[w];
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) {
+        gt_before += w < (int)warp ? n_gt[w] : 0u;
+        eq_before += w < (int)warp ? n_eq[w] : 0u;
     }
-    uint32_t at = lo + gt_before + min(eq_before, left);
+    uint32_t* at = out + lo + gt_before + min(eq_before, left);
+    uint32_t eq_left = left - min(eq_before, left);             // of the keys that equal `prefix`, those still to come stay
+    const uint32_t first = lo + begin;
     for (uint32_t i0 = w0; i0 < w1; i0 += 32) {
         const uint32_t i = i0 + lane, k = i < w1 ? key_at(i) : 0u;
+        bool keep = i < w1 && k > prefix;
         const uint32_t m_eq = __ballot_sync(0xFFFFFFFFu, i < w1 && k == prefix);
-        const bool keep = i < w1 && (k > prefix || (k == prefix && eq_before + __popc(m_eq & below) < left));
+        if (m_eq) {
+            if ((m_eq >> lane & 1u) && (uint32_t)__popc(m_eq & below) < eq_left) keep = true;
+            eq_left -= min((uint32_t)__popc(m_eq), eq_left);
+        }
         const uint32_t m_keep = __ballot_sync(0xFFFFFFFFu, keep);
-        if (keep) out[at + __popc(m_keep & below)] = lo + begin + i;
+        if (keep) at[__popc(m_keep & below)] = first + i;
         at += __popc(m_keep);
-        eq_before += __popc(m_eq);
     }
     if (parts > 1) cluster.sync();                              // a CTA's counts may still be read by its neighbours
 }
@@ -385,11 +454,13 @@ int32_t tkv_evict_select_enqueue(const TkvEvictSelect* p, void* stream) {
     if (e == cudaSuccess && prev != p->device) e = cudaSetDevice(p->device);
     if (e == cudaSuccess) {
         const size_t smem = a.staged ? (size_t)slice * 4 : 0;
-        if (smem > 32 * 1024) e = cudaFuncSetAttribute(evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(STAGE_TOKENS * 4));
+        const bool large = slice > 8192;                        // 256 threads take short slices eight rows to an SM
+        auto kernel = large ? evict_select<512> : evict_select<256>;
+        if (smem > 32 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(STAGE_TOKENS * 4));
         if (e == cudaSuccess) {
             cudaLaunchConfig_t cfg{};
             cfg.gridDim = dim3((unsigned)(rows * cluster));
-            cfg.blockDim = dim3(SEL_THREADS);
+            cfg.blockDim = dim3(large ? 512 : 256);
             cfg.dynamicSmemBytes = smem;
             cfg.stream = static_cast<cudaStream_t>(stream);
             cudaLaunchAttribute at[1];
@@ -398,7 +469,7 @@ int32_t tkv_evict_select_enqueue(const TkvEvictSelect* p, void* stream) {
             at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
             cfg.attrs = at;
             cfg.numAttrs = 1;
-            e = cudaLaunchKernelEx(&cfg, evict_select, a);
+            e = cudaLaunchKernelEx(&cfg, kernel, a);
         }
     }
     if (prev >= 0 && prev != p->device) cudaSetDevice(prev);

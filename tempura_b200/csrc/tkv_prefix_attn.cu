@@ -172,6 +172,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             a.plan[1 + a.n_groups] = total;
         }
     }
+    asm volatile("griddepcontrol.launch_dependents;");          // the kernel for the tokens behind the prefixes may start where SMs are free
     if ((uint64_t)blockIdx.x * share >= total) return;
     const uint32_t u_begin = blockIdx.x * share, u_end = min(total, u_begin + share);
 
@@ -425,7 +426,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 if (!ok) break;
                 if (warp_live) {
                     tc_fence_after();
-                    constexpr int CH = FP8 ? 64 : 128;          // scores held in registers; an E4M3 pool's are read twice
+                    constexpr int CH = 64;                      // scores held in registers; they are read twice (all 128 do not fit beside the rest)
                     const int left = (int)min(limit > t0 ? limit - t0 : 0u, (uint32_t)KT);   // tokens of the tile that the row attends to
                     auto tile = [&](auto masked_type) {
                     constexpr bool MASKED = decltype(masked_type)::value;
@@ -880,7 +881,7 @@ int32_t tkv_prefix_attn_enqueue(const TkvPool* pool, const TkvPrefixAttn* p, voi
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         if (pool->head_dim == 128) e = fp8 ? launch_prefix<128, true>(mk, mv, a, st) : launch_prefix<128, false>(mk, mv, a, st);
         else e = fp8 ? launch_prefix<64, true>(mk, mv, a, st) : launch_prefix<64, false>(mk, mv, a, st);
-        if (e == cudaSuccess) e = tkv_rows::launch_rows(pool->head_dim, fp8, false, r, l.own, st);
+        if (e == cudaSuccess) e = tkv_rows::launch_rows(pool->head_dim, fp8, false, r, l.own, true, st);
         if (e == cudaSuccess) e = pool->head_dim == 128 ? launch_join<128>(j, st) : launch_join<64>(j, st);
     }
     if (prev >= 0 && prev != pool->device) cudaSetDevice(prev);

@@ -187,6 +187,7 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
                 report(a.status, 2u);
                 if (blockIdx.x == 0) a.plan[0] = 0;             // nothing was computed
             }
+            asm volatile("griddepcontrol.wait;" ::: "memory");
             return;
         }
     }
@@ -379,6 +380,8 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
                 for (uint32_t it = 0; it < (1u << 17); it++)
                     if (bar_test(smem_addr(&full[x][k % a.stages]), (k / a.stages) & 1u)) break;
         }
+        // Launched beside the kernel before it (shared-prefix attention), this grid ends after that one: whoever waits for this grid has both.
+        asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
 
@@ -650,7 +653,8 @@ inline Split split_for(uint64_t blocks, uint32_t n_kv_heads, uint32_t ctas) {
     return s;
 }
 
-template <int D, bool FP8, bool F32, bool WIDE> cudaError_t launch_one(Args a, const Split& sp, cudaStream_t st) {
+// beside: the launch does not wait for the kernel before it on the stream, which has to be one that this one does not read from
+template <int D, bool FP8, bool F32, bool WIDE> cudaError_t launch_one(Args a, const Split& sp, bool beside, cudaStream_t st) {
     using S = Shape<D, FP8>;
     a.heads = sp.heads;
     a.streams = sp.streams;
@@ -672,17 +676,26 @@ template <int D, bool FP8, bool F32, bool WIDE> cudaError_t launch_one(Args a, c
         if (e != cudaSuccess) return e;
         granted.fetch_or(bit, std::memory_order_relaxed);
     }
-    kernel<<<sp.grid, threads_of(FP8, F32), smem, st>>>(a);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(sp.grid);
+    cfg.blockDim = dim3(threads_of(FP8, F32));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = beside ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
 }
-template <int D, bool FP8> cudaError_t launch_type(bool f32, const Args& a, const Split& sp, cudaStream_t st) {
+template <int D, bool FP8> cudaError_t launch_type(bool f32, const Args& a, const Split& sp, bool beside, cudaStream_t st) {
     const bool wide = a.group > 4;
-    if (f32) return wide ? launch_one<D, FP8, true, true>(a, sp, st) : launch_one<D, FP8, true, false>(a, sp, st);
-    return wide ? launch_one<D, FP8, false, true>(a, sp, st) : launch_one<D, FP8, false, false>(a, sp, st);
+    if (f32) return wide ? launch_one<D, FP8, true, true>(a, sp, beside, st) : launch_one<D, FP8, true, false>(a, sp, beside, st);
+    return wide ? launch_one<D, FP8, false, true>(a, sp, beside, st) : launch_one<D, FP8, false, false>(a, sp, beside, st);
 }
-inline cudaError_t launch_rows(uint32_t head_dim, bool fp8, bool f32, const Args& a, const Split& sp, cudaStream_t st) {
-    if (head_dim == 128) return fp8 ? launch_type<128, true>(f32, a, sp, st) : launch_type<128, false>(f32, a, sp, st);
-    return fp8 ? launch_type<64, true>(f32, a, sp, st) : launch_type<64, false>(f32, a, sp, st);
+inline cudaError_t launch_rows(uint32_t head_dim, bool fp8, bool f32, const Args& a, const Split& sp, bool beside, cudaStream_t st) {
+    if (head_dim == 128) return fp8 ? launch_type<128, true>(f32, a, sp, beside, st) : launch_type<128, false>(f32, a, sp, beside, st);
+    return fp8 ? launch_type<64, true>(f32, a, sp, beside, st) : launch_type<64, false>(f32, a, sp, beside, st);
 }
 
 }  // namespace tkv_rows

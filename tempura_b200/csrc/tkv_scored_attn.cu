@@ -342,7 +342,7 @@ int32_t tkv_scored_attn_enqueue(const TkvPool* pool, const TkvScoredAttn* p, voi
     if (e == cudaSuccess) {
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         const bool f32 = p->q_dtype == TKV_DTYPE_F32;
-        e = tkv_rows::launch_rows(pool->head_dim, es == 1, f32, a, l.split, st);
+        e = tkv_rows::launch_rows(pool->head_dim, es == 1, f32, a, l.split, false, st);
         if (e == cudaSuccess) {
             const unsigned grid = (unsigned)finish_grid;
             if (pool->head_dim == 128) e = f32 ? launch_finish<128, true>(f, grid, st) : launch_finish<128, false>(f, grid, st);
