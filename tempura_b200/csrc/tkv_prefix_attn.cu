@@ -66,11 +66,11 @@ struct Args {
 
 __host__ __device__ constexpr int softmax_warps() { return 8; }
 __host__ __device__ constexpr int feed_warps(bool fp8) { return fp8 ? 4 : 1; }
-__host__ __device__ constexpr int threads_of(bool fp8) { return (softmax_warps() + feed_warps(fp8) + 1) * 32; }
+__host__ __device__ constexpr int threads_of(bool fp8) { return (softmax_warps() + feed_warps(fp8) + 2) * 32; }   // and an MMA issuer per stream
 
 struct Control {
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t q_ready[2], s_full[2], p_full[2], pv_done[2], drained;
+    uint64_t q_ready[2], s_full[2], p_full[2], pv_done[2], drained[2];
     uint32_t tmem, fail;
     float scales[4][16];                     // per cached tile (mod 4): K scales of its 8 blocks, V scales
 };
@@ -86,6 +86,11 @@ struct Item {
 __device__ __forceinline__ uint32_t row_blocks(uint32_t rows) { return (rows + 255) / 256; }
 
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) { mma<false>(d, a, b, idesc, acc); }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0;
+}
 // A operand from tensor memory: lane = row, two F16 of the row per column
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
@@ -141,14 +146,15 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         for (int i = 0; i < 2; i++) {
             mbar_init(c->k_full + i, FP8 ? FEED : 1);
             mbar_init(c->v_full + i, FP8 ? FEED : 1);
-            mbar_init(c->k_empty + i, 1);
-            mbar_init(c->v_empty + i, 1);
+            mbar_init(c->k_empty + i, 2);
+            mbar_init(c->v_empty + i, 2);
             mbar_init(c->q_ready + i, SM / 2);
             mbar_init(c->s_full + i, 1);
             mbar_init(c->p_full + i, SM / 2);
             mbar_init(c->pv_done + i, 1);
         }
-        mbar_init(&c->drained, 1);
+        mbar_init(c->drained, 1);
+        mbar_init(c->drained + 1, 1);
         c->fail = (smem_u32(smem) & 1023u) ? 2u : 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -224,64 +230,47 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         n_of[0] = same_rows ? (it.n_tiles + 1) / 2 : it.n_tiles;
         n_of[1] = same_rows ? it.n_tiles / 2 : it.n_tiles;
 
-        if (warp == SM + FEED) {
-            // ---- MMA issuer: whichever stream is ready goes next ----
-            if (lane == 0) {
-                const uint32_t q_lo = smem_u32(q_tile) >> 4, k_lo = smem_u32(k_ring) >> 4, v_lo = smem_u32(v_ring) >> 4;
-                uint32_t jq[2] = {0, 0}, jp[2] = {0, 0}, k_left[2] = {0, 0}, v_left[2] = {0, 0}, idle = 0;
-                const uint32_t readers = same_rows ? 1u : 2u;
-                for (int x = 0; x < 2 && ok; x++) ok = bar_wait(smem_u32(c->q_ready + x), item_no & 1u, fail);
-                while (ok && (jp[0] < n_of[0] || jp[1] < n_of[1])) {
-                    bool did = false;
+        if (warp >= SM + FEED) {
+            // ---- MMA issuers, a warp per stream.  Waits sleep in hardware (a polling issuer took issue slots from the softmax warps of its
+            // scheduler and held the tile up by 1 000 cycles), and the warp issues together through an elected lane. ----
+            const uint32_t x = warp - (SM + FEED), n_x = x ? n_of[1] : n_of[0], pv_x = x ? n_pv[1] : n_pv[0];
+            const uint32_t q_lo = (smem_u32(q_tile) >> 4) + x * (TILE >> 4), k_lo = smem_u32(k_ring) >> 4, v_lo = smem_u32(v_ring) >> 4;
+            const uint32_t ts = tmem + TM_S + x * 128, to = tmem + TM_O + x * 128;
+            auto wait = [&](uint64_t* bar, uint32_t parity) {
+                if (ok) ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(bar), parity & 1u, fail));
+            };
+            wait(c->q_ready + x, item_no);
+            for (uint32_t j = 0; j < n_x && ok; j++) {
+                const uint32_t i = same_rows ? 2 * j + x : j, t = tiles_done + i, st = t & 1u, nb = blocks_in(i);
+                wait(c->k_full + st, t >> 1);
+                if (pv_x + j > 0) wait(c->pv_done + x, pv_x + j - 1);      // S is free when the product that read P over it is done
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
 #pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        const uint32_t i = same_rows ? 2 * jq[x] + x : jq[x];
-                        if (jq[x] == jp[x] && jq[x] < n_of[x]) {
-                            const uint32_t t = tiles_done + i, st = t & 1u, total_pv = n_pv[x] + jp[x];
-                            // S of this stream is free when the product that read P over it is done
-                            if (mbar_test(c->k_full + st, (t >> 1) & 1u) && (total_pv == 0 || mbar_test(c->pv_done + x, (total_pv - 1) & 1u))) {
-                                tc_fence_after();
-#pragma unroll
-                                for (int ks = 0; ks < KSTEPS; ks++) {
-                                    const uint32_t off = (ks / 4) * (GROUP_BYTES >> 4) + (ks % 4) * 2;
-                                    mma_ss(tmem + TM_S + x * 128, DESC_K | (q_lo + x * (TILE >> 4) + off), DESC_K | (k_lo + st * (TILE >> 4) + off), IDESC_QK,
-                                           ks > 0 ? 1u : 0u);
-                                }
-                                tc_commit(c->s_full + x);
-                                if (++k_left[st] == readers) {
-                                    tc_commit(c->k_empty + st);
-                                    k_left[st] = 0;
-                                }
-                                jq[x]++;
-                                did = true;
-                            }
-                        } else if (jq[x] == jp[x] + 1) {
-                            const uint32_t ip = same_rows ? 2 * jp[x] + x : jp[x], t = tiles_done + ip, st = t & 1u, total_pv = n_pv[x] + jp[x];
-                            if (mbar_test(c->p_full + x, total_pv & 1u) && mbar_test(c->v_full + st, (t >> 1) & 1u)) {
-                                tc_fence_after();
-                                const uint32_t nb = blocks_in(ip);       // a block is one k-step: blocks behind the prefix are left out
-                                for (uint32_t ks = 0; ks < nb; ks++)
-                                    mma_ts(tmem + TM_O + x * 128, tmem + TM_S + x * 128 + ks * 8, DESC_V | (v_lo + st * (TILE >> 4) + ks * (2048u >> 4)), IDESC_PV,
-                                           (jp[x] > 0 || ks > 0) ? 1u : 0u);
-                                tc_commit(c->pv_done + x);
-                                if (++v_left[st] == readers) {
-                                    tc_commit(c->v_empty + st);
-                                    v_left[st] = 0;
-                                }
-                                jp[x]++;
-                                did = true;
-                            }
-                        }
+                    for (int ks = 0; ks < KSTEPS; ks++) {
+                        const uint32_t off = (ks / 4) * (GROUP_BYTES >> 4) + (ks % 4) * 2;
+                        mma_ss(ts, DESC_K | (q_lo + off), DESC_K | (k_lo + st * (TILE >> 4) + off), IDESC_QK, ks > 0 ? 1u : 0u);
                     }
-                    if (did) {
-                        idle = 0;
-                    } else {
-                        if (++idle > (1u << 24) || ((idle & 63u) == 0 && *fail)) ok = false;    // bounded: a stuck barrier ends the CTA, not the GPU
-                        __nanosleep(20);
-                    }
+                    tc_commit(c->s_full + x);
+                    tc_commit(c->k_empty + st);                            // a tile goes back after two readings
+                    if (same_rows) tc_commit(c->k_empty + st);
                 }
-                if (!ok) atomicCAS(&c->fail, 0u, 4u);
+                __syncwarp();
+                wait(c->p_full + x, pv_x + j);
+                wait(c->v_full + st, t >> 1);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    for (uint32_t ks = 0; ks < nb; ks++)                   // a block is one k-step: blocks behind the prefix are left out
+                        mma_ts(to, ts + ks * 8, DESC_V | (v_lo + st * (TILE >> 4) + ks * (2048u >> 4)), IDESC_PV, (j > 0 || ks > 0) ? 1u : 0u);
+                    tc_commit(c->pv_done + x);
+                    tc_commit(c->v_empty + st);
+                    if (same_rows) tc_commit(c->v_empty + st);
+                }
+                __syncwarp();
             }
+            if (!ok && lane == 0) atomicCAS(&c->fail, 0u, 4u);
             __syncwarp();
         } else if (warp >= SM) {
             if (!FP8) {
@@ -558,12 +547,13 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         n_pv[1] += n_of[1];
         u += it.n_tiles;
     }
+    if (warp >= SM + FEED && lane == 0) {                       // whatever ended the loop, no product is under way when tensor memory is given back
+        uint64_t* bar = c->drained + (warp - (SM + FEED));
+        tc_commit(bar);
+        for (uint32_t i = 0; i < (1u << 22) && !mbar_test(bar, 0u); i++) {}
+    }
+    __syncthreads();
     if (warp == SM + FEED) {
-        if (lane == 0) {                                        // whatever ended the loop, no product is under way when tensor memory is given back
-            tc_commit(&c->drained);
-            for (uint32_t i = 0; i < (1u << 22) && !mbar_test(&c->drained, 0u); i++) {}
-        }
-        __syncwarp();
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
