@@ -10,9 +10,10 @@
 //
 // A CTA works on up to 256 rows of one (group, kv head) as two streams of 128 with their own S, P and O: with more than 128 rows
 // the streams are two row tiles that read the same cached tiles; with fewer they are the same rows on alternate cached tiles (two
-// partial results).  While the softmax of one stream runs, the tensor cores work for the other.  A softmax thread owns a row: no
-// exchange between threads.  P goes back to tensor memory, over the S it was made from, as the A operand of the second product, so
-// shared memory holds Q and the K and V tiles only.  The row maximum in use is raised, and O rescaled, only when a score exceeds it by 2^6.
+// partial results).  A stream goes 64 cached tokens at a time through two S buffers: the scores of the next step are there when
+// the softmax of this one ends.  (One buffer of 128 tokens per stream left the softmax warps waiting for two products per tile:
+// 4 800 cycles per tile of both streams.)  A softmax thread owns a row: no exchange between threads.  P goes back to tensor memory, over
+// the S it was made from, as the A operand of the second product, so shared memory holds Q and the K and V tiles only.  The row maximum in use is raised, and O rescaled, only when a score exceeds it by 2^6.
 // An F16 pool's tiles arrive as tensor-map boxes, in the 128-byte swizzle the MMA reads.  An E4M3 pool's tiles are widened to F16
 // on the way by four warps (exact); K's block scale multiplies the scores, V's the probabilities, in units of a power of two above every
 // scale met so far.  Both operands of both products are then F16 and the products exact; a probability is rounded to F16 once (2^-11 of
@@ -46,7 +47,7 @@ using namespace tkv_tc;
 using tkv_rows::bar_wait;
 
 constexpr uint32_t CTAS = 148;               // one per SM of the part this is built for; partial results are sized by it
-constexpr int BS = 16, KT = 128;             // tokens of a block, of a cached tile
+constexpr int BS = 16, KT = 128, ST = 64;    // tokens of a block, of a cached tile, of a step
 constexpr int GROUP_BYTES = 128 * 128;       // a [128 rows][128 B] swizzled column group of an operand tile
 constexpr float RAISE = 6.0f;
 constexpr uint32_t MIN_SHARE = 2;            // cached tiles
@@ -70,7 +71,7 @@ __host__ __device__ constexpr int threads_of(bool fp8) { return (softmax_warps()
 
 struct Control {
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t q_ready[2], s_full[2], p_full[2], pv_done[2], drained[2];
+    uint64_t q_ready[2], s_full[2][2], p_full[2][2], pv_done[2][2], drained[2];   // [stream][S buffer]
     uint32_t tmem, fail;
     float scales[4][16];                     // per cached tile (mod 4): K scales of its 8 blocks, V scales
 };
@@ -104,11 +105,11 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     constexpr int TILE = NCG * GROUP_BYTES;                     // Q, K or V tile of 128 rows
     constexpr int KSTEPS = D / 16;
     constexpr int THREADS = threads_of(FP8), SM = softmax_warps(), FEED = feed_warps(FP8);
-    constexpr uint32_t IDESC_QK = instr_desc2(0u, 0u, 0u, 0u, 128u), IDESC_PV = instr_desc2(0u, 0u, 0u, 1u, (uint32_t)D);   // B = V, MN-major
+    constexpr uint32_t IDESC_QK = instr_desc2(0u, 0u, 0u, 0u, (uint32_t)ST), IDESC_PV = instr_desc2(0u, 0u, 0u, 1u, (uint32_t)D);   // B = V, MN-major
     constexpr uint64_t DESC_HI = ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
     constexpr uint64_t DESC_K = DESC_HI | ((uint64_t)1u << 16);
     constexpr uint64_t DESC_V = DESC_HI | ((uint64_t)(GROUP_BYTES >> 4) << 16);        // the second 64 dims one column group further
-    constexpr uint32_t TM_S = 0, TM_O = 256;                    // tensor memory columns: S (and P over it) of stream x at 128 x, O at 256 + 128 x
+    constexpr uint32_t TM_S = 0, TM_O = 256;                    // tensor memory columns: S (and P over it) of stream x, buffer b at 128 x + 64 b, O at 256 + 128 x
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     extern __shared__ __align__(1024) unsigned char smem[];
@@ -149,9 +150,11 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             mbar_init(c->k_empty + i, 2);
             mbar_init(c->v_empty + i, 2);
             mbar_init(c->q_ready + i, SM / 2);
-            mbar_init(c->s_full + i, 1);
-            mbar_init(c->p_full + i, SM / 2);
-            mbar_init(c->pv_done + i, 1);
+            for (int b = 0; b < 2; b++) {
+                mbar_init(&c->s_full[i][b], 1);
+                mbar_init(&c->p_full[i][b], SM / 2);
+                mbar_init(&c->pv_done[i][b], 1);
+            }
         }
         mbar_init(c->drained, 1);
         mbar_init(c->drained + 1, 1);
@@ -204,7 +207,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         at = cum[lo];
     }
     uint32_t tiles_done = 0;                                    // cached tiles of this CTA before the item at hand: places in the rings
-    uint32_t n_pv[2] = {0, 0};                                  // products P.V of each stream so far: phases of its barriers
+    uint32_t n_steps[2] = {0, 0};                               // steps of each stream before the item at hand: phases of its barriers
     uint32_t issued[2] = {0, 0};                                // F16 producer: tiles of K, of V asked for
     bool ok = true;
     for (uint32_t u = u_begin, item_no = 0; u < u_end; item_no++) {
@@ -226,49 +229,75 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         const uint32_t* table = a.tables + (size_t)it.first_seq * a.table_stride;
         const uint32_t n_blocks = it.prefix / BS;
         auto blocks_in = [&](uint32_t i) { return min(8u, n_blocks - (it.tile + i) * 8u); };   // of the item's i-th tile
+        auto steps_in = [&](uint32_t i) { return blocks_in(i) > 4u ? 2u : 1u; };
         uint32_t n_of[2];                                       // tiles of each stream
         n_of[0] = same_rows ? (it.n_tiles + 1) / 2 : it.n_tiles;
         n_of[1] = same_rows ? it.n_tiles / 2 : it.n_tiles;
 
         if (warp >= SM + FEED) {
             // ---- MMA issuers, a warp per stream.  Waits sleep in hardware (a polling issuer took issue slots from the softmax warps of its
-            // scheduler and held the tile up by 1 000 cycles), and the warp issues together through an elected lane. ----
-            const uint32_t x = warp - (SM + FEED), n_x = x ? n_of[1] : n_of[0], pv_x = x ? n_pv[1] : n_pv[0];
+            // scheduler and held the tile up by 1 000 cycles), and the warp issues together through an elected lane.  The scores run two
+            // steps ahead of the second product. ----
+            const uint32_t x = warp - (SM + FEED), n_x = x ? n_of[1] : n_of[0], s_x = x ? n_steps[1] : n_steps[0];
             const uint32_t q_lo = (smem_u32(q_tile) >> 4) + x * (TILE >> 4), k_lo = smem_u32(k_ring) >> 4, v_lo = smem_u32(v_ring) >> 4;
             const uint32_t ts = tmem + TM_S + x * 128, to = tmem + TM_O + x * 128;
             auto wait = [&](uint64_t* bar, uint32_t parity) {
                 if (ok) ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(bar), parity & 1u, fail));
             };
             wait(c->q_ready + x, item_no);
-            for (uint32_t j = 0; j < n_x && ok; j++) {
-                const uint32_t i = same_rows ? 2 * j + x : j, t = tiles_done + i, st = t & 1u, nb = blocks_in(i);
-                wait(c->k_full + st, t >> 1);
-                if (pv_x + j > 0) wait(c->pv_done + x, pv_x + j - 1);      // S is free when the product that read P over it is done
-                if (!ok) break;
+            uint32_t jq = 0, hq = 0, nq = s_x, np = s_x;         // tile and half of the next scores; steps of scores and of products issued
+            auto scores = [&]() {                                // of the next step, if there is one
+                if (jq >= n_x || !ok) return;
+                const uint32_t i = same_rows ? 2 * jq + x : jq, t = tiles_done + i, st = t & 1u, b = nq & 1u;
+                if (hq == 0) wait(c->k_full + st, t >> 1);
+                if (nq >= 2) wait(&c->pv_done[x][b], (nq >> 1) - 1u);      // the buffer is free when the product that read P over it is done
+                if (!ok) return;
                 tc_fence_after();
+                const bool last = hq + 1 == steps_in(i);
                 if (elect_one()) {
 #pragma unroll
                     for (int ks = 0; ks < KSTEPS; ks++) {
                         const uint32_t off = (ks / 4) * (GROUP_BYTES >> 4) + (ks % 4) * 2;
-                        mma_ss(ts, DESC_K | (q_lo + off), DESC_K | (k_lo + st * (TILE >> 4) + off), IDESC_QK, ks > 0 ? 1u : 0u);
+                        mma_ss(ts + b * ST, DESC_K | (q_lo + off), DESC_K | (k_lo + st * (TILE >> 4) + hq * (ST * 128u >> 4) + off), IDESC_QK, ks > 0 ? 1u : 0u);
                     }
-                    tc_commit(c->s_full + x);
-                    tc_commit(c->k_empty + st);                            // a tile goes back after two readings
-                    if (same_rows) tc_commit(c->k_empty + st);
+                    tc_commit(&c->s_full[x][b]);
+                    if (last) {
+                        tc_commit(c->k_empty + st);                        // a tile goes back after two readings
+                        if (same_rows) tc_commit(c->k_empty + st);
+                    }
                 }
                 __syncwarp();
-                wait(c->p_full + x, pv_x + j);
-                wait(c->v_full + st, t >> 1);
-                if (!ok) break;
-                tc_fence_after();
-                if (elect_one()) {
-                    for (uint32_t ks = 0; ks < nb; ks++)                   // a block is one k-step: blocks behind the prefix are left out
-                        mma_ts(to, ts + ks * 8, DESC_V | (v_lo + st * (TILE >> 4) + ks * (2048u >> 4)), IDESC_PV, (j > 0 || ks > 0) ? 1u : 0u);
-                    tc_commit(c->pv_done + x);
-                    tc_commit(c->v_empty + st);
-                    if (same_rows) tc_commit(c->v_empty + st);
+                nq++;
+                if (last) {
+                    jq++;
+                    hq = 0;
+                } else {
+                    hq = 1;
                 }
-                __syncwarp();
+            };
+            scores();
+            scores();
+            for (uint32_t j = 0; j < n_x && ok; j++) {
+                const uint32_t i = same_rows ? 2 * j + x : j, t = tiles_done + i, st = t & 1u, steps = steps_in(i);
+                for (uint32_t h = 0; h < steps && ok; h++, np++) {
+                    const uint32_t b = np & 1u, nb = min(4u, blocks_in(i) - 4u * h);
+                    wait(&c->p_full[x][b], np >> 1);
+                    if (h == 0) wait(c->v_full + st, t >> 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        for (uint32_t ks = 0; ks < nb; ks++)               // a block is one k-step: blocks behind the prefix are left out
+                            mma_ts(to, ts + b * ST + ks * 8, DESC_V | (v_lo + st * (TILE >> 4) + (4 * h + ks) * (2048u >> 4)), IDESC_PV,
+                                   (j > 0 || h > 0 || ks > 0) ? 1u : 0u);
+                        tc_commit(&c->pv_done[x][b]);
+                        if (h + 1 == steps) {
+                            tc_commit(c->v_empty + st);
+                            if (same_rows) tc_commit(c->v_empty + st);
+                        }
+                    }
+                    __syncwarp();
+                    scores();
+                }
             }
             if (!ok && lane == 0) atomicCAS(&c->fail, 0u, 4u);
             __syncwarp();
@@ -388,7 +417,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
         } else {
             // ---- softmax: one row per thread ----
-            const uint32_t x = warp >> 2, n_x = x ? n_of[1] : n_of[0], pv_x = x ? n_pv[1] : n_pv[0], r = (warp & 3u) * 32u + lane, row = it.row0 + (same_rows ? 0u : x * 128u) + r;   // of the group and kv head
+            const uint32_t x = warp >> 2, n_x = x ? n_of[1] : n_of[0], s_x = x ? n_steps[1] : n_steps[0], r = (warp & 3u) * 32u + lane, row = it.row0 + (same_rows ? 0u : x * 128u) + r;   // of the group and kv head
             const bool live = row < it.rows && (same_rows ? r < it.block_rows : x * 128u + r < it.block_rows);
             const bool warp_live = __any_sync(0xFFFFFFFFu, live);
             const uint32_t seq = it.first_seq + (live ? row / a.group : 0u), head = it.kvh * a.group + (live ? row % a.group : 0u);
@@ -408,118 +437,107 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
             const uint32_t lanes = ((warp & 3u) * 32u) << 16, ts = tmem + TM_S + x * 128 + lanes, to = tmem + TM_O + x * 128 + lanes;
             float m = -INFINITY, l = 0.0f, v_ref = FP8 ? 0x1p-100f : 1.0f, v_inv = FP8 ? 0x1p+100f : 1.0f;
+            uint32_t n = s_x;                                   // steps of this stream so far
             for (uint32_t j = 0; j < n_x && ok; j++) {
-                const uint32_t i = same_rows ? 2 * j + x : j, t0 = (it.tile + i) * KT, slot = (tiles_done + i) & 3u;
-                ok = bar_wait(smem_u32(c->s_full + x), (pv_x + j) & 1u, fail);
-                ok = __all_sync(0xFFFFFFFFu, ok);
-                if (!ok) break;
-                if (warp_live) {
-                    tc_fence_after();
-                    constexpr int CH = 64;                      // scores held in registers; they are read twice (all 128 do not fit beside the rest)
-                    const int left = (int)min(limit > t0 ? limit - t0 : 0u, (uint32_t)KT);   // tokens of the tile that the row attends to
-                    auto tile = [&](auto masked_type) {
-                    constexpr bool MASKED = decltype(masked_type)::value;
-                    uint32_t v[CH / 32][32];
-                    float mx = -INFINITY;
-#pragma unroll
-                    for (int c0 = 0; c0 < KT; c0 += CH) {
-#pragma unroll
-                        for (int k = 0; k < CH; k += 32) tmem_ld32(ts + c0 + k, v[k / 32]);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int b = 0; b < CH / 16; b++) {
-                            float top = -INFINITY;              // neither scale is negative: the maximum commutes with them
-#pragma unroll
-                            for (int k = 0; k < 16; k++)
-                                top = fmaxf(top, MASKED && c0 + b * 16 + k >= left ? -INFINITY : __uint_as_float(v[b / 2][(b & 1) * 16 + k]));
-                            mx = fmaxf(mx, top == -INFINITY ? top : top * (FP8 ? a.scale_log2 * c->scales[slot][c0 / 16 + b] : a.scale_log2));
-                        }
-                    }
-                    // ---- a raised maximum or V scale rescales the row of O; the previous product is done, or S would not be here ----
-                    float factor = 1.0f;
-                    if (mx > m + RAISE) {
-                        factor = m == -INFINITY ? 0.0f : fast_exp2(m - mx);
-                        m = mx;
-                        l *= factor;
-                    }
-                    if (FP8) {
-                        float top = 0.0f;
-#pragma unroll
-                        for (int b = 0; b < 8; b++) top = fmaxf(top, c->scales[slot][8 + b]);
-                        if (top > v_ref) {                      // the same in every thread
-                            const float up = __uint_as_float(min((__float_as_uint(top) >> 23) + 1u, 253u) << 23);
-                            factor *= v_ref / up;
-                            v_ref = up;
-                            v_inv = 1.0f / up;
-                        }
-                    }
-                    if (j > 0 && __any_sync(0xFFFFFFFFu, factor != 1.0f)) {
-#pragma unroll 1
-                        for (uint32_t c0 = 0; c0 < (uint32_t)D; c0 += 16) {
-                            uint32_t o[16];
-                            tmem_ld16(to + c0, o);
+                const uint32_t i = same_rows ? 2 * j + x : j, slot = (tiles_done + i) & 3u, steps = steps_in(i);
+                for (uint32_t h = 0; h < steps; h++, n++) {
+                    const uint32_t t0 = (it.tile + i) * KT + h * ST, b = n & 1u;
+                    ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(&c->s_full[x][b]), (n >> 1) & 1u, fail));
+                    if (!ok) break;
+                    if (warp_live) {
+                        tc_fence_after();
+                        const int left = (int)min(limit > t0 ? limit - t0 : 0u, (uint32_t)ST);   // tokens of the step that the row attends to
+                        const uint32_t tb = ts + b * ST;
+                        const float* sc = c->scales[slot] + 4 * h;
+                        auto step = [&](auto masked_type) {
+                            constexpr bool MASKED = decltype(masked_type)::value;
+                            uint32_t v[2][32];
+                            tmem_ld32(tb, v[0]);
+                            tmem_ld32(tb + 32, v[1]);
                             tmem_wait_ld();
+                            float mx = -INFINITY;               // neither scale is negative: the maximum commutes with them
 #pragma unroll
-                            for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
-                            tmem_st16(to + c0, o);
-                        }
-                        tmem_wait_st();
-                    }
-                    // ---- probabilities, as F16 pairs over the scores ----
-                    const float sub = m == -INFINITY ? 0.0f : m;
-                    float sum = 0.0f;
+                            for (int q = 0; q < 4; q++) {       // a block
+                                float top = -INFINITY;
 #pragma unroll
-                    for (int c0 = 0; c0 < KT; c0 += CH) {       // P of tokens [c0, c0 + CH) goes to columns [c0 / 2, (c0 + CH) / 2): scores already read
-                        if (CH < KT) {
-#pragma unroll
-                            for (int k = 0; k < CH; k += 32) tmem_ld32(ts + c0 + k, v[k / 32]);
-                            tmem_wait_ld();
-                        }
-#pragma unroll
-                        for (int b = 0; b < CH / 16; b++) {
-                            const float ks = FP8 ? a.scale_log2 * c->scales[slot][c0 / 16 + b] : a.scale_log2;
-                            const float vn = FP8 ? c->scales[slot][8 + c0 / 16 + b] * v_inv : 1.0f;
-#pragma unroll
-                            for (int k = 0; k < 16; k += 2) {
-                                float p0 = fast_exp2(__fmaf_rn(__uint_as_float(v[b / 2][(b & 1) * 16 + k]), ks, -sub));
-                                float p1 = fast_exp2(__fmaf_rn(__uint_as_float(v[b / 2][(b & 1) * 16 + k + 1]), ks, -sub));
-                                if (MASKED) {
-                                    p0 = c0 + b * 16 + k < left ? p0 : 0.0f;
-                                    p1 = c0 + b * 16 + k + 1 < left ? p1 : 0.0f;
-                                }
-                                sum += p0 + p1;
-                                if (FP8) {
-                                    p0 *= vn;
-                                    p1 *= vn;
-                                }
-                                const __half2 h = __floats2half2_rn(p0, p1);
-                                v[b / 4][((b & 3) * 16 + k) / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                                for (int k = 0; k < 16; k++)
+                                    top = fmaxf(top, MASKED && q * 16 + k >= left ? -INFINITY : __uint_as_float(v[q / 2][(q & 1) * 16 + k]));
+                                mx = FP8 ? fmaxf(mx, top == -INFINITY ? top : top * sc[q]) : fmaxf(mx, top);
                             }
-                        }
+                            mx = mx == -INFINITY ? mx : mx * a.scale_log2;
+                            // ---- a raised maximum or V scale rescales the row of O, once the product of the step before is done ----
+                            float factor = 1.0f;
+                            if (mx > m + RAISE) {
+                                factor = m == -INFINITY ? 0.0f : fast_exp2(m - mx);
+                                m = mx;
+                                l *= factor;
+                            }
+                            if (FP8) {
+                                const float top = fmaxf(fmaxf(sc[8], sc[9]), fmaxf(sc[10], sc[11]));
+                                if (top > v_ref) {              // the same in every thread
+                                    const float up = __uint_as_float(min((__float_as_uint(top) >> 23) + 1u, 253u) << 23);
+                                    factor *= v_ref / up;
+                                    v_ref = up;
+                                    v_inv = 1.0f / up;
+                                }
+                            }
+                            if (n > s_x && __any_sync(0xFFFFFFFFu, factor != 1.0f)) {
+                                ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(&c->pv_done[x][b ^ 1u]), ((n - 1) >> 1) & 1u, fail));
+                                tc_fence_after();
+#pragma unroll 1
+                                for (uint32_t c0 = 0; c0 < (uint32_t)D; c0 += 16) {
+                                    uint32_t o[16];
+                                    tmem_ld16(to + c0, o);
+                                    tmem_wait_ld();
 #pragma unroll
-                        for (int k = 0; k < CH / 2; k += 32) tmem_st32(ts + c0 / 2 + k, v[k / 32]);
+                                    for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
+                                    tmem_st16(to + c0, o);
+                                }
+                                tmem_wait_st();
+                            }
+                            // ---- probabilities, as F16 pairs over the scores ----
+                            const float sub = m == -INFINITY ? 0.0f : -m;
+                            float sum = 0.0f;
+#pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                const float ks = FP8 ? a.scale_log2 * sc[q] : a.scale_log2, vn = FP8 ? sc[8 + q] * v_inv : 1.0f;
+#pragma unroll
+                                for (int k = 0; k < 16; k += 2) {
+                                    float p0 = fast_exp2(__fmaf_rn(__uint_as_float(v[q / 2][(q & 1) * 16 + k]), ks, sub));
+                                    float p1 = fast_exp2(__fmaf_rn(__uint_as_float(v[q / 2][(q & 1) * 16 + k + 1]), ks, sub));
+                                    if (MASKED) {
+                                        p0 = q * 16 + k < left ? p0 : 0.0f;
+                                        p1 = q * 16 + k + 1 < left ? p1 : 0.0f;
+                                    }
+                                    sum += p0 + p1;
+                                    if (FP8) {
+                                        p0 *= vn;
+                                        p1 *= vn;
+                                    }
+                                    const __half2 hp = __floats2half2_rn(p0, p1);
+                                    v[0][q * 8 + k / 2] = *reinterpret_cast<const uint32_t*>(&hp);
+                                }
+                            }
+                            tmem_st32(tb, v[0]);
+                            tmem_wait_st();
+                            l += sum;
+                        };
+                        if (__any_sync(0xFFFFFFFFu, left < ST)) step(std::true_type{});
+                        else step(std::false_type{});
+                        tc_fence_before();
                     }
-                    tmem_wait_st();
-                    l += sum;
-                    };
-                    if (__any_sync(0xFFFFFFFFu, left < KT)) tile(std::true_type{});
-                    else tile(std::false_type{});
-                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&c->p_full[x][b]);
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(c->p_full + x);
             }
             // ---- partial result of the row ----
-            const uint32_t n = n_x;
+            const bool any = n > s_x;
             const uint64_t dst = it.out_row + (same_rows ? x * it.block_rows + r : x * 128u + r);
-            if (ok && n) {
-                ok = bar_wait(smem_u32(c->pv_done + x), (pv_x + n - 1) & 1u, fail);
-                ok = __all_sync(0xFFFFFFFFu, ok);
-            }
+            if (ok && any) ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(&c->pv_done[x][(n - 1) & 1u]), ((n - 1) >> 1) & 1u, fail));
             if (ok && warp_live) {
                 tc_fence_after();
-                if (live) *reinterpret_cast<float2*>(a.part_ml + dst * 2) = n ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
-                if (n) {
+                if (live) *reinterpret_cast<float2*>(a.part_ml + dst * 2) = any ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
+                if (any) {
 #pragma unroll 1
                     for (uint32_t c0 = 0; c0 < (uint32_t)D; c0 += 32) {
                         uint32_t o[32];
@@ -543,8 +561,9 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         if (*fail) break;                                       // the same for all threads: nobody writes it between the two barriers
         __syncthreads();
         tiles_done += it.n_tiles;
-        n_pv[0] += n_of[0];
-        n_pv[1] += n_of[1];
+        const uint32_t last = it.n_tiles - 1, cut = 2 - steps_in(last);    // only a prefix's last tile has one step
+        n_steps[0] += 2 * n_of[0] - (same_rows && (last & 1u) ? 0 : cut);
+        n_steps[1] += 2 * n_of[1] - (same_rows && !(last & 1u) ? 0 : cut);
         u += it.n_tiles;
     }
     if (warp >= SM + FEED && lane == 0) {                       // whatever ended the loop, no product is under way when tensor memory is given back
