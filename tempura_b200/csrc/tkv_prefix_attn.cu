@@ -192,7 +192,8 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = c->tmem;
+    const uint32_t tmem = 0;                                    // all 512 columns are this CTA's: they begin at 0
+    if (tid == 0 && c->tmem != 0) c->fail = 2u;
 
     // ---- the group of the first tile ----
     uint32_t g, at;                                             // tiles before group g
@@ -238,9 +239,14 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             // ---- MMA issuers, a warp per stream.  Waits sleep in hardware (a polling issuer took issue slots from the softmax warps of its
             // scheduler and held the tile up by 1 000 cycles), and the warp issues together through an elected lane.  The scores run two
             // steps ahead of the second product. ----
-            const uint32_t x = warp - (SM + FEED), n_x = x ? n_of[1] : n_of[0], s_x = x ? n_steps[1] : n_steps[0];
+            // Broadcast from one lane, what selects operands is known to be the warp's own: addresses then are computed once per warp.
+            auto uni = [](uint32_t v) { return __shfl_sync(0xFFFFFFFFu, v, 0); };
+            const uint32_t x = uni(warp - (SM + FEED)), n_x = uni(x ? n_of[1] : n_of[0]), s_x = uni(x ? n_steps[1] : n_steps[0]);
+            const uint32_t done = uni(tiles_done), n_left = uni(n_blocks - it.tile * 8u);
+            const bool same = uni(same_rows ? 1u : 0u) != 0;
+            auto blocks_at = [&](uint32_t i) { return min(8u, n_left - i * 8u); };
             const uint32_t q_lo = (smem_u32(q_tile) >> 4) + x * (TILE >> 4), k_lo = smem_u32(k_ring) >> 4, v_lo = smem_u32(v_ring) >> 4;
-            const uint32_t ts = tmem + TM_S + x * 128, to = tmem + TM_O + x * 128;
+            const uint32_t ts = TM_S + x * 128, to = TM_O + x * 128;
             auto wait = [&](uint64_t* bar, uint32_t parity) {
                 if (ok) ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(bar), parity & 1u, fail));
             };
@@ -248,12 +254,12 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             uint32_t jq = 0, hq = 0, nq = s_x, np = s_x;         // tile and half of the next scores; steps of scores and of products issued
             auto scores = [&]() {                                // of the next step, if there is one
                 if (jq >= n_x || !ok) return;
-                const uint32_t i = same_rows ? 2 * jq + x : jq, t = tiles_done + i, st = t & 1u, b = nq & 1u;
+                const uint32_t i = same ? 2 * jq + x : jq, t = done + i, st = t & 1u, b = nq & 1u;
                 if (hq == 0) wait(c->k_full + st, t >> 1);
                 if (nq >= 2) wait(&c->pv_done[x][b], (nq >> 1) - 1u);      // the buffer is free when the product that read P over it is done
                 if (!ok) return;
                 tc_fence_after();
-                const bool last = hq + 1 == steps_in(i);
+                const bool last = hq + 1 == (blocks_at(i) > 4u ? 2u : 1u);
                 if (elect_one()) {
 #pragma unroll
                     for (int ks = 0; ks < KSTEPS; ks++) {
@@ -263,7 +269,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     tc_commit(&c->s_full[x][b]);
                     if (last) {
                         tc_commit(c->k_empty + st);                        // a tile goes back after two readings
-                        if (same_rows) tc_commit(c->k_empty + st);
+                        if (same) tc_commit(c->k_empty + st);
                     }
                 }
                 __syncwarp();
@@ -278,21 +284,22 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             scores();
             scores();
             for (uint32_t j = 0; j < n_x && ok; j++) {
-                const uint32_t i = same_rows ? 2 * j + x : j, t = tiles_done + i, st = t & 1u, steps = steps_in(i);
+                const uint32_t i = same ? 2 * j + x : j, t = done + i, st = t & 1u, steps = blocks_at(i) > 4u ? 2u : 1u;
                 for (uint32_t h = 0; h < steps && ok; h++, np++) {
-                    const uint32_t b = np & 1u, nb = min(4u, blocks_in(i) - 4u * h);
+                    const uint32_t b = np & 1u, nb = min(4u, blocks_at(i) - 4u * h);
                     wait(&c->p_full[x][b], np >> 1);
                     if (h == 0) wait(c->v_full + st, t >> 1);
                     if (!ok) break;
                     tc_fence_after();
                     if (elect_one()) {
-                        for (uint32_t ks = 0; ks < nb; ks++)               // a block is one k-step: blocks behind the prefix are left out
-                            mma_ts(to, ts + b * ST + ks * 8, DESC_V | (v_lo + st * (TILE >> 4) + (4 * h + ks) * (2048u >> 4)), IDESC_PV,
+#pragma unroll
+                        for (uint32_t ks = 0; ks < 4; ks++)                // a block is one k-step: blocks behind the prefix are left out
+                            if (ks < nb) mma_ts(to, ts + b * ST + ks * 8, DESC_V | (v_lo + st * (TILE >> 4) + (4 * h + ks) * (2048u >> 4)), IDESC_PV,
                                    (j > 0 || h > 0 || ks > 0) ? 1u : 0u);
                         tc_commit(&c->pv_done[x][b]);
                         if (h + 1 == steps) {
                             tc_commit(c->v_empty + st);
-                            if (same_rows) tc_commit(c->v_empty + st);
+                            if (same) tc_commit(c->v_empty + st);
                         }
                     }
                     __syncwarp();
@@ -423,13 +430,16 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             const uint32_t seq = it.first_seq + (live ? row / a.group : 0u), head = it.kvh * a.group + (live ? row % a.group : 0u);
             const uint32_t limit = live ? min(min(a.kv_lens[seq], a.max_kv_len), it.prefix) : 0u;
             {
-                const uint4* src = reinterpret_cast<const uint4*>(a.q + ((size_t)seq * a.n_q_heads + head) * D);
-                unsigned char* qt = q_tile + x * TILE;
+                // Q rows of the warp, whole rows per load (a row per thread took 8 000 cycles)
+                constexpr int CPR = D / 8, RPL = 32 / CPR;      // 16-byte chunks of a row; rows per load
+                const uint32_t q_row = seq * a.n_q_heads + head, alive = __ballot_sync(0xFFFFFFFFu, live), ch = lane % CPR;
+                unsigned char* qt = q_tile + x * TILE + (ch / 8) * GROUP_BYTES;
 #pragma unroll
-                for (int ch = 0; ch < D / 8; ch++) {
-                    uint4 v = live ? __ldg(src + ch) : make_uint4(0, 0, 0, 0);
+                for (int r0 = 0; r0 < 32; r0 += RPL) {
+                    const uint32_t o = r0 + lane / CPR, from = __shfl_sync(0xFFFFFFFFu, q_row, o);
+                    uint4 v = (alive >> o) & 1u ? __ldg(reinterpret_cast<const uint4*>(a.q + (size_t)from * D) + ch) : make_uint4(0, 0, 0, 0);
                     v = make_uint4(v.x ^ a.q_sign, v.y ^ a.q_sign, v.z ^ a.q_sign, v.w ^ a.q_sign);
-                    *reinterpret_cast<uint4*>(qt + (ch / 8) * GROUP_BYTES + swz(r, ch % 8)) = v;
+                    *reinterpret_cast<uint4*>(qt + swz((warp & 3u) * 32u + o, ch % 8)) = v;
                 }
                 fence_async_smem();
                 __syncwarp();
@@ -538,18 +548,32 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 tc_fence_after();
                 if (live) *reinterpret_cast<float2*>(a.part_ml + dst * 2) = any ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
                 if (any) {
+                    // through the stream's Q tile, which no product reads any more, half of the dims at a time: the rows of a warp follow one
+                    // another in memory, so a store covers whole half rows (a row per thread took 9 000 cycles)
+                    constexpr int DH = D / 2, CH = DH / 4;      // dims of a pass; its 16-byte chunks per row
+                    unsigned char* stage = q_tile + x * TILE + (warp & 3u) * (TILE / 4);
+                    const uint32_t n_live = (uint32_t)__popc(__ballot_sync(0xFFFFFFFFu, live));
+                    float* rows_out = a.part_o + (dst - lane) * D;
 #pragma unroll 1
-                    for (uint32_t c0 = 0; c0 < (uint32_t)D; c0 += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(to + c0, o);
-                        tmem_wait_ld();
-                        if (live) {
+                    for (int d0 = 0; d0 < D; d0 += DH) {
 #pragma unroll
-                            for (int k = 0; k < 32; k += 4)
-                                *reinterpret_cast<float4*>(a.part_o + dst * D + c0 + k) =
-                                    make_float4(__uint_as_float(o[k]) * v_ref, __uint_as_float(o[k + 1]) * v_ref, __uint_as_float(o[k + 2]) * v_ref,
-                                                __uint_as_float(o[k + 3]) * v_ref);
+                        for (int c0 = 0; c0 < DH; c0 += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(to + d0 + c0, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 8; k++)
+                                *reinterpret_cast<float4*>(stage + lane * (DH * 4) + (((c0 / 4 + k) ^ (lane % CH)) * 16)) =
+                                    make_float4(__uint_as_float(o[4 * k]) * v_ref, __uint_as_float(o[4 * k + 1]) * v_ref, __uint_as_float(o[4 * k + 2]) * v_ref,
+                                                __uint_as_float(o[4 * k + 3]) * v_ref);
                         }
+                        __syncwarp();
+#pragma unroll 8
+                        for (uint32_t n16 = lane; n16 < n_live * CH; n16 += 32) {
+                            const uint32_t o = n16 / CH, k = n16 % CH;
+                            *reinterpret_cast<float4*>(rows_out + (size_t)o * D + d0 + 4 * k) = *reinterpret_cast<const float4*>(stage + o * (DH * 4) + ((k ^ (o % CH)) * 16));
+                        }
+                        __syncwarp();
                     }
                 }
             }
