@@ -355,30 +355,34 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     row = n / CPR;
                     ch = n % CPR;
                 };
+                // block ids a tile ahead of the loads that use them; an id outside the pool becomes 0 and is remembered, without a branch that would wait
+                uint32_t id[PER], sc_id = 0;
+                bool foreign = false;
+                auto look_up = [&](uint32_t i) {
+                    const uint32_t nb = i < it.n_tiles ? blocks_in(i) : 0u;
+#pragma unroll
+                    for (int e = 0; e < PER; e++) {
+                        uint32_t row, ch;
+                        piece(e, row, ch);
+                        id[e] = row / BS < nb ? table[(it.tile + i) * 8u + row / BS] : ~0u;
+                    }
+                    sc_id = (t128 & 7u) < nb ? table[(it.tile + i) * 8u + (t128 & 7u)] : ~0u;
+                };
                 auto load = [&](uint4 (&r)[PER], const char* base, uint32_t i) {
                     const uint32_t nb = blocks_in(i);
 #pragma unroll
                     for (int e = 0; e < PER; e++) {
                         uint32_t row, ch;
                         piece(e, row, ch);
-                        r[e] = make_uint4(0, 0, 0, 0);
-                        if (row / BS < nb) {
-                            const uint32_t blk = table[(it.tile + i) * 8u + row / BS];
-                            if (blk < a.total_blocks)
-                                r[e] = __ldg(reinterpret_cast<const uint4*>(base + (uint64_t)blk * a.block_stride + (size_t)(row % BS) * a.row_stride + (size_t)it.kvh * D + ch * 16));
-                            else atomicCAS(&c->fail, 0u, 2u);
-                        }
+                        const bool in = id[e] < a.total_blocks;
+                        foreign |= !in && row / BS < nb;
+                        r[e] = in ? __ldg(reinterpret_cast<const uint4*>(base + (uint64_t)id[e] * a.block_stride + (size_t)(row % BS) * a.row_stride + (size_t)it.kvh * D + ch * 16))
+                                  : make_uint4(0, 0, 0, 0);
                     }
                 };
-                auto load_scales = [&](uint32_t i) {
+                auto load_scales = [&]() {
                     sc = 1.0f;
-                    if (t128 < 16 && a.k_scales) {
-                        sc = 0.0f;
-                        if ((t128 & 7u) < blocks_in(i)) {
-                            const uint32_t blk = table[(it.tile + i) * 8u + (t128 & 7u)];
-                            if (blk < a.total_blocks) sc = __ldg((t128 < 8 ? a.k_scales : a.v_scales) + (size_t)blk * a.n_kv_heads + it.kvh);
-                        }
-                    }
+                    if (t128 < 16 && a.k_scales) sc = sc_id < a.total_blocks ? __ldg((t128 < 8 ? a.k_scales : a.v_scales) + (size_t)sc_id * a.n_kv_heads + it.kvh) : 0.0f;
                 };
                 auto widen = [&](unsigned char* tile, const uint4 (&r)[PER]) {
 #pragma unroll
@@ -399,9 +403,11 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     fence_async_smem();
                     __syncwarp();
                 };
-                load_scales(0);
+                look_up(0);
+                load_scales();
                 load(kr, a.k8, 0);
                 load(vr, a.v8, 0);
+                look_up(1);
                 for (uint32_t i = 0; i < it.n_tiles && ok; i++) {
                     const uint32_t t = tiles_done + i, st = t & 1u;
                     if (t >= 2) ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(c->k_empty + st), ((t >> 1) - 1u) & 1u, fail));
@@ -410,7 +416,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     widen(k_ring + st * TILE, kr);
                     if (lane == 0) mbar_arrive(c->k_full + st);
                     if (i + 1 < it.n_tiles) {
-                        load_scales(i + 1);
+                        load_scales();
                         load(kr, a.k8, i + 1);
                     }
                     if (t >= 2) ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(c->v_empty + st), ((t >> 1) - 1u) & 1u, fail));
@@ -418,8 +424,10 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     widen(v_ring + st * TILE, vr);
                     if (lane == 0) mbar_arrive(c->v_full + st);
                     if (i + 1 < it.n_tiles) load(vr, a.v8, i + 1);
+                    look_up(i + 2);
                     if (*fail) ok = false;
                 }
+                if (foreign) atomicCAS(&c->fail, 0u, 2u);
                 if (!ok && lane == 0) atomicCAS(&c->fail, 0u, 4u);
             }
         } else {
