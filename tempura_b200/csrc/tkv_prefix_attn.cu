@@ -118,7 +118,8 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     unsigned char* k_ring = q_tile + 2 * TILE;                  // two
     unsigned char* v_ring = k_ring + 2 * TILE;                  // two
     const volatile uint32_t* fail = &c->fail;
-    __shared__ uint32_t cum[THREADS + 1], warp_sum[THREADS / 32];
+    uint32_t* cum = reinterpret_cast<uint32_t*>(q_tile);        // [THREADS + 1], until the first item
+    uint32_t* warp_sum = cum + THREADS + 1;                     // [THREADS / 32]
 
     if (__syncthreads_or(tkv_rows::groups_bad(a.group_starts, a.prefix_lens, a.n_groups, a.n_seqs, a.max_prefix_len, tid, THREADS))) {
         if (tid == 0) {
@@ -207,6 +208,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         g = lo * per;
         at = cum[lo];
     }
+    __syncthreads();                                            // Q goes where the sums were
     uint32_t tiles_done = 0;                                    // cached tiles of this CTA before the item at hand: places in the rings
     uint32_t n_steps[2] = {0, 0};                               // steps of each stream before the item at hand: phases of its barriers
     uint32_t issued[2] = {0, 0};                                // F16 producer: tiles of K, of V asked for
@@ -251,59 +253,60 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 if (ok) ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(bar), parity & 1u, fail));
             };
             wait(c->q_ready + x, item_no);
-            uint32_t jq = 0, hq = 0, nq = s_x, np = s_x;         // tile and half of the next scores; steps of scores and of products issued
-            auto scores = [&]() {                                // of the next step, if there is one
-                if (jq >= n_x || !ok) return;
-                const uint32_t i = same ? 2 * jq + x : jq, t = done + i, st = t & 1u, b = nq & 1u;
-                if (hq == 0) wait(c->k_full + st, t >> 1);
-                if (nq >= 2) wait(&c->pv_done[x][b], (nq >> 1) - 1u);      // the buffer is free when the product that read P over it is done
-                if (!ok) return;
-                tc_fence_after();
-                const bool last = hq + 1 == (blocks_at(i) > 4u ? 2u : 1u);
-                if (elect_one()) {
-#pragma unroll
-                    for (int ks = 0; ks < KSTEPS; ks++) {
-                        const uint32_t off = (ks / 4) * (GROUP_BYTES >> 4) + (ks % 4) * 2;
-                        mma_ss(ts + b * ST, DESC_K | (q_lo + off), DESC_K | (k_lo + st * (TILE >> 4) + hq * (ST * 128u >> 4) + off), IDESC_QK, ks > 0 ? 1u : 0u);
-                    }
-                    tc_commit(&c->s_full[x][b]);
-                    if (last) {
-                        tc_commit(c->k_empty + st);                        // a tile goes back after two readings
-                        if (same) tc_commit(c->k_empty + st);
-                    }
+            uint32_t jq = 0, hq = 0, nq = s_x;                   // tile, half and number of the next scores
+            uint32_t jp = 0, hp = 0, np = s_x;                   // of the next product
+            while (ok && jp < n_x) {
+                // The scores run up to two steps ahead, but a tile that is not there yet holds up no product: that would hold up its V's place, too.
+                const uint32_t iq = same ? 2 * jq + x : jq, tq = done + iq, sq = tq & 1u;
+                bool ahead = jq < n_x && nq - np < 2;
+                if (ahead && hq == 0) {
+                    if (np == nq) wait(c->k_full + sq, tq >> 1);
+                    else ahead = __all_sync(0xFFFFFFFFu, mbar_test(c->k_full + sq, (tq >> 1) & 1u));
                 }
-                __syncwarp();
-                nq++;
-                if (last) {
-                    jq++;
-                    hq = 0;
-                } else {
-                    hq = 1;
-                }
-            };
-            scores();
-            scores();
-            for (uint32_t j = 0; j < n_x && ok; j++) {
-                const uint32_t i = same ? 2 * j + x : j, t = done + i, st = t & 1u, steps = blocks_at(i) > 4u ? 2u : 1u;
-                for (uint32_t h = 0; h < steps && ok; h++, np++) {
-                    const uint32_t b = np & 1u, nb = min(4u, blocks_at(i) - 4u * h);
-                    wait(&c->p_full[x][b], np >> 1);
-                    if (h == 0) wait(c->v_full + st, t >> 1);
+                if (ahead) {
+                    const uint32_t b = nq & 1u;
+                    if (nq >= 2) wait(&c->pv_done[x][b], (nq >> 1) - 1u);  // the buffer is free when the product that read P over it is done
                     if (!ok) break;
                     tc_fence_after();
+                    const bool last = hq + 1 == (blocks_at(iq) > 4u ? 2u : 1u);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int ks = 0; ks < KSTEPS; ks++) {
+                            const uint32_t off = (ks / 4) * (GROUP_BYTES >> 4) + (ks % 4) * 2;
+                            mma_ss(ts + b * ST, DESC_K | (q_lo + off), DESC_K | (k_lo + sq * (TILE >> 4) + hq * (ST * 128u >> 4) + off), IDESC_QK, ks > 0 ? 1u : 0u);
+                        }
+                        tc_commit(&c->s_full[x][b]);
+                        if (last) {
+                            tc_commit(c->k_empty + sq);                    // a tile goes back after two readings
+                            if (same) tc_commit(c->k_empty + sq);
+                        }
+                    }
+                    __syncwarp();
+                    nq++;
+                    hq = last ? 0 : 1;
+                    jq += last ? 1 : 0;
+                } else {
+                    const uint32_t i = same ? 2 * jp + x : jp, t = done + i, st = t & 1u, b = np & 1u, all = blocks_at(i), nb = min(4u, all - 4u * hp);
+                    wait(&c->p_full[x][b], np >> 1);
+                    if (hp == 0) wait(c->v_full + st, t >> 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const bool last = hp + 1 == (all > 4u ? 2u : 1u);
                     if (elect_one()) {
 #pragma unroll
                         for (uint32_t ks = 0; ks < 4; ks++)                // a block is one k-step: blocks behind the prefix are left out
-                            if (ks < nb) mma_ts(to, ts + b * ST + ks * 8, DESC_V | (v_lo + st * (TILE >> 4) + (4 * h + ks) * (2048u >> 4)), IDESC_PV,
-                                   (j > 0 || h > 0 || ks > 0) ? 1u : 0u);
+                            if (ks < nb) mma_ts(to, ts + b * ST + ks * 8, DESC_V | (v_lo + st * (TILE >> 4) + (4 * hp + ks) * (2048u >> 4)), IDESC_PV,
+                                   (jp > 0 || hp > 0 || ks > 0) ? 1u : 0u);
                         tc_commit(&c->pv_done[x][b]);
-                        if (h + 1 == steps) {
+                        if (last) {
                             tc_commit(c->v_empty + st);
                             if (same) tc_commit(c->v_empty + st);
                         }
                     }
                     __syncwarp();
-                    scores();
+                    np++;
+                    hp = last ? 0 : 1;
+                    jp += last ? 1 : 0;
                 }
             }
             if (!ok && lane == 0) atomicCAS(&c->fail, 0u, 4u);
@@ -345,52 +348,50 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                             for (uint32_t n = 0; n < (1u << 20) && !mbar_test((kv ? c->v_full : c->k_full) + (t & 1u), (t >> 1) & 1u); n++) {}
                 }
             } else {
-                // ---- widening: 128 threads, 16 bytes of a token at a time, a tile ahead in registers ----
+                // ---- widening: 128 threads, 16 bytes of a token at a time.  The bytes arrive a tile ahead by asynchronous copies; a thread copies
+                // what it will widen, so its own wait is enough.  (In registers they did not fit beside the softmax's share of them.) ----
                 constexpr int CPR = D / 16, PER = 128 * CPR / 128;             // 16-byte pieces of a row; per thread and tile
                 const uint32_t t128 = tid - SM * 32;
-                uint4 kr[PER], vr[PER];
-                float sc = 0.0f;
-                auto piece = [&](int e, uint32_t& row, uint32_t& ch) {          // a warp's 32 pieces: whole rows
-                    const uint32_t n = e * 128 + t128;
-                    row = n / CPR;
-                    ch = n % CPR;
-                };
-                // block ids a tile ahead of the loads that use them; an id outside the pool becomes 0 and is remembered, without a branch that would wait
+                const uint32_t raw[2] = {smem_u32(v_ring + 2 * TILE) + t128 * 16, smem_u32(v_ring + 2 * TILE) + 128 * D + t128 * 16};
+                // block ids a tile ahead of the copies that use them; an id outside the pool is remembered, without a branch that would wait
                 uint32_t id[PER], sc_id = 0;
                 bool foreign = false;
+                float sc = 1.0f;
                 auto look_up = [&](uint32_t i) {
                     const uint32_t nb = i < it.n_tiles ? blocks_in(i) : 0u;
 #pragma unroll
                     for (int e = 0; e < PER; e++) {
-                        uint32_t row, ch;
-                        piece(e, row, ch);
-                        id[e] = row / BS < nb ? table[(it.tile + i) * 8u + row / BS] : ~0u;
+                        const uint32_t b = (e * 128 + t128) / CPR / BS;
+                        id[e] = b < nb ? table[(it.tile + i) * 8u + b] : ~0u;
                     }
                     sc_id = (t128 & 7u) < nb ? table[(it.tile + i) * 8u + (t128 & 7u)] : ~0u;
                 };
-                auto load = [&](uint4 (&r)[PER], const char* base, uint32_t i) {
-                    const uint32_t nb = blocks_in(i);
+                auto copy = [&](int kv, uint32_t i) {                          // nothing but the group's mark behind the item's last tile
+                    if (i < it.n_tiles) {
+                        const char* base = (kv ? a.v8 : a.k8) + (size_t)it.kvh * D;
+                        const uint32_t nb = blocks_in(i);
 #pragma unroll
-                    for (int e = 0; e < PER; e++) {
-                        uint32_t row, ch;
-                        piece(e, row, ch);
-                        const bool in = id[e] < a.total_blocks;
-                        foreign |= !in && row / BS < nb;
-                        r[e] = in ? __ldg(reinterpret_cast<const uint4*>(base + (uint64_t)id[e] * a.block_stride + (size_t)(row % BS) * a.row_stride + (size_t)it.kvh * D + ch * 16))
-                                  : make_uint4(0, 0, 0, 0);
+                        for (int e = 0; e < PER; e++) {
+                            const uint32_t n = e * 128 + t128, row = n / CPR, ch = n % CPR;   // a warp's pieces: whole rows
+                            const bool in = id[e] < a.total_blocks;
+                            foreign |= !in && row / BS < nb;
+                            const char* src = base + (uint64_t)(in ? id[e] : 0u) * a.block_stride + (size_t)(row % BS) * a.row_stride + ch * 16;
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(raw[kv] + e * 2048u), "l"(src), "r"(in ? 16u : 0u) : "memory");
+                        }
                     }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
                 };
                 auto load_scales = [&]() {
                     sc = 1.0f;
                     if (t128 < 16 && a.k_scales) sc = sc_id < a.total_blocks ? __ldg((t128 < 8 ? a.k_scales : a.v_scales) + (size_t)sc_id * a.n_kv_heads + it.kvh) : 0.0f;
                 };
-                auto widen = [&](unsigned char* tile, const uint4 (&r)[PER]) {
+                auto widen = [&](unsigned char* tile, int kv) {
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");       // all but the other tensor's, asked for last
 #pragma unroll
                     for (int e = 0; e < PER; e++) {
-                        uint32_t row, ch;
-                        piece(e, row, ch);
-                        const uint32_t w[4] = {r[e].x, r[e].y, r[e].z, r[e].w};
-                        uint32_t h[8];
+                        const uint32_t n = e * 128 + t128, row = n / CPR, ch = n % CPR;
+                        uint32_t w[4], h[8];
+                        tkv_rows::shared_read16(raw[kv] + e * 2048u, w);
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             h[2 * k] = tkv_rows::e4m3x2_h2(w[k] & 0xFFFFu);
@@ -405,28 +406,27 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 };
                 look_up(0);
                 load_scales();
-                load(kr, a.k8, 0);
-                load(vr, a.v8, 0);
+                copy(0, 0);
+                copy(1, 0);
                 look_up(1);
                 for (uint32_t i = 0; i < it.n_tiles && ok; i++) {
                     const uint32_t t = tiles_done + i, st = t & 1u;
                     if (t >= 2) ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(c->k_empty + st), ((t >> 1) - 1u) & 1u, fail));
                     if (!ok) break;
                     if (t128 < 16) c->scales[t & 3u][t128] = sc;
-                    widen(k_ring + st * TILE, kr);
+                    widen(k_ring + st * TILE, 0);
                     if (lane == 0) mbar_arrive(c->k_full + st);
-                    if (i + 1 < it.n_tiles) {
-                        load_scales();
-                        load(kr, a.k8, i + 1);
-                    }
+                    load_scales();
+                    copy(0, i + 1);
                     if (t >= 2) ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(c->v_empty + st), ((t >> 1) - 1u) & 1u, fail));
                     if (!ok) break;
-                    widen(v_ring + st * TILE, vr);
+                    widen(v_ring + st * TILE, 1);
                     if (lane == 0) mbar_arrive(c->v_full + st);
-                    if (i + 1 < it.n_tiles) load(vr, a.v8, i + 1);
+                    copy(1, i + 1);
                     look_up(i + 2);
                     if (*fail) ok = false;
                 }
+                asm volatile("cp.async.wait_all;" ::: "memory");
                 if (foreign) atomicCAS(&c->fail, 0u, 2u);
                 if (!ok && lane == 0) atomicCAS(&c->fail, 0u, 4u);
             }
@@ -755,8 +755,8 @@ Layout layout_of(uint32_t n_seqs, uint32_t n_groups, uint32_t n_q_heads, uint32_
 }
 
 template <int D, bool FP8> cudaError_t launch_prefix(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, cudaStream_t st) {
-    constexpr size_t smem = CTRL_BYTES + 6 * (size_t)(D / 64) * GROUP_BYTES;
-    static_assert(smem + 4096 <= 227 * 1024, "shared memory of one CTA");
+    constexpr size_t smem = CTRL_BYTES + 6 * (size_t)(D / 64) * GROUP_BYTES + (FP8 ? 2 * 128 * (size_t)D : 0);
+    static_assert(smem <= 227 * 1024, "shared memory of one CTA");
     auto kernel = prefix_attn_tc<D, FP8>;
     static std::atomic<uint64_t> granted{0};                    // devices on which this kernel may use that much shared memory
     int dev = 0;
