@@ -9,8 +9,8 @@
 // results (m, l, O) of both: out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.
 //
 // A CTA works on up to 256 rows of one (group, kv head) as two streams of 128 with their own S, P and O: with more than 128 rows
-// the streams are two row tiles that read the same cached tiles; with fewer they are the same rows on alternate cached tiles (two
-// partial results).  A stream goes 64 cached tokens at a time through two S buffers: the scores of the next step are there when
+// the streams are two row tiles that read the same cached tiles; with fewer they are the same rows on the two halves of every cached
+// tile (two partial results).  A stream goes 64 cached tokens at a time through two S buffers: the scores of the next step are there when
 // the softmax of this one ends.  (One buffer of 128 tokens per stream left the softmax warps waiting for two products per tile:
 // 4 800 cycles per tile of both streams.)  A softmax thread owns a row: no exchange between threads.  P goes back to tensor memory, over
 // the S it was made from, as the A operand of the second product, so shared memory holds Q and the K and V tiles only.  The row maximum in use is raised, and O rescaled, only when a score exceeds it by 2^6.
@@ -228,14 +228,11 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             it.n_tiles = min(nt - it.tile, u_end - u);
             it.out_row = 2ull * ((uint64_t)(it.first_seq - a.group_starts[0]) * a.group * a.n_kv_heads + (uint64_t)it.kvh * it.rows + it.row0) + 512ull * blockIdx.x;
         }
-        const bool same_rows = it.block_rows <= 128;            // both streams the same rows, alternate tiles
+        const bool same_rows = it.block_rows <= 128;            // both streams the same rows, on halves of the tiles
         const uint32_t* table = a.tables + (size_t)it.first_seq * a.table_stride;
         const uint32_t n_blocks = it.prefix / BS;
         auto blocks_in = [&](uint32_t i) { return min(8u, n_blocks - (it.tile + i) * 8u); };   // of the item's i-th tile
         auto steps_in = [&](uint32_t i) { return blocks_in(i) > 4u ? 2u : 1u; };
-        uint32_t n_of[2];                                       // tiles of each stream
-        n_of[0] = same_rows ? (it.n_tiles + 1) / 2 : it.n_tiles;
-        n_of[1] = same_rows ? it.n_tiles / 2 : it.n_tiles;
 
         if (warp >= SM + FEED) {
             // ---- MMA issuers, a warp per stream.  Waits sleep in hardware (a polling issuer took issue slots from the softmax warps of its
@@ -243,74 +240,79 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             // steps ahead of the second product. ----
             // Broadcast from one lane, what selects operands is known to be the warp's own: addresses then are computed once per warp.
             auto uni = [](uint32_t v) { return __shfl_sync(0xFFFFFFFFu, v, 0); };
-            const uint32_t x = uni(warp - (SM + FEED)), n_x = uni(x ? n_of[1] : n_of[0]), s_x = uni(x ? n_steps[1] : n_steps[0]);
+            const uint32_t x = uni(warp - (SM + FEED)), s_x = uni(x ? n_steps[1] : n_steps[0]), n_t = uni(it.n_tiles);
             const uint32_t done = uni(tiles_done), n_left = uni(n_blocks - it.tile * 8u);
             const bool same = uni(same_rows ? 1u : 0u) != 0;
             auto blocks_at = [&](uint32_t i) { return min(8u, n_left - i * 8u); };
             const uint32_t q_lo = (smem_u32(q_tile) >> 4) + x * (TILE >> 4), k_lo = smem_u32(k_ring) >> 4, v_lo = smem_u32(v_ring) >> 4;
             const uint32_t ts = TM_S + x * 128, to = TM_O + x * 128;
             auto wait = [&](uint64_t* bar, uint32_t parity) {
-                if (ok) ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(bar), parity & 1u, fail));
+                if (ok) ok = bar_wait(smem_u32(bar), parity & 1u, fail);
             };
+            if (elect_one()) {
             wait(c->q_ready + x, item_no);
-            uint32_t jq = 0, hq = 0, nq = s_x;                   // tile, half and number of the next scores
-            uint32_t jp = 0, hp = 0, np = s_x;                   // of the next product
-            while (ok && jp < n_x) {
+            // steps of this stream in tile i: both halves, or (same rows) half x if it holds a block
+            auto steps_at = [&](uint32_t i) { return same ? (blocks_at(i) > 4u * x ? 1u : 0u) : blocks_at(i) > 4u ? 2u : 1u; };
+            const uint32_t n_i = n_t - (steps_at(n_t - 1) == 0 ? 1u : 0u);   // tiles with a step
+            uint32_t iq = 0, hq = 0, nq = s_x;                   // tile, step in it and number of the next scores
+            uint32_t ip = 0, hp = 0, np = s_x;                   // of the next product
+            while (ok && ip < n_i) {
                 // The scores run up to two steps ahead, but a tile that is not there yet holds up no product: that would hold up its V's place, too.
-                const uint32_t iq = same ? 2 * jq + x : jq, tq = done + iq, sq = tq & 1u;
-                bool ahead = jq < n_x && nq - np < 2;
+                const uint32_t tq = done + iq, sq = tq & 1u;
+                bool ahead = iq < n_i && nq - np < 2;
                 if (ahead && hq == 0) {
                     if (np == nq) wait(c->k_full + sq, tq >> 1);
-                    else ahead = __all_sync(0xFFFFFFFFu, mbar_test(c->k_full + sq, (tq >> 1) & 1u));
+                    else ahead = mbar_test(c->k_full + sq, (tq >> 1) & 1u);
                 }
                 if (ahead) {
-                    const uint32_t b = nq & 1u;
+                    const uint32_t b = nq & 1u, half = same ? x : hq;
                     if (nq >= 2) wait(&c->pv_done[x][b], (nq >> 1) - 1u);  // the buffer is free when the product that read P over it is done
                     if (!ok) break;
                     tc_fence_after();
-                    const bool last = hq + 1 == (blocks_at(iq) > 4u ? 2u : 1u);
-                    if (elect_one()) {
+                    const bool last = hq + 1 == steps_at(iq);
+                    {
 #pragma unroll
                         for (int ks = 0; ks < KSTEPS; ks++) {
                             const uint32_t off = (ks / 4) * (GROUP_BYTES >> 4) + (ks % 4) * 2;
-                            mma_ss(ts + b * ST, DESC_K | (q_lo + off), DESC_K | (k_lo + sq * (TILE >> 4) + hq * (ST * 128u >> 4) + off), IDESC_QK, ks > 0 ? 1u : 0u);
+                            mma_ss(ts + b * ST, DESC_K | (q_lo + off), DESC_K | (k_lo + sq * (TILE >> 4) + half * (ST * 128u >> 4) + off), IDESC_QK, ks > 0 ? 1u : 0u);
                         }
                         tc_commit(&c->s_full[x][b]);
-                        if (last) {
-                            tc_commit(c->k_empty + sq);                    // a tile goes back after two readings
-                            if (same) tc_commit(c->k_empty + sq);
-                        }
+                        if (last) tc_commit(c->k_empty + sq);              // a tile goes back when both streams have read it
                     }
-                    __syncwarp();
                     nq++;
                     hq = last ? 0 : 1;
-                    jq += last ? 1 : 0;
+                    iq += last ? 1 : 0;
                 } else {
-                    const uint32_t i = same ? 2 * jp + x : jp, t = done + i, st = t & 1u, b = np & 1u, all = blocks_at(i), nb = min(4u, all - 4u * hp);
+                    const uint32_t t = done + ip, st = t & 1u, b = np & 1u, half = same ? x : hp, nb = min(4u, blocks_at(ip) - 4u * half);
                     wait(&c->p_full[x][b], np >> 1);
                     if (hp == 0) wait(c->v_full + st, t >> 1);
                     if (!ok) break;
                     tc_fence_after();
-                    const bool last = hp + 1 == (all > 4u ? 2u : 1u);
-                    if (elect_one()) {
+                    const bool last = hp + 1 == steps_at(ip);
+                    {
 #pragma unroll
                         for (uint32_t ks = 0; ks < 4; ks++)                // a block is one k-step: blocks behind the prefix are left out
-                            if (ks < nb) mma_ts(to, ts + b * ST + ks * 8, DESC_V | (v_lo + st * (TILE >> 4) + (4 * hp + ks) * (2048u >> 4)), IDESC_PV,
-                                   (jp > 0 || hp > 0 || ks > 0) ? 1u : 0u);
+                            if (ks < nb) mma_ts(to, ts + b * ST + ks * 8, DESC_V | (v_lo + st * (TILE >> 4) + (4 * half + ks) * (2048u >> 4)), IDESC_PV,
+                                   (np > s_x || ks > 0) ? 1u : 0u);
                         tc_commit(&c->pv_done[x][b]);
-                        if (last) {
-                            tc_commit(c->v_empty + st);
-                            if (same) tc_commit(c->v_empty + st);
-                        }
+                        if (last) tc_commit(c->v_empty + st);
                     }
-                    __syncwarp();
                     np++;
                     hp = last ? 0 : 1;
-                    jp += last ? 1 : 0;
+                    ip += last ? 1 : 0;
                 }
             }
-            if (!ok && lane == 0) atomicCAS(&c->fail, 0u, 4u);
+            if (ok && n_i < n_t) {                               // the last tile has nothing for this stream: it goes back unread, once it is there
+                const uint32_t t = done + n_i, st = t & 1u;
+                wait(c->k_full + st, t >> 1);
+                if (ok) mbar_arrive(c->k_empty + st);
+                wait(c->v_full + st, t >> 1);
+                if (ok) mbar_arrive(c->v_empty + st);
+            }
+            if (!ok) atomicCAS(&c->fail, 0u, 4u);
+            }
             __syncwarp();
+            ok = *fail == 0;
         } else if (warp >= SM) {
             if (!FP8) {
                 // ---- producer: eight lanes, a block each ----
@@ -432,7 +434,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
         } else {
             // ---- softmax: one row per thread ----
-            const uint32_t x = warp >> 2, n_x = x ? n_of[1] : n_of[0], s_x = x ? n_steps[1] : n_steps[0], r = (warp & 3u) * 32u + lane, row = it.row0 + (same_rows ? 0u : x * 128u) + r;   // of the group and kv head
+            const uint32_t x = warp >> 2, s_x = x ? n_steps[1] : n_steps[0], r = (warp & 3u) * 32u + lane, row = it.row0 + (same_rows ? 0u : x * 128u) + r;   // of the group and kv head
             const bool live = row < it.rows && (same_rows ? r < it.block_rows : x * 128u + r < it.block_rows);
             const bool warp_live = __any_sync(0xFFFFFFFFu, live);
             const uint32_t seq = it.first_seq + (live ? row / a.group : 0u), head = it.kvh * a.group + (live ? row % a.group : 0u);
@@ -456,9 +458,9 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             const uint32_t lanes = ((warp & 3u) * 32u) << 16, ts = tmem + TM_S + x * 128 + lanes, to = tmem + TM_O + x * 128 + lanes;
             float m = -INFINITY, l = 0.0f, v_ref = FP8 ? 0x1p-100f : 1.0f, v_inv = FP8 ? 0x1p+100f : 1.0f;
             uint32_t n = s_x;                                   // steps of this stream so far
-            for (uint32_t j = 0; j < n_x && ok; j++) {
-                const uint32_t i = same_rows ? 2 * j + x : j, slot = (tiles_done + i) & 3u, steps = steps_in(i);
-                for (uint32_t h = 0; h < steps; h++, n++) {
+            for (uint32_t i = 0; i < it.n_tiles && ok; i++) {
+                const uint32_t slot = (tiles_done + i) & 3u, h_end = same_rows ? (blocks_in(i) > 4u * x ? x + 1 : x) : steps_in(i);
+                for (uint32_t h = same_rows ? x : 0u; h < h_end; h++, n++) {
                     const uint32_t t0 = (it.tile + i) * KT + h * ST, b = n & 1u;
                     ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(&c->s_full[x][b]), (n >> 1) & 1u, fail));
                     if (!ok) break;
@@ -593,9 +595,9 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         if (*fail) break;                                       // the same for all threads: nobody writes it between the two barriers
         __syncthreads();
         tiles_done += it.n_tiles;
-        const uint32_t last = it.n_tiles - 1, cut = 2 - steps_in(last);    // only a prefix's last tile has one step
-        n_steps[0] += 2 * n_of[0] - (same_rows && (last & 1u) ? 0 : cut);
-        n_steps[1] += 2 * n_of[1] - (same_rows && !(last & 1u) ? 0 : cut);
+        const uint32_t cut = 2 - steps_in(it.n_tiles - 1);      // only a prefix's last tile may hold one half
+        n_steps[0] += same_rows ? it.n_tiles : 2 * it.n_tiles - cut;
+        n_steps[1] += same_rows ? it.n_tiles - cut : 2 * it.n_tiles - cut;
         u += it.n_tiles;
     }
     if (warp >= SM + FEED && lane == 0) {                       // whatever ended the loop, no product is under way when tensor memory is given back
