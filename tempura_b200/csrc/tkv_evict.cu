@@ -5,7 +5,7 @@
 //     new_len = min(len, max(budget, protect + recent)),
 // ties to the lower index.  Scores become 32-bit keys that compare like the numbers (NaN below everything, -0 = +0); the key that
 // the last kept token has is found by histograms over 11, 11 and 10 bits of it, each over the tokens whose higher bits
-// agree with what is known; once these are few, one warp finishes bit by bit in registers.  A last pass writes the indices in ascending order (ballots inside a warp, prefix sums across warps
+// agree with what is known; once these are few, a thread ranks each of them against all.  A last pass writes the indices in ascending order (ballots inside a warp, prefix sums across warps
 // and CTAs).  Scores are read once into shared memory; the bound is HBM for many rows and latency for few, so a row is split over a
 // thread-block cluster, whose CTAs add their histograms through distributed shared memory, where there are fewer rows than SMs.
 //
@@ -17,6 +17,7 @@
 // are multiplied by scale / new scale <= 1 and rounded to E4M3 once more (half a step, 2^-4 relative, and flushed to zero below
 // 2^-6 as every writer of this pool does).  Taking the rows' absolute maximum instead would round every row again at every eviction.
 #include <cooperative_groups.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -24,8 +25,6 @@
 #include <stdint.h>
 
 #include "../../include/tkv.h"
-#define TKV_KERNELS_TEMPLATES_ONLY
-#include "tkv_kernels.cuh"
 
 namespace tkv_internal {
 int32_t set_error(int32_t code, int32_t cuda_code, const char* text);
@@ -37,7 +36,7 @@ namespace cg = cooperative_groups;
 
 constexpr int BS = 16;
 constexpr int BINS = 2048;
-constexpr int FEW = 256;                     // tokens that one warp holds in registers
+constexpr int FEW = 256;                     // tokens that are ranked against one another: at most one per thread
 constexpr uint32_t STAGE_TOKENS = 49152;     // tokens of a row that a CTA keeps in shared memory; longer slices are read again in every pass
 constexpr uint32_t MAX_CLUSTER = 8;
 
@@ -66,7 +65,7 @@ __device__ __forceinline__ uint32_t key_of(float x) {
     return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
 
-template <int THREADS> __global__ void __launch_bounds__(THREADS) evict_select(const SelectArgs a) {
+template <int THREADS> __global__ void __launch_bounds__(THREADS, 1536 / THREADS) evict_select(const SelectArgs a) {
     constexpr int WARPS = THREADS / 32, PER_THREAD = BINS / THREADS;
     static_assert(BINS % (4 * THREADS) == 0, "every thread clears the same number of bins");
     cg::cluster_group cluster = cg::this_cluster();
@@ -171,7 +170,7 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) evict_select(c
         const uint32_t in_bin = chosen[3];
         if (pass == 2) break;
         if (parts == 1 && in_bin <= (uint32_t)FEW) {
-            // few tokens share the known bits: they are gathered and one warp finds the rest of the key, bit by bit, in registers
+            // few tokens share the known bits: they are gathered
             for (uint32_t i0 = warp * 32; i0 < n; i0 += THREADS) {
                 const uint32_t i = i0 + lane, k = i < n ? key_at(i) : 0u;
                 const bool hit = i < n && (k & mask) == prefix;
@@ -184,22 +183,18 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) evict_select(c
                 }
             }
             __syncthreads();
-            if (warp == 0) {
-                uint32_t k[FEW / 32];
-#pragma unroll
-                for (int q = 0; q < FEW / 32; q++) k[q] = q * 32 + lane < in_bin ? few[q * 32 + lane] : ~prefix;   // ~prefix never matches
-                for (int b = shift - 1; b >= 0; b--) {
-                    const uint32_t bit = 1u << b, want = prefix | bit;
-                    mask |= bit;
-                    uint32_t ones = 0;
-#pragma unroll
-                    for (int q = 0; q < FEW / 32; q++) ones += __popc(__ballot_sync(0xFFFFFFFFu, (k[q] & mask) == want));
-                    if (left <= ones) prefix = want;
-                    else left -= ones;
+            // The key that `left` of them reach: every thread ranks one of them against all, threads of equal keys alike.
+            if (tid < in_bin) {
+                const uint32_t mine = few[tid];
+                uint32_t gt = 0, ge = 0;
+#pragma unroll 4
+                for (uint32_t i = 0; i < in_bin; i++) {
+                    gt += few[i] > mine;
+                    ge += few[i] >= mine;
                 }
-                if (lane == 0) {
-                    chosen[0] = prefix;
-                    chosen[1] = left;
+                if (gt < left && left <= ge) {
+                    chosen[0] = mine;
+                    chosen[1] = left - gt;
                 }
             }
             __syncthreads();
@@ -277,6 +272,16 @@ struct CompactArgs {
     uint32_t row_stride, n_seqs, n_kv_heads, table_stride, max_kv_len, total_blocks, kept_stride, score_stride;
 };
 constexpr int CMP_THREADS = 256;
+
+// Two E4M3 bytes of products that are at most 448: to nearest even, below 2^-6 to a signed zero like every writer of the pool (the
+// conversion alone would leave subnormals there); NaN stays NaN.
+__device__ __forceinline__ uint32_t encode_pair(float lo, float hi) {
+    if (fabsf(lo) < 0x1p-6f) lo = __uint_as_float(__float_as_uint(lo) & 0x80000000u);
+    if (fabsf(hi) < 0x1p-6f) hi = __uint_as_float(__float_as_uint(hi) & 0x80000000u);
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
 
 // ROW: bytes of one kv head's row.  blockIdx: x = (sequence, kv head), y = layer, z = K, V, scores.
 template <int ROW, bool SCALED> __global__ void __launch_bounds__(CMP_THREADS) evict_compact(const __grid_constant__ CompactArgs a) {
@@ -386,7 +391,7 @@ template <int ROW, bool SCALED> __global__ void __launch_bounds__(CMP_THREADS) e
                         asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h0) : "h"((unsigned short)(w[i] & 0xFFFFu)));
                         asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h1) : "h"((unsigned short)(w[i] >> 16)));
                         const float2 x0 = __half22float2(*reinterpret_cast<__half2*>(&h0)), x1 = __half22float2(*reinterpret_cast<__half2*>(&h1));
-                        w[i] = tkv::e4m3_encode_pair_hw(__fmul_rn(x0.x, f), __fmul_rn(x0.y, f)) | (tkv::e4m3_encode_pair_hw(__fmul_rn(x1.x, f), __fmul_rn(x1.y, f)) << 16);
+                        w[i] = encode_pair(__fmul_rn(x0.x, f), __fmul_rn(x0.y, f)) | (encode_pair(__fmul_rn(x1.x, f), __fmul_rn(x1.y, f)) << 16);
                     }
                     v[u] = make_uint4(w[0], w[1], w[2], w[3]);
                 }

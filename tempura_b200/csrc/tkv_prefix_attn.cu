@@ -624,23 +624,25 @@ struct JoinArgs {
 // WPR warps join the partial results of one (sequence, query head): one where there are rows enough to fill the machine, eight where
 // few rows have many parts.  Bound by latency and L2.
 template <int D, int WPR> __global__ void __launch_bounds__(256) prefix_join(const JoinArgs a) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");          // launched ahead of the second kernel's end
+    // what the caller wrote is read while the kernels before this one still run
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     const uint64_t row = WPR == 1 ? (uint64_t)blockIdx.x * 8 + warp : blockIdx.x;
     const bool in = row < (uint64_t)a.n_seqs * a.n_q_heads;
     const uint32_t s = in ? (uint32_t)(row / a.n_q_heads) : 0u, head = in ? (uint32_t)(row % a.n_q_heads) : 0u;
-    const uint32_t share_t = a.pre_plan[0], share_b = a.own_plan[0];
-    const uint32_t g = tkv_rows::group_of(a.group_starts, a.n_groups, s);
+    const uint32_t g = tkv_rows::group_of(a.group_starts, a.n_groups, s), g_in = min(g, a.n_groups - 1);
+    const uint32_t base = a.group_starts[0], s0 = a.group_starts[g_in], s1 = a.group_starts[g_in + 1], prefix = a.prefix_lens[g_in];
+    asm volatile("griddepcontrol.wait;" ::: "memory");          // launched ahead of the second kernel's end, which comes after the first one's
+    const uint32_t share_t = a.pre_plan[0], share_b = a.own_plan[0], tiles_before = a.pre_plan[1 + g_in], lo = a.own_plan[1 + s], hi = a.own_plan[2 + s];
     if (!in || share_t == 0 || share_b == 0 || g == a.n_groups) return;   // (all warps of a row alike) refused, or a row behind the last sequence
     // parts of the prefix
-    const uint32_t s0 = a.group_starts[g], rows = (a.group_starts[g + 1] - s0) * a.group, kvh = head / a.group, r = (s - s0) * a.group + head % a.group;
-    const uint32_t rb = r / 256, block_rows = min(256u, rows - rb * 256), nt = (a.prefix_lens[g] + KT - 1) / KT;
+    const uint32_t rows = (s1 - s0) * a.group, kvh = head / a.group, r = (s - s0) * a.group + head % a.group;
+    const uint32_t rb = r / 256, block_rows = min(256u, rows - rb * 256), nt = (prefix + KT - 1) / KT;
     const bool same_rows = block_rows <= 128;
-    const uint32_t t0 = a.pre_plan[1 + g] + (kvh * row_blocks(rows) + rb) * nt, c0 = nt ? t0 / share_t : 0u, k = same_rows ? 2u : 1u;
+    const uint32_t t0 = tiles_before + (kvh * row_blocks(rows) + rb) * nt, c0 = nt ? t0 / share_t : 0u, k = same_rows ? 2u : 1u;
     const uint32_t n_pre = nt ? ((t0 + nt - 1) / share_t - c0 + 1) * k : 0u;
-    const uint64_t first = 2ull * ((uint64_t)(s0 - a.group_starts[0]) * a.group * a.n_kv_heads + (uint64_t)kvh * rows + rb * 256) + 512ull * c0 + r % 256;
+    const uint64_t first = 2ull * ((uint64_t)(s0 - base) * a.group * a.n_kv_heads + (uint64_t)kvh * rows + rb * 256) + 512ull * c0 + r % 256;
     // parts of the tokens behind it
-    const uint32_t lo = a.own_plan[1 + s], hi = a.own_plan[2 + s], p0 = hi > lo ? lo / share_b : 0u;
+    const uint32_t p0 = hi > lo ? lo / share_b : 0u;
     const uint32_t n_own = hi > lo ? ((hi - 1) / share_b - p0 + 1) * a.subs : 0u, n = n_pre + n_own;
     auto part = [&](uint32_t i, const float*& o, const float*& ml) {
         if (i < n_pre) {
