@@ -112,11 +112,19 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS, 1536 / THREADS
         if (tid == 0) chosen[2] = 0;
         __syncthreads();
         if (pass == 0) {                                        // the scores are read here
-#pragma unroll 4
-            for (uint32_t i = tid; i < n; i += THREADS) {
-                const uint32_t k = key_of(src[i]);
-                if (a.staged) keys[i] = k;
-                atomicAdd(&hist[k >> 21], 1u);
+            constexpr int AHEAD = 8;                            // asked for together
+            for (uint32_t i0 = tid; i0 < n; i0 += AHEAD * THREADS) {
+                float x[AHEAD];
+#pragma unroll
+                for (int q = 0; q < AHEAD; q++) x[q] = i0 + q * THREADS < n ? src[i0 + q * THREADS] : 0.0f;
+#pragma unroll
+                for (int q = 0; q < AHEAD; q++) {
+                    const uint32_t i = i0 + q * THREADS, k = key_of(x[q]);
+                    if (i < n) {
+                        if (a.staged) keys[i] = k;
+                        atomicAdd(&hist[k >> 21], 1u);
+                    }
+                }
             }
         } else {
             for (uint32_t i = tid; i < n; i += THREADS) {
