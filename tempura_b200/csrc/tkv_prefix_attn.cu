@@ -16,8 +16,9 @@
 // the S it was made from, as the A operand of the second product, so shared memory holds Q and the K and V tiles only.  The row maximum in use is raised, and O rescaled, only when a score exceeds it by 2^6.
 // An F16 pool's tiles arrive as tensor-map boxes, in the 128-byte swizzle the MMA reads.  An E4M3 pool's tiles are widened to F16
 // on the way by four warps (exact); K's block scale multiplies the scores, V's the probabilities, in units of a power of two above every
-// scale met so far.  Both operands of both products are then F16 and the products exact; a probability is rounded to F16 once (2^-11 of
-// its value at most, like the output itself).
+// scale met so far.  Both operands of both products are then F16 and the products exact.  With up to 128 rows, where the tensor cores
+// wait for the cache, a probability is two F16 terms (22 bits); with more, where they are the bound, it is rounded to F16 once: 2^-11 of its
+// value at most, as much as the rounding of the output.
 //
 // Work split: the cached tiles of all (group, kv head, row block) items, one after another, in equal shares, one per CTA; a share may
 // begin and end inside an item.  The partial rows of item i and share c start at 2 * (rows before item i) + 512 * c, which keeps them
@@ -87,6 +88,10 @@ struct Item {
 __device__ __forceinline__ uint32_t row_blocks(uint32_t rows) { return (rows + 255) / 256; }
 
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) { mma<false>(d, a, b, idesc, acc); }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
 __device__ __forceinline__ bool elect_one() {
     uint32_t yes;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
@@ -294,6 +299,11 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         for (uint32_t ks = 0; ks < 4; ks++)                // a block is one k-step: blocks behind the prefix are left out
                             if (ks < nb) mma_ts(to, ts + b * ST + ks * 8, DESC_V | (v_lo + st * (TILE >> 4) + (4 * half + ks) * (2048u >> 4)), IDESC_PV,
                                    (np > s_x || ks > 0) ? 1u : 0u);
+                        if (same) {                                        // the second terms of the probabilities
+#pragma unroll
+                            for (uint32_t ks = 0; ks < 4; ks++)
+                                if (ks < nb) mma_ts(to, ts + b * ST + 32 + ks * 8, DESC_V | (v_lo + st * (TILE >> 4) + (4 * half + ks) * (2048u >> 4)), IDESC_PV, 1u);
+                        }
                         tc_commit(&c->pv_done[x][b]);
                         if (last) tc_commit(c->v_empty + st);
                     }
@@ -469,8 +479,8 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         const int left = (int)min(limit > t0 ? limit - t0 : 0u, (uint32_t)ST);   // tokens of the step that the row attends to
                         const uint32_t tb = ts + b * ST;
                         const float* sc = c->scales[slot] + 4 * h;
-                        auto step = [&](auto masked_type) {
-                            constexpr bool MASKED = decltype(masked_type)::value;
+                        auto step = [&](auto masked_type, auto two_type) {
+                            constexpr bool MASKED = decltype(masked_type)::value, TWO = decltype(two_type)::value;
                             uint32_t v[2][32];
                             tmem_ld32(tb, v[0]);
                             tmem_ld32(tb + 32, v[1]);
@@ -518,6 +528,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                             // ---- probabilities, as F16 pairs over the scores ----
                             const float sub = m == -INFINITY ? 0.0f : -m;
                             float sum = 0.0f;
+                            uint32_t second[2][8];
 #pragma unroll
                             for (int q = 0; q < 4; q++) {
                                 const float ks = FP8 ? a.scale_log2 * sc[q] : a.scale_log2, vn = FP8 ? sc[8 + q] * v_inv : 1.0f;
@@ -534,16 +545,29 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                                         p0 *= vn;
                                         p1 *= vn;
                                     }
+                                    // into the registers of the block's scores: eight of first terms, eight of second ones
                                     const __half2 hp = __floats2half2_rn(p0, p1);
-                                    v[0][q * 8 + k / 2] = *reinterpret_cast<const uint32_t*>(&hp);
+                                    v[q / 2][(q & 1) * 16 + k / 2] = *reinterpret_cast<const uint32_t*>(&hp);
+                                    if (TWO) {
+                                        const float2 fp = __half22float2(hp);
+                                        const __half2 lp = __floats2half2_rn(p0 - fp.x, p1 - fp.y);
+                                        second[q & 1][k / 2] = *reinterpret_cast<const uint32_t*>(&lp);
+                                    }
                                 }
+                                tmem_st8(tb + q * 8, v[q / 2] + (q & 1) * 16);
+                                if (TWO) tmem_st8(tb + 32 + q * 8, second[q & 1]);
                             }
-                            tmem_st32(tb, v[0]);
                             tmem_wait_st();
                             l += sum;
                         };
-                        if (__any_sync(0xFFFFFFFFu, left < ST)) step(std::true_type{});
-                        else step(std::false_type{});
+                        const bool masked = __any_sync(0xFFFFFFFFu, left < ST);
+                        if (same_rows) {
+                            if (masked) step(std::true_type{}, std::true_type{});
+                            else step(std::false_type{}, std::true_type{});
+                        } else {
+                            if (masked) step(std::true_type{}, std::false_type{});
+                            else step(std::false_type{}, std::false_type{});
+                        }
                         tc_fence_before();
                     }
                     __syncwarp();
