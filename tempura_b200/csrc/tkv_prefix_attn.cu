@@ -10,7 +10,8 @@
 //
 // A CTA works on up to 256 rows of one (group, kv head) as two streams of 128 with their own S, P and O: with more than 128 rows
 // the streams are two row tiles that read the same cached tiles; with fewer they are the same rows on the two halves of every cached
-// tile (two partial results).  A stream goes 64 cached tokens at a time through two S buffers: the scores of the next step are there when
+// tile (two partial results).  Up to 64 or 32 rows are there two or four times: the copies take the blocks of a step in turns, so
+// that a softmax warp, whose time per step is latency, has half or a quarter of it to do; P of the blocks that are not its own is 0.  A stream goes 64 cached tokens at a time through two S buffers: the scores of the next step are there when
 // the softmax of this one ends.  (One buffer of 128 tokens per stream left the softmax warps waiting for two products per tile:
 // 4 800 cycles per tile of both streams.)  A softmax thread owns a row: no exchange between threads.  P goes back to tensor memory, over
 // the S it was made from, as the A operand of the second product, so shared memory holds Q and the K and V tiles only.  The row maximum in use is raised, and O rescaled, only when a score exceeds it by 2^6.
@@ -21,7 +22,7 @@
 // value at most, as much as the rounding of the output.
 //
 // Work split: the cached tiles of all (group, kv head, row block) items, one after another, in equal shares, one per CTA; a share may
-// begin and end inside an item.  The partial rows of item i and share c start at 2 * (rows before item i) + 512 * c, which keeps them
+// begin and end inside an item.  The partial rows of item i and share c start at 8 * (rows before item i) + 512 * c, which keeps them
 // apart because both only grow along the work.
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -85,6 +86,8 @@ struct Item {
     uint32_t kvh, prefix, tile, n_tiles;          // tiles [tile, tile + n_tiles) of the prefix
     uint64_t out_row;                             // first partial row
 };
+// copies of the rows of a short row block
+__host__ __device__ __forceinline__ uint32_t copies_of(uint32_t block_rows) { return block_rows <= 32 ? 4u : block_rows <= 64 ? 2u : 1u; }
 __device__ __forceinline__ uint32_t row_blocks(uint32_t rows) { return (rows + 255) / 256; }
 
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) { mma<false>(d, a, b, idesc, acc); }
@@ -231,7 +234,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             it.block_rows = min(256u, it.rows - it.row0);
             it.tile = (u - at) % nt;
             it.n_tiles = min(nt - it.tile, u_end - u);
-            it.out_row = 2ull * ((uint64_t)(it.first_seq - a.group_starts[0]) * a.group * a.n_kv_heads + (uint64_t)it.kvh * it.rows + it.row0) + 512ull * blockIdx.x;
+            it.out_row = 8ull * ((uint64_t)(it.first_seq - a.group_starts[0]) * a.group * a.n_kv_heads + (uint64_t)it.kvh * it.rows + it.row0) + 512ull * blockIdx.x;
         }
         const bool same_rows = it.block_rows <= 128;            // both streams the same rows, on halves of the tiles
         const uint32_t* table = a.tables + (size_t)it.first_seq * a.table_stride;
@@ -444,8 +447,10 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
         } else {
             // ---- softmax: one row per thread ----
-            const uint32_t x = warp >> 2, s_x = x ? n_steps[1] : n_steps[0], r = (warp & 3u) * 32u + lane, row = it.row0 + (same_rows ? 0u : x * 128u) + r;   // of the group and kv head
-            const bool live = row < it.rows && (same_rows ? r < it.block_rows : x * 128u + r < it.block_rows);
+            const uint32_t x = warp >> 2, s_x = x ? n_steps[1] : n_steps[0], r = (warp & 3u) * 32u + lane;
+            const uint32_t copies = same_rows ? copies_of(it.block_rows) : 1u, copy = r / (128u / copies), r_own = r % (128u / copies);   // copy: the warp's
+            const uint32_t row = it.row0 + (same_rows ? 0u : x * 128u) + r_own;    // of the group and kv head
+            const bool live = same_rows ? r_own < it.block_rows : x * 128u + r_own < it.block_rows;
             const bool warp_live = __any_sync(0xFFFFFFFFu, live);
             const uint32_t seq = it.first_seq + (live ? row / a.group : 0u), head = it.kvh * a.group + (live ? row % a.group : 0u);
             const uint32_t limit = live ? min(min(a.kv_lens[seq], a.max_kv_len), it.prefix) : 0u;
@@ -479,20 +484,23 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         const int left = (int)min(limit > t0 ? limit - t0 : 0u, (uint32_t)ST);   // tokens of the step that the row attends to
                         const uint32_t tb = ts + b * ST;
                         const float* sc = c->scales[slot] + 4 * h;
-                        auto step = [&](auto masked_type, auto two_type) {
-                            constexpr bool MASKED = decltype(masked_type)::value, TWO = decltype(two_type)::value;
-                            uint32_t v[2][32];
-                            tmem_ld32(tb, v[0]);
-                            tmem_ld32(tb + 32, v[1]);
+                        auto step = [&](auto masked_type, auto copies_type) {
+                            constexpr bool MASKED = decltype(masked_type)::value, TWO = decltype(copies_type)::value > 0;
+                            constexpr int NB = 4 / (TWO ? decltype(copies_type)::value : 1);   // blocks of this warp: q0 ..
+                            const uint32_t q0 = TWO ? copy * NB : 0u;
+                            const float* sq = sc + q0;
+                            const int mine = left - (int)q0 * 16;
+                            uint32_t v[NB][16];
+#pragma unroll
+                            for (int q = 0; q < NB; q++) tmem_ld16(tb + (q0 + q) * 16, v[q]);
                             tmem_wait_ld();
                             float mx = -INFINITY;               // neither scale is negative: the maximum commutes with them
 #pragma unroll
-                            for (int q = 0; q < 4; q++) {       // a block
+                            for (int q = 0; q < NB; q++) {      // a block
                                 float top = -INFINITY;
 #pragma unroll
-                                for (int k = 0; k < 16; k++)
-                                    top = fmaxf(top, MASKED && q * 16 + k >= left ? -INFINITY : __uint_as_float(v[q / 2][(q & 1) * 16 + k]));
-                                mx = FP8 ? fmaxf(mx, top == -INFINITY ? top : top * sc[q]) : fmaxf(mx, top);
+                                for (int k = 0; k < 16; k++) top = fmaxf(top, MASKED && q * 16 + k >= mine ? -INFINITY : __uint_as_float(v[q][k]));
+                                mx = FP8 ? fmaxf(mx, top == -INFINITY ? top : top * sq[q]) : fmaxf(mx, top);
                             }
                             mx = mx == -INFINITY ? mx : mx * a.scale_log2;
                             // ---- a raised maximum or V scale rescales the row of O, once the product of the step before is done ----
@@ -503,8 +511,10 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                                 l *= factor;
                             }
                             if (FP8) {
-                                const float top = fmaxf(fmaxf(sc[8], sc[9]), fmaxf(sc[10], sc[11]));
-                                if (top > v_ref) {              // the same in every thread
+                                float top = sq[8];
+#pragma unroll
+                                for (int q = 1; q < NB; q++) top = fmaxf(top, sq[8 + q]);
+                                if (top > v_ref) {              // the same in every thread of the warp
                                     const float up = __uint_as_float(min((__float_as_uint(top) >> 23) + 1u, 253u) << 23);
                                     factor *= v_ref / up;
                                     v_ref = up;
@@ -528,46 +538,55 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                             // ---- probabilities, as F16 pairs over the scores ----
                             const float sub = m == -INFINITY ? 0.0f : -m;
                             float sum = 0.0f;
-                            uint32_t second[2][8];
 #pragma unroll
-                            for (int q = 0; q < 4; q++) {
-                                const float ks = FP8 ? a.scale_log2 * sc[q] : a.scale_log2, vn = FP8 ? sc[8 + q] * v_inv : 1.0f;
+                            for (int q = 0; q < NB; q++) {
+                                const float ks = FP8 ? a.scale_log2 * sq[q] : a.scale_log2, vn = FP8 ? sq[8 + q] * v_inv : 1.0f;
+                                uint32_t first[8], second[8];
 #pragma unroll
                                 for (int k = 0; k < 16; k += 2) {
-                                    float p0 = fast_exp2(__fmaf_rn(__uint_as_float(v[q / 2][(q & 1) * 16 + k]), ks, sub));
-                                    float p1 = fast_exp2(__fmaf_rn(__uint_as_float(v[q / 2][(q & 1) * 16 + k + 1]), ks, sub));
+                                    float p0 = fast_exp2(__fmaf_rn(__uint_as_float(v[q][k]), ks, sub));
+                                    float p1 = fast_exp2(__fmaf_rn(__uint_as_float(v[q][k + 1]), ks, sub));
                                     if (MASKED) {
-                                        p0 = q * 16 + k < left ? p0 : 0.0f;
-                                        p1 = q * 16 + k + 1 < left ? p1 : 0.0f;
+                                        p0 = q * 16 + k < mine ? p0 : 0.0f;
+                                        p1 = q * 16 + k + 1 < mine ? p1 : 0.0f;
                                     }
                                     sum += p0 + p1;
                                     if (FP8) {
                                         p0 *= vn;
                                         p1 *= vn;
                                     }
-                                    // into the registers of the block's scores: eight of first terms, eight of second ones
                                     const __half2 hp = __floats2half2_rn(p0, p1);
-                                    v[q / 2][(q & 1) * 16 + k / 2] = *reinterpret_cast<const uint32_t*>(&hp);
+                                    first[k / 2] = *reinterpret_cast<const uint32_t*>(&hp);
                                     if (TWO) {
                                         const float2 fp = __half22float2(hp);
                                         const __half2 lp = __floats2half2_rn(p0 - fp.x, p1 - fp.y);
-                                        second[q & 1][k / 2] = *reinterpret_cast<const uint32_t*>(&lp);
+                                        second[k / 2] = *reinterpret_cast<const uint32_t*>(&lp);
                                     }
                                 }
-                                tmem_st8(tb + q * 8, v[q / 2] + (q & 1) * 16);
-                                if (TWO) tmem_st8(tb + 32 + q * 8, second[q & 1]);
+                                tmem_st8(tb + (q0 + q) * 8, first);
+                                if (TWO) tmem_st8(tb + 32 + (q0 + q) * 8, second);
+                            }
+                            if (NB < 4) {                       // the other copies' blocks
+                                const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+                                for (uint32_t q = 0; q < 4; q++)
+                                    if (q / NB != copy) {
+                                        tmem_st8(tb + q * 8, zero);
+                                        tmem_st8(tb + 32 + q * 8, zero);
+                                    }
                             }
                             tmem_wait_st();
                             l += sum;
                         };
                         const bool masked = __any_sync(0xFFFFFFFFu, left < ST);
-                        if (same_rows) {
-                            if (masked) step(std::true_type{}, std::true_type{});
-                            else step(std::false_type{}, std::true_type{});
-                        } else {
-                            if (masked) step(std::true_type{}, std::false_type{});
-                            else step(std::false_type{}, std::false_type{});
-                        }
+                        auto dispatch = [&](auto copies_type) {
+                            if (masked) step(std::true_type{}, copies_type);
+                            else step(std::false_type{}, copies_type);
+                        };
+                        if (!same_rows) dispatch(std::integral_constant<int, 0>{});
+                        else if (copies == 4) dispatch(std::integral_constant<int, 4>{});
+                        else if (copies == 2) dispatch(std::integral_constant<int, 2>{});
+                        else dispatch(std::integral_constant<int, 1>{});
                         tc_fence_before();
                     }
                     __syncwarp();
@@ -576,7 +595,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
             // ---- partial result of the row ----
             const bool any = n > s_x;
-            const uint64_t dst = it.out_row + (same_rows ? x * it.block_rows + r : x * 128u + r);
+            const uint64_t dst = it.out_row + (same_rows ? (x * copies + copy) * it.block_rows + r_own : x * 128u + r);
             if (ok && any) ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(&c->pv_done[x][(n - 1) & 1u]), ((n - 1) >> 1) & 1u, fail));
             if (ok && warp_live) {
                 tc_fence_after();
@@ -587,7 +606,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     constexpr int DH = D / 2, CH = DH / 4;      // dims of a pass; its 16-byte chunks per row
                     unsigned char* stage = q_tile + x * TILE + (warp & 3u) * (TILE / 4);
                     const uint32_t n_live = (uint32_t)__popc(__ballot_sync(0xFFFFFFFFu, live));
-                    float* rows_out = a.part_o + (dst - lane) * D;
+                    float* rows_out = a.part_o + (dst - lane) * D;             // (the warp's first row is alive if any is)
 #pragma unroll 1
                     for (int d0 = 0; d0 < D; d0 += DH) {
 #pragma unroll
@@ -662,9 +681,9 @@ template <int D, int WPR> __global__ void __launch_bounds__(256) prefix_join(con
     const uint32_t rows = (s1 - s0) * a.group, kvh = head / a.group, r = (s - s0) * a.group + head % a.group;
     const uint32_t rb = r / 256, block_rows = min(256u, rows - rb * 256), nt = (prefix + KT - 1) / KT;
     const bool same_rows = block_rows <= 128;
-    const uint32_t t0 = tiles_before + (kvh * row_blocks(rows) + rb) * nt, c0 = nt ? t0 / share_t : 0u, k = same_rows ? 2u : 1u;
+    const uint32_t t0 = tiles_before + (kvh * row_blocks(rows) + rb) * nt, c0 = nt ? t0 / share_t : 0u, k = same_rows ? 2u * copies_of(block_rows) : 1u;
     const uint32_t n_pre = nt ? ((t0 + nt - 1) / share_t - c0 + 1) * k : 0u;
-    const uint64_t first = 2ull * ((uint64_t)(s0 - base) * a.group * a.n_kv_heads + (uint64_t)kvh * rows + rb * 256) + 512ull * c0 + r % 256;
+    const uint64_t first = 8ull * ((uint64_t)(s0 - base) * a.group * a.n_kv_heads + (uint64_t)kvh * rows + rb * 256) + 512ull * c0 + r % 256;
     // parts of the tokens behind it
     const uint32_t p0 = hi > lo ? lo / share_b : 0u;
     const uint32_t n_own = hi > lo ? ((hi - 1) / share_b - p0 + 1) * a.subs : 0u, n = n_pre + n_own;
@@ -772,7 +791,7 @@ Layout layout_of(uint32_t n_seqs, uint32_t n_groups, uint32_t n_q_heads, uint32_
     const uint64_t tiles = (n_groups + (uint64_t)n_seqs * group / 256) * n_kv_heads * nt;      // at most: every group ends in a row block of its own
     l.parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(CTAS, (tiles + MIN_SHARE - 1) / MIN_SHARE));
     l.own = tkv_rows::split_for((uint64_t)n_seqs * ((max_kv_len + 15ull) / 16), n_kv_heads, CTAS);
-    const uint64_t rows = 2ull * n_seqs * n_q_heads + 512ull * l.parts, slots = ((uint64_t)l.own.parts + n_seqs) * 2;   // two results per slot of an E4M3 pool
+    const uint64_t rows = 8ull * n_seqs * n_q_heads + 512ull * l.parts, slots = ((uint64_t)l.own.parts + n_seqs) * 2;   // two results per slot of an E4M3 pool
     l.pre_ml = up(4ull * (n_groups + 2ull), 256);
     l.pre_o = l.pre_ml + up(rows * 8, 256);
     l.own_plan = l.pre_o + up(rows * head_dim * 4, 256);
