@@ -446,6 +446,7 @@ int32_t tkv_evict_select_enqueue(const TkvEvictSelect* p, void* stream) {
     uint32_t cluster = 1;
     while (cluster < MAX_CLUSTER && (rows * cluster < 296 ? p->max_kv_len / cluster > 2048 : p->max_kv_len / cluster > STAGE_TOKENS)) cluster *= 2;
     if (rows * cluster > 0x7FFFFFFFull) return fail(TKV_ERR_INVALID_CONFIG, "%llu rows: batch too large", rows);
+    if (p->new_lens == p->kv_lens) return fail(TKV_ERR_INVALID_CONFIG, "new_lens must not be kv_lens: every row reads the old length");
     const uint32_t slice = (p->max_kv_len + cluster - 1) / cluster;
     SelectArgs a{};
     a.scores = reinterpret_cast<const float*>(p->scores);

@@ -102,6 +102,13 @@ def test_select_refuses(L, change, code):
     assert L.tkv_evict_select_enqueue(C.byref(select(**change)), None) == code
 
 
+def test_select_refuses_to_write_the_lengths_it_reads(L):
+    assert L.tkv_evict_select_enqueue(C.byref(select(kv_lens=A, new_lens=A)), None) == BAD
+    text = C.create_string_buffer(256)
+    L.tkv_last_error(text, 256)
+    assert b"new_lens" in text.value
+
+
 @pytest.mark.parametrize("change,code", [({"layer_begin": 1}, BAD), ({"n_layers": 3}, BAD), ({"layer_begin": 0xFFFFFFFF}, BAD), ({"tables": 0}, BAD), ({"kv_lens": 0}, BAD),
                                          ({"kept": 0}, BAD), ({"new_lens": 0}, BAD), ({"kept": A + 2}, BAD), ({"table_stride": 9}, DIM),
                                          ({"scores": A, "score_stride": 100}, DIM), ({"n_seqs": 0x80000000}, BAD)])
