@@ -453,7 +453,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             const bool live = same_rows ? r_own < it.block_rows : x * 128u + r_own < it.block_rows;
             const bool warp_live = __any_sync(0xFFFFFFFFu, live);
             const uint32_t seq = it.first_seq + (live ? row / a.group : 0u), head = it.kvh * a.group + (live ? row % a.group : 0u);
-            const uint32_t limit = live ? min(min(a.kv_lens[seq], a.max_kv_len), it.prefix) : 0u;
+            const uint32_t limit = live && min(a.kv_lens[seq], a.max_kv_len) >= it.prefix ? it.prefix : 0u;   // shorter members: rows_attn
             {
                 // Q rows of the warp, whole rows per load (a row per thread took 8 000 cycles)
                 constexpr int CPR = D / 8, RPL = 32 / CPR;      // 16-byte chunks of a row; rows per load

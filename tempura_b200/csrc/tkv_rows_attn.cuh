@@ -142,14 +142,21 @@ __device__ __forceinline__ uint32_t group_of(const uint32_t* starts, uint32_t n_
     return lo;
 }
 
-// tokens [x, y) of sequence s that the rows kernel attends to; x is a whole number of blocks
+// Tokens [x, y) of sequence s that the rows kernel attends to; x is a whole number of blocks.  A member that ends inside its group's
+// prefix comes here whole (x = SHORT), with the table row that names the prefix: in the matrix product over the prefix the tokens
+// behind its end would be zeros times V, and 0 x infinity and 0 x NaN are NaN.
+constexpr uint32_t SHORT = 1;                // below a block: x / BS is 0
 __device__ __forceinline__ uint2 own_range(const Args& a, uint32_t s) {
     const uint32_t len = min(a.kv_lens[s], a.max_kv_len);
     if (!a.group_starts) return make_uint2(0u, len);
     const uint32_t g = group_of(a.group_starts, a.n_groups, s);
     if (g == a.n_groups) return make_uint2(0u, 0u);
     const uint32_t begin = a.prefix_lens[g];
-    return begin < len ? make_uint2(begin, len) : make_uint2(0u, 0u);
+    return begin < len ? make_uint2(begin, len) : begin == len ? make_uint2(0u, 0u) : make_uint2(SHORT, len);
+}
+// the table row of a sequence with that range
+__device__ __forceinline__ uint32_t table_row(const Args& a, uint2 range, uint32_t s) {
+    return range.x == SHORT ? a.group_starts[group_of(a.group_starts, a.n_groups, s)] : s;
 }
 __device__ __forceinline__ uint32_t blocks_of(uint2 r) { return (r.y + BS - 1) / BS - r.x / BS; }
 
@@ -164,6 +171,7 @@ template <int D, bool FP8> struct Shape {
 struct Cursor {
     uint32_t seq, block, left;                                  // block of the sequence; blocks left in it for this part
     uint32_t len;                                               // tokens of the sequence
+    uint32_t row;                                               // of the block table
     uint32_t rest;                                              // blocks left for this part behind this sequence
 };
 
@@ -265,6 +273,7 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
         c.block = r.x / BS + (first - at);
         c.left = min(blocks_of(r) - (first - at), n);
         c.len = r.y;
+        c.row = table_row(a, r, s);
         c.rest = n - c.left;
         return c;
     };
@@ -275,10 +284,11 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
         x.block = r.x / BS;
         x.left = min(blocks_of(r), x.rest);
         x.len = r.y;
+        x.row = table_row(a, r, x.seq);
         x.rest -= x.left;
     };
     // a table entry; it is checked where it is used, a few blocks later, so that nothing waits for the load here
-    auto table_entry = [&](const Cursor& x, uint32_t i) -> uint32_t { return __ldg(a.tables + (size_t)x.seq * a.table_stride + x.block + i); };
+    auto table_entry = [&](const Cursor& x, uint32_t i) -> uint32_t { return __ldg(a.tables + (size_t)x.row * a.table_stride + x.block + i); };
     auto checked = [&](uint32_t id) -> uint32_t {
         if (id < a.total_blocks) return id;
         report(a.status, 2u);                                   // never dereferenced: block 0 is read instead and the launch reports it

@@ -389,6 +389,42 @@ def test_prefix_attention_leaves_padded_rows_and_serves_short_members(H):
     assert (out[2] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", ["f16", "e4m3"])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_prefix_attention_row_blocks_of_every_width(H, dtype, head_dim):
+    """Groups of one query head per kv head whose row counts are at, below and above each width at which rows are laid out differently."""
+    sizes = [1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257]
+    c, q, attn, lens = prefix_case(H, dtype, 1, head_dim, 1, sizes, [16 * (1 + 3 * g) for g in range(len(sizes))], [3, 0, 17], seed=21)
+    attn.out.fill_(float("nan"))
+    out = attn.enqueue(0)
+    assert int(attn.status.item()) == 0
+    for s, (want, _, vmax) in enumerate(c.attention(0, q, attn.sm_scale)):
+        out_close(out[s], want, vmax, False)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "e4m3"])
+@pytest.mark.parametrize("poison", ["nan", "inf"])
+def test_prefix_attention_member_shorter_than_its_prefix_sees_nothing_behind_its_end(H, dtype, poison):
+    """What the prefix holds behind a short member's end, NaN and infinities included, is no part of that member's result."""
+    import torch
+    c, q, attn, lens = prefix_case(H, dtype, 2, 128, 4, [3, 2], [160, 32], [-90, 5, 0, -16, 3], seed=22)
+    assert lens[0] == 70 and lens[3] == 16
+    for s, first in ((0, 70), (3, 16)):
+        for t in range(first, 160 if s == 0 else 32):
+            for is_v in (False, True):
+                row = c.pool.blocks(0, is_v)[int(attn.tables[s, t // BS]), t % BS]
+                if dtype == "f16":
+                    row.fill_(float(poison) * (-1 if t % 2 else 1))
+                else:
+                    row.fill_(0x7F if t % 2 else 0xFF)                # the type has no infinity
+    attn.out.fill_(float("nan"))
+    out = attn.enqueue(0)
+    assert int(attn.status.item()) == 0
+    want = c.attention(0, q, attn.sm_scale)
+    for s in (0, 3):
+        out_close(out[s], want[s][0], want[s][2], False)
+
+
 def test_prefix_attention_equals_decode_attention_without_groups_of_more_than_one(H):
     """Every sequence its own group: what the plain decode attention computes, to both kernels' rounding."""
     import torch
@@ -420,6 +456,24 @@ def test_prefix_attention_in_a_graph_with_changing_groups(H):
     for s, (want, _, vmax) in enumerate(c.attention(0, q, attn.sm_scale)[:6]):
         out_close(attn.out[s], want, vmax, False)
     assert (attn.out[6] == 3.0).all()
+
+
+def test_two_calls_at_once_on_two_streams(H):
+    """Handles of their own share no workspace: calls that run side by side give what each gives alone, bit for bit."""
+    import torch
+    cases = [prefix_case(H, "f16", 2, 64, 4, [5, 40], [400, 1600], [20, 3], seed=31), prefix_case(H, "e4m3", 4, 128, 2, [9, 1], [320, 64], [70], seed=32)]
+    alone = [attn.enqueue(0).clone() for _, _, attn, _ in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (_, _, attn, _), stream in zip(cases, streams):
+            with torch.cuda.stream(stream):
+                attn.out.fill_(float("nan"))
+            attn.enqueue(0, stream)
+    torch.cuda.synchronize()
+    for (_, _, attn, _), want in zip(cases, alone):
+        assert int(attn.status.item()) == 0
+        assert torch.equal(attn.out, want)
 
 
 def test_prefix_attention_negative_scale_and_equal_scores(H):
