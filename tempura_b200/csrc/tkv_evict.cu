@@ -4,15 +4,16 @@
 // Select.  Of a row of `len` tokens the first `protect`, the last `recent` and the best-scored others stay, together
 //     new_len = min(len, max(budget, protect + recent)),
 // ties to the lower index.  Scores become 32-bit keys that compare like the numbers (NaN below everything, -0 = +0); the key that
-// the last kept token has is found by histograms over 11, 11 and 10 bits of it, each over the tokens whose higher bits
-// agree with what is known; once these are few, a thread ranks each of them against all.  A last pass writes the indices in ascending order (ballots inside a warp, prefix sums across warps
-// and CTAs).  Scores are read once into shared memory; the bound is HBM for many rows and latency for few, so a row is split over a
-// thread-block cluster, whose CTAs add their histograms through distributed shared memory, where there are fewer rows than SMs.
+// the last kept token has is found by histograms over 11, 11 and 10 bits of it, each over the tokens whose higher bits agree with what is
+// known; once these are few, a thread ranks each of them against all.  A last pass writes the indices in ascending order (ballots inside a
+// warp, prefix sums across warps and CTAs).  Scores are read once into shared memory; the bound is instruction issue for many rows (4 096
+// rows of up to 4 096 tokens: 56 us for 52.6 MB, 45 million warp instructions) and latency for few (88 rows of 512: 6.1 us).  A long row
+// is split over a thread-block cluster, whose CTAs add their histograms through distributed shared memory.
 //
 // Compact.  Row j takes what row kept[j] >= j holds, in place.  A CTA owns one row set (layer, sequence, kv head, K or V) and
 // walks it in tiles: it reads all rows of a tile, waits, then stores them.  A row that a tile overwrites can only be the source of
 // rows at or before it, which are in this tile or an earlier one, so nothing is lost and no second buffer is needed.  Bound by HBM: a moved
-// row is read and written once.  Rows that stay are not touched, protected (shared) blocks among them.
+// row is read and written once (2.19 GB of F16 rows in 356 us, 6.15 TB/s; scaled E4M3 rows, re-encoded, 526 MB in 124 us, 4.2 TB/s: arithmetic).  Rows that stay are not touched, protected (shared) blocks among them.
 // A block of a scaled E4M3 pool has one scale: it becomes the largest of its new rows' scales.  Rows that had it keep their bytes; the others
 // are multiplied by scale / new scale <= 1 and rounded to E4M3 once more (half a step, 2^-4 relative, and flushed to zero below
 // 2^-6 as every writer of this pool does).  Taking the rows' absolute maximum instead would round every row again at every eviction.
@@ -442,9 +443,10 @@ int32_t tkv_evict_select_enqueue(const TkvEvictSelect* p, void* stream) {
     const uint32_t widest = std::max(p->budget < p->max_kv_len ? p->budget : 0u, p->recent < p->max_kv_len ? p->recent : 0u);
     if (widest > p->kept_stride)
         return fail(TKV_ERR_DIMENSION_MISMATCH, "dimension mismatch: expected %llu, got %llu (kept_stride below the budget)", widest, p->kept_stride);
-    // One CTA per row from two rows per SM on; below that a cluster per row, as long as a CTA still has 2 048 tokens of its own.
+    // One CTA per row up to 32 768 tokens, then the smallest cluster whose CTAs have no more (64 rows of 16 384 tokens: 17 us by one CTA each, 72 by
+    // clusters of four, whose barriers cost more than its CTAs save; 64 of 40 000: 33 by one CTA each, 27 by two, 47 by four).
     uint32_t cluster = 1;
-    while (cluster < MAX_CLUSTER && (rows * cluster < 296 ? p->max_kv_len / cluster > 2048 : p->max_kv_len / cluster > STAGE_TOKENS)) cluster *= 2;
+    while (cluster < MAX_CLUSTER && p->max_kv_len / cluster > 32768) cluster *= 2;
     if (rows * cluster > 0x7FFFFFFFull) return fail(TKV_ERR_INVALID_CONFIG, "%llu rows: batch too large", rows);
     if (p->new_lens == p->kv_lens) return fail(TKV_ERR_INVALID_CONFIG, "new_lens must not be kv_lens: every row reads the old length");
     const uint32_t slice = (p->max_kv_len + cluster - 1) / cluster;
@@ -468,7 +470,8 @@ int32_t tkv_evict_select_enqueue(const TkvEvictSelect* p, void* stream) {
     if (e == cudaSuccess && prev != p->device) e = cudaSetDevice(p->device);
     if (e == cudaSuccess) {
         const size_t smem = a.staged ? (size_t)slice * 4 : 0;
-        const bool large = slice > 8192;                        // 256 threads take short slices eight rows to an SM
+        // 256 threads take rows eight to an SM, 512 a row faster: 512 x 6 000 tokens 23 us and 27, but 64 x 8 192 20 us and 14, 512 x 16 384 92 and 46
+        const bool large = slice > 8192 || (rows <= 296 && slice > 1024);
         auto kernel = large ? evict_select<512> : evict_select<256>;
         if (smem > 32 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(STAGE_TOKENS * 4));
         if (e == cudaSuccess) {
