@@ -8,21 +8,24 @@
 // per group instead of once per sequence.  The tokens behind the prefix go through rows_attn, and a third kernel joins the partial
 // results (m, l, O) of both: out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.
 //
-// A CTA works on up to 256 rows of one (group, kv head) as two streams of 128 with their own S, P and O: with more than 128 rows
-// the streams are two row tiles that read the same cached tiles; with fewer they are the same rows on the two halves of every cached
-// tile (two partial results).  Up to 64 or 32 rows are there two or four times: the copies take the blocks of a step in turns, so
-// that a softmax warp, whose time per step is latency, has half or a quarter of it to do; P of the blocks that are not its own is 0.  A stream goes 64 cached tokens at a time through two S buffers: the scores of the next step are there when
-// the softmax of this one ends.  (One buffer of 128 tokens per stream left the softmax warps waiting for two products per tile:
-// 4 800 cycles per tile of both streams.)  A softmax thread owns a row: no exchange between threads.  P goes back to tensor memory, over
-// the S it was made from, as the A operand of the second product, so shared memory holds Q and the K and V tiles only.  The row maximum in use is raised, and O rescaled, only when a score exceeds it by 2^6.
+// A CTA works on up to 256 rows of one (group, kv head) as two streams of 128 with their own S, P and O that read the same cached tiles; with
+// up to 128 rows the second stream issues nothing.  (Letting both streams take the same rows on halves of every tile doubles the partial results:
+// 30 sequences on 2 048 tokens 38 us against 33, 16 on 8 192 45 against 36, 8 on 16 384 of an E4M3 pool 55 against 44; only with many tiles per
+// CTA it is ahead: 45 in 7 groups, E4M3, 86 against 91.)  A stream goes 64 cached tokens at a time through two S buffers: the scores of the next
+// step are there when the softmax of this one ends.  (One buffer of 128 tokens per stream left the softmax warps waiting for two products per
+// tile: 4 800 cycles per tile of both streams.)  A softmax thread owns a row: no exchange between threads.  P goes back to tensor memory, over
+// the S it was made from, as the A operand of the second product, so shared memory holds Q and the K and V tiles only.  The row maximum in use
+// is raised, and O rescaled, only when a score exceeds it by 2^6.
+// Measured: 128 sequences on 16 384 tokens, 64 query heads: 85 us of the call's 117, 0.49 of the measured bf16 rate.  A step of 64 tokens takes
+// both streams some 1 800 cycles, of which the products are 1 260 and the rest hand-offs between softmax and issuers.
 // An F16 pool's tiles arrive as tensor-map boxes, in the 128-byte swizzle the MMA reads.  An E4M3 pool's tiles are widened to F16
 // on the way by four warps (exact); K's block scale multiplies the scores, V's the probabilities, in units of a power of two above every
 // scale met so far.  Both operands of both products are then F16 and the products exact.  With up to 128 rows, where the tensor cores
-// wait for the cache, a probability is two F16 terms (22 bits); with more, where they are the bound, it is rounded to F16 once: 2^-11 of its
-// value at most, as much as the rounding of the output.
+// wait for the softmax, a probability is two F16 terms (22 bits: 0.21e-3 off 64 bits, what the rounding of the output alone gives, against
+// 0.32e-3 with one term); with more, where a second set of products would be on the bound, it is rounded to F16 once, 2^-11 of its value at most.
 //
 // Work split: the cached tiles of all (group, kv head, row block) items, one after another, in equal shares, one per CTA; a share may
-// begin and end inside an item.  The partial rows of item i and share c start at 8 * (rows before item i) + 512 * c, which keeps them
+// begin and end inside an item.  The partial rows of item i and share c start at (rows before item i) + 256 * c, which keeps them
 // apart because both only grow along the work.
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -52,7 +55,9 @@ constexpr uint32_t CTAS = 148;               // one per SM of the part this is b
 constexpr int BS = 16, KT = 128, ST = 64;    // tokens of a block, of a cached tile, of a step
 constexpr int GROUP_BYTES = 128 * 128;       // a [128 rows][128 B] swizzled column group of an operand tile
 constexpr float RAISE = 6.0f;
-constexpr uint32_t MIN_SHARE = 2;            // cached tiles
+// Cached tiles of a share: at least two where there are shares for more than half of the SMs, so that the kernel for the tokens behind the prefix
+// finds SMs beside this one (64 sequences on 2 048 tokens: 41 us with 2, 53 with 1), else one (3 on 48: 14 us, 18 with 2).
+__host__ __device__ __forceinline__ uint32_t min_share(uint64_t tiles) { return 2 * tiles > CTAS ? 2u : 1u; }
 
 struct Args {
     const uint32_t *tables, *kv_lens, *group_starts, *prefix_lens;
@@ -86,8 +91,6 @@ struct Item {
     uint32_t kvh, prefix, tile, n_tiles;          // tiles [tile, tile + n_tiles) of the prefix
     uint64_t out_row;                             // first partial row
 };
-// copies of the rows of a short row block
-__host__ __device__ __forceinline__ uint32_t copies_of(uint32_t block_rows) { return block_rows <= 32 ? 4u : block_rows <= 64 ? 2u : 1u; }
 __device__ __forceinline__ uint32_t row_blocks(uint32_t rows) { return (rows + 255) / 256; }
 
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) { mma<false>(d, a, b, idesc, acc); }
@@ -177,7 +180,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     cum[tid] = before + incl - mine;
     if (tid == THREADS - 1) cum[THREADS] = before + incl;
     __syncthreads();
-    const uint32_t total = cum[THREADS], share = max((total + a.parts - 1) / a.parts, MIN_SHARE);
+    const uint32_t total = cum[THREADS], share = max((total + a.parts - 1) / a.parts, min_share(total));
     if (blockIdx.x == 0) {
         uint32_t at = cum[tid];
         for (uint32_t i = 0; i < per; i++)
@@ -218,7 +221,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     }
     __syncthreads();                                            // Q goes where the sums were
     uint32_t tiles_done = 0;                                    // cached tiles of this CTA before the item at hand: places in the rings
-    uint32_t n_steps[2] = {0, 0};                               // steps of each stream before the item at hand: phases of its barriers
+    uint32_t n_steps = 0;                                       // steps of each stream before the item at hand: phases of its barriers
     uint32_t issued[2] = {0, 0};                                // F16 producer: tiles of K, of V asked for
     bool ok = true;
     for (uint32_t u = u_begin, item_no = 0; u < u_end; item_no++) {
@@ -234,9 +237,9 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             it.block_rows = min(256u, it.rows - it.row0);
             it.tile = (u - at) % nt;
             it.n_tiles = min(nt - it.tile, u_end - u);
-            it.out_row = 8ull * ((uint64_t)(it.first_seq - a.group_starts[0]) * a.group * a.n_kv_heads + (uint64_t)it.kvh * it.rows + it.row0) + 512ull * blockIdx.x;
+            it.out_row = (uint64_t)(it.first_seq - a.group_starts[0]) * a.group * a.n_kv_heads + (uint64_t)it.kvh * it.rows + it.row0 + 256ull * blockIdx.x;
         }
-        const bool same_rows = it.block_rows <= 128;            // both streams the same rows, on halves of the tiles
+        const bool few = it.block_rows <= 128;                  // nothing for the second stream
         const uint32_t* table = a.tables + (size_t)it.first_seq * a.table_stride;
         const uint32_t n_blocks = it.prefix / BS;
         auto blocks_in = [&](uint32_t i) { return min(8u, n_blocks - (it.tile + i) * 8u); };   // of the item's i-th tile
@@ -248,9 +251,9 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             // steps ahead of the second product. ----
             // Broadcast from one lane, what selects operands is known to be the warp's own: addresses then are computed once per warp.
             auto uni = [](uint32_t v) { return __shfl_sync(0xFFFFFFFFu, v, 0); };
-            const uint32_t x = uni(warp - (SM + FEED)), s_x = uni(x ? n_steps[1] : n_steps[0]), n_t = uni(it.n_tiles);
+            const uint32_t x = uni(warp - (SM + FEED)), s_x = uni(n_steps), n_t = uni(it.n_tiles);
             const uint32_t done = uni(tiles_done), n_left = uni(n_blocks - it.tile * 8u);
-            const bool same = uni(same_rows ? 1u : 0u) != 0;
+            const bool two = uni(few ? 1u : 0u) != 0, idle = two && x != 0;   // two terms per probability; a stream without rows
             auto blocks_at = [&](uint32_t i) { return min(8u, n_left - i * 8u); };
             const uint32_t q_lo = (smem_u32(q_tile) >> 4) + x * (TILE >> 4), k_lo = smem_u32(k_ring) >> 4, v_lo = smem_u32(v_ring) >> 4;
             const uint32_t ts = TM_S + x * 128, to = TM_O + x * 128;
@@ -259,68 +262,59 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             };
             if (elect_one()) {
             wait(c->q_ready + x, item_no);
-            // steps of this stream in tile i: both halves, or (same rows) half x if it holds a block
-            auto steps_at = [&](uint32_t i) { return same ? (blocks_at(i) > 4u * x ? 1u : 0u) : blocks_at(i) > 4u ? 2u : 1u; };
-            const uint32_t n_i = n_t - (steps_at(n_t - 1) == 0 ? 1u : 0u);   // tiles with a step
+            auto steps_at = [&](uint32_t i) { return blocks_at(i) > 4u ? 2u : 1u; };
             uint32_t iq = 0, hq = 0, nq = s_x;                   // tile, step in it and number of the next scores
             uint32_t ip = 0, hp = 0, np = s_x;                   // of the next product
-            while (ok && ip < n_i) {
+            while (ok && ip < n_t) {
                 // The scores run up to two steps ahead, but a tile that is not there yet holds up no product: that would hold up its V's place, too.
                 const uint32_t tq = done + iq, sq = tq & 1u;
-                bool ahead = iq < n_i && nq - np < 2;
+                bool ahead = iq < n_t && nq - np < 2;
                 if (ahead && hq == 0) {
                     if (np == nq) wait(c->k_full + sq, tq >> 1);
                     else ahead = mbar_test(c->k_full + sq, (tq >> 1) & 1u);
                 }
                 if (ahead) {
-                    const uint32_t b = nq & 1u, half = same ? x : hq;
+                    const uint32_t b = nq & 1u;
                     if (nq >= 2) wait(&c->pv_done[x][b], (nq >> 1) - 1u);  // the buffer is free when the product that read P over it is done
                     if (!ok) break;
                     tc_fence_after();
                     const bool last = hq + 1 == steps_at(iq);
-                    {
+                    if (!idle) {
 #pragma unroll
                         for (int ks = 0; ks < KSTEPS; ks++) {
                             const uint32_t off = (ks / 4) * (GROUP_BYTES >> 4) + (ks % 4) * 2;
-                            mma_ss(ts + b * ST, DESC_K | (q_lo + off), DESC_K | (k_lo + sq * (TILE >> 4) + half * (ST * 128u >> 4) + off), IDESC_QK, ks > 0 ? 1u : 0u);
+                            mma_ss(ts + b * ST, DESC_K | (q_lo + off), DESC_K | (k_lo + sq * (TILE >> 4) + hq * (ST * 128u >> 4) + off), IDESC_QK, ks > 0 ? 1u : 0u);
                         }
-                        tc_commit(&c->s_full[x][b]);
-                        if (last) tc_commit(c->k_empty + sq);              // a tile goes back when both streams have read it
                     }
+                    tc_commit(&c->s_full[x][b]);
+                    if (last) tc_commit(c->k_empty + sq);                  // a tile goes back when both streams have read it
                     nq++;
                     hq = last ? 0 : 1;
                     iq += last ? 1 : 0;
                 } else {
-                    const uint32_t t = done + ip, st = t & 1u, b = np & 1u, half = same ? x : hp, nb = min(4u, blocks_at(ip) - 4u * half);
+                    const uint32_t t = done + ip, st = t & 1u, b = np & 1u, nb = min(4u, blocks_at(ip) - 4u * hp);
                     wait(&c->p_full[x][b], np >> 1);
                     if (hp == 0) wait(c->v_full + st, t >> 1);
                     if (!ok) break;
                     tc_fence_after();
                     const bool last = hp + 1 == steps_at(ip);
-                    {
+                    if (!idle) {
+                        const uint64_t v_desc = DESC_V | (v_lo + st * (TILE >> 4) + 4 * hp * (2048u >> 4));
 #pragma unroll
                         for (uint32_t ks = 0; ks < 4; ks++)                // a block is one k-step: blocks behind the prefix are left out
-                            if (ks < nb) mma_ts(to, ts + b * ST + ks * 8, DESC_V | (v_lo + st * (TILE >> 4) + (4 * half + ks) * (2048u >> 4)), IDESC_PV,
-                                   (np > s_x || ks > 0) ? 1u : 0u);
-                        if (same) {                                        // the second terms of the probabilities
+                            if (ks < nb) mma_ts(to, ts + b * ST + ks * 8, v_desc + ks * (2048u >> 4), IDESC_PV, (np > s_x || ks > 0) ? 1u : 0u);
+                        if (two) {                                         // the second terms of the probabilities
 #pragma unroll
                             for (uint32_t ks = 0; ks < 4; ks++)
-                                if (ks < nb) mma_ts(to, ts + b * ST + 32 + ks * 8, DESC_V | (v_lo + st * (TILE >> 4) + (4 * half + ks) * (2048u >> 4)), IDESC_PV, 1u);
+                                if (ks < nb) mma_ts(to, ts + b * ST + 32 + ks * 8, v_desc + ks * (2048u >> 4), IDESC_PV, 1u);
                         }
-                        tc_commit(&c->pv_done[x][b]);
-                        if (last) tc_commit(c->v_empty + st);
                     }
+                    tc_commit(&c->pv_done[x][b]);
+                    if (last) tc_commit(c->v_empty + st);
                     np++;
                     hp = last ? 0 : 1;
                     ip += last ? 1 : 0;
                 }
-            }
-            if (ok && n_i < n_t) {                               // the last tile has nothing for this stream: it goes back unread, once it is there
-                const uint32_t t = done + n_i, st = t & 1u;
-                wait(c->k_full + st, t >> 1);
-                if (ok) mbar_arrive(c->k_empty + st);
-                wait(c->v_full + st, t >> 1);
-                if (ok) mbar_arrive(c->v_empty + st);
             }
             if (!ok) atomicCAS(&c->fail, 0u, 4u);
             }
@@ -447,10 +441,9 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
         } else {
             // ---- softmax: one row per thread ----
-            const uint32_t x = warp >> 2, s_x = x ? n_steps[1] : n_steps[0], r = (warp & 3u) * 32u + lane;
-            const uint32_t copies = same_rows ? copies_of(it.block_rows) : 1u, copy = r / (128u / copies), r_own = r % (128u / copies);   // copy: the warp's
-            const uint32_t row = it.row0 + (same_rows ? 0u : x * 128u) + r_own;    // of the group and kv head
-            const bool live = same_rows ? r_own < it.block_rows : x * 128u + r_own < it.block_rows;
+            const uint32_t x = warp >> 2, s_x = n_steps, r = (warp & 3u) * 32u + lane;
+            const uint32_t row = it.row0 + x * 128u + r;        // of the group and kv head
+            const bool live = x * 128u + r < it.block_rows;
             const bool warp_live = __any_sync(0xFFFFFFFFu, live);
             const uint32_t seq = it.first_seq + (live ? row / a.group : 0u), head = it.kvh * a.group + (live ? row % a.group : 0u);
             const uint32_t limit = live && min(a.kv_lens[seq], a.max_kv_len) >= it.prefix ? it.prefix : 0u;   // shorter members: rows_attn
@@ -474,8 +467,8 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             float m = -INFINITY, l = 0.0f, v_ref = FP8 ? 0x1p-100f : 1.0f, v_inv = FP8 ? 0x1p+100f : 1.0f;
             uint32_t n = s_x;                                   // steps of this stream so far
             for (uint32_t i = 0; i < it.n_tiles && ok; i++) {
-                const uint32_t slot = (tiles_done + i) & 3u, h_end = same_rows ? (blocks_in(i) > 4u * x ? x + 1 : x) : steps_in(i);
-                for (uint32_t h = same_rows ? x : 0u; h < h_end; h++, n++) {
+                const uint32_t slot = (tiles_done + i) & 3u, h_end = steps_in(i);
+                for (uint32_t h = 0; h < h_end; h++, n++) {
                     const uint32_t t0 = (it.tile + i) * KT + h * ST, b = n & 1u;
                     ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(&c->s_full[x][b]), (n >> 1) & 1u, fail));
                     if (!ok) break;
@@ -484,23 +477,20 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         const int left = (int)min(limit > t0 ? limit - t0 : 0u, (uint32_t)ST);   // tokens of the step that the row attends to
                         const uint32_t tb = ts + b * ST;
                         const float* sc = c->scales[slot] + 4 * h;
-                        auto step = [&](auto masked_type, auto copies_type) {
-                            constexpr bool MASKED = decltype(masked_type)::value, TWO = decltype(copies_type)::value > 0;
-                            constexpr int NB = 4 / (TWO ? decltype(copies_type)::value : 1);   // blocks of this warp: q0 ..
-                            const uint32_t q0 = TWO ? copy * NB : 0u;
-                            const float* sq = sc + q0;
-                            const int mine = left - (int)q0 * 16;
+                        auto step = [&](auto masked_type, auto two_type) {
+                            constexpr bool MASKED = decltype(masked_type)::value, TWO = decltype(two_type)::value;
+                            constexpr int NB = ST / BS;
                             uint32_t v[NB][16];
 #pragma unroll
-                            for (int q = 0; q < NB; q++) tmem_ld16(tb + (q0 + q) * 16, v[q]);
+                            for (int q = 0; q < NB; q++) tmem_ld16(tb + q * 16, v[q]);
                             tmem_wait_ld();
                             float mx = -INFINITY;               // neither scale is negative: the maximum commutes with them
 #pragma unroll
                             for (int q = 0; q < NB; q++) {      // a block
                                 float top = -INFINITY;
 #pragma unroll
-                                for (int k = 0; k < 16; k++) top = fmaxf(top, MASKED && q * 16 + k >= mine ? -INFINITY : __uint_as_float(v[q][k]));
-                                mx = FP8 ? fmaxf(mx, top == -INFINITY ? top : top * sq[q]) : fmaxf(mx, top);
+                                for (int k = 0; k < 16; k++) top = fmaxf(top, MASKED && q * 16 + k >= left ? -INFINITY : __uint_as_float(v[q][k]));
+                                mx = FP8 ? fmaxf(mx, top == -INFINITY ? top : top * sc[q]) : fmaxf(mx, top);
                             }
                             mx = mx == -INFINITY ? mx : mx * a.scale_log2;
                             // ---- a raised maximum or V scale rescales the row of O, once the product of the step before is done ----
@@ -511,10 +501,10 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                                 l *= factor;
                             }
                             if (FP8) {
-                                float top = sq[8];
+                                float top = sc[8];
 #pragma unroll
-                                for (int q = 1; q < NB; q++) top = fmaxf(top, sq[8 + q]);
-                                if (top > v_ref) {              // the same in every thread of the warp
+                                for (int q = 1; q < NB; q++) top = fmaxf(top, sc[8 + q]);
+                                if (top > v_ref) {              // the same in every thread
                                     const float up = __uint_as_float(min((__float_as_uint(top) >> 23) + 1u, 253u) << 23);
                                     factor *= v_ref / up;
                                     v_ref = up;
@@ -540,15 +530,15 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                             float sum = 0.0f;
 #pragma unroll
                             for (int q = 0; q < NB; q++) {
-                                const float ks = FP8 ? a.scale_log2 * sq[q] : a.scale_log2, vn = FP8 ? sq[8 + q] * v_inv : 1.0f;
+                                const float ks = FP8 ? a.scale_log2 * sc[q] : a.scale_log2, vn = FP8 ? sc[8 + q] * v_inv : 1.0f;
                                 uint32_t first[8], second[8];
 #pragma unroll
                                 for (int k = 0; k < 16; k += 2) {
                                     float p0 = fast_exp2(__fmaf_rn(__uint_as_float(v[q][k]), ks, sub));
                                     float p1 = fast_exp2(__fmaf_rn(__uint_as_float(v[q][k + 1]), ks, sub));
                                     if (MASKED) {
-                                        p0 = q * 16 + k < mine ? p0 : 0.0f;
-                                        p1 = q * 16 + k + 1 < mine ? p1 : 0.0f;
+                                        p0 = q * 16 + k < left ? p0 : 0.0f;
+                                        p1 = q * 16 + k + 1 < left ? p1 : 0.0f;
                                     }
                                     sum += p0 + p1;
                                     if (FP8) {
@@ -563,30 +553,20 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                                         second[k / 2] = *reinterpret_cast<const uint32_t*>(&lp);
                                     }
                                 }
-                                tmem_st8(tb + (q0 + q) * 8, first);
-                                if (TWO) tmem_st8(tb + 32 + (q0 + q) * 8, second);
-                            }
-                            if (NB < 4) {                       // the other copies' blocks
-                                const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-                                for (uint32_t q = 0; q < 4; q++)
-                                    if (q / NB != copy) {
-                                        tmem_st8(tb + q * 8, zero);
-                                        tmem_st8(tb + 32 + q * 8, zero);
-                                    }
+                                tmem_st8(tb + q * 8, first);
+                                if (TWO) tmem_st8(tb + 32 + q * 8, second);
                             }
                             tmem_wait_st();
                             l += sum;
                         };
                         const bool masked = __any_sync(0xFFFFFFFFu, left < ST);
-                        auto dispatch = [&](auto copies_type) {
-                            if (masked) step(std::true_type{}, copies_type);
-                            else step(std::false_type{}, copies_type);
-                        };
-                        if (!same_rows) dispatch(std::integral_constant<int, 0>{});
-                        else if (copies == 4) dispatch(std::integral_constant<int, 4>{});
-                        else if (copies == 2) dispatch(std::integral_constant<int, 2>{});
-                        else dispatch(std::integral_constant<int, 1>{});
+                        if (few) {
+                            if (masked) step(std::true_type{}, std::true_type{});
+                            else step(std::false_type{}, std::true_type{});
+                        } else {
+                            if (masked) step(std::true_type{}, std::false_type{});
+                            else step(std::false_type{}, std::false_type{});
+                        }
                         tc_fence_before();
                     }
                     __syncwarp();
@@ -595,7 +575,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
             // ---- partial result of the row ----
             const bool any = n > s_x;
-            const uint64_t dst = it.out_row + (same_rows ? (x * copies + copy) * it.block_rows + r_own : x * 128u + r);
+            const uint64_t dst = it.out_row + x * 128u + r;
             if (ok && any) ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(&c->pv_done[x][(n - 1) & 1u]), ((n - 1) >> 1) & 1u, fail));
             if (ok && warp_live) {
                 tc_fence_after();
@@ -639,8 +619,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         __syncthreads();
         tiles_done += it.n_tiles;
         const uint32_t cut = 2 - steps_in(it.n_tiles - 1);      // only a prefix's last tile may hold one half
-        n_steps[0] += same_rows ? it.n_tiles : 2 * it.n_tiles - cut;
-        n_steps[1] += same_rows ? it.n_tiles - cut : 2 * it.n_tiles - cut;
+        n_steps += 2 * it.n_tiles - cut;
         u += it.n_tiles;
     }
     if (warp >= SM + FEED && lane == 0) {                       // whatever ended the loop, no product is under way when tensor memory is given back
@@ -661,11 +640,11 @@ struct JoinArgs {
     const float *pre_o, *pre_ml, *own_o, *own_ml;   // partial results over the prefixes, over the tokens behind them
     const uint32_t *pre_plan, *own_plan, *kv_lens, *group_starts, *prefix_lens;
     __half* out;
-    uint32_t n_seqs, n_groups, n_q_heads, n_kv_heads, group, subs;
+    uint32_t n_seqs, n_groups, n_q_heads, n_kv_heads, group;
 };
 
 // WPR warps join the partial results of one (sequence, query head): one where there are rows enough to fill the machine, eight where
-// few rows have many parts.  Bound by latency and L2.
+// few rows have many parts (960 rows: 38 us for the whole call with eight, 42 with one; 8 192 rows: 136 and 117).  Bound by latency and L2.
 template <int D, int WPR> __global__ void __launch_bounds__(256) prefix_join(const JoinArgs a) {
     // what the caller wrote is read while the kernels before this one still run
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
@@ -679,21 +658,20 @@ template <int D, int WPR> __global__ void __launch_bounds__(256) prefix_join(con
     if (!in || share_t == 0 || share_b == 0 || g == a.n_groups) return;   // (all warps of a row alike) refused, or a row behind the last sequence
     // parts of the prefix
     const uint32_t rows = (s1 - s0) * a.group, kvh = head / a.group, r = (s - s0) * a.group + head % a.group;
-    const uint32_t rb = r / 256, block_rows = min(256u, rows - rb * 256), nt = (prefix + KT - 1) / KT;
-    const bool same_rows = block_rows <= 128;
-    const uint32_t t0 = tiles_before + (kvh * row_blocks(rows) + rb) * nt, c0 = nt ? t0 / share_t : 0u, k = same_rows ? 2u * copies_of(block_rows) : 1u;
-    const uint32_t n_pre = nt ? ((t0 + nt - 1) / share_t - c0 + 1) * k : 0u;
-    const uint64_t first = 8ull * ((uint64_t)(s0 - base) * a.group * a.n_kv_heads + (uint64_t)kvh * rows + rb * 256) + 512ull * c0 + r % 256;
+    const uint32_t rb = r / 256, nt = (prefix + KT - 1) / KT;
+    const uint32_t t0 = tiles_before + (kvh * row_blocks(rows) + rb) * nt, c0 = nt ? t0 / share_t : 0u;
+    const uint32_t n_pre = nt ? (t0 + nt - 1) / share_t - c0 + 1 : 0u;
+    const uint64_t first = (uint64_t)(s0 - base) * a.group * a.n_kv_heads + (uint64_t)kvh * rows + r + 256ull * c0;
     // parts of the tokens behind it
     const uint32_t p0 = hi > lo ? lo / share_b : 0u;
-    const uint32_t n_own = hi > lo ? ((hi - 1) / share_b - p0 + 1) * a.subs : 0u, n = n_pre + n_own;
+    const uint32_t n_own = hi > lo ? (hi - 1) / share_b - p0 + 1 : 0u, n = n_pre + n_own;
     auto part = [&](uint32_t i, const float*& o, const float*& ml) {
         if (i < n_pre) {
-            const uint64_t at = first + (i / k) * 512ull + (i % k) * block_rows;
+            const uint64_t at = first + i * 256ull;
             o = a.pre_o + at * D;
             ml = a.pre_ml + at * 2;
         } else {
-            const uint64_t at = ((uint64_t)(p0 + s) * a.subs + (i - n_pre)) * a.n_q_heads + head;
+            const uint64_t at = ((uint64_t)(p0 + s) + (i - n_pre)) * a.n_q_heads + head;
             o = a.own_o + at * D;
             ml = a.own_ml + at * 2;
         }
@@ -789,9 +767,9 @@ Layout layout_of(uint32_t n_seqs, uint32_t n_groups, uint32_t n_q_heads, uint32_
     Layout l;
     const uint64_t group = n_q_heads / n_kv_heads, nt = (max_prefix_len + KT - 1ull) / KT;
     const uint64_t tiles = (n_groups + (uint64_t)n_seqs * group / 256) * n_kv_heads * nt;      // at most: every group ends in a row block of its own
-    l.parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(CTAS, (tiles + MIN_SHARE - 1) / MIN_SHARE));
+    l.parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(CTAS, tiles));
     l.own = tkv_rows::split_for((uint64_t)n_seqs * ((max_kv_len + 15ull) / 16), n_kv_heads, CTAS);
-    const uint64_t rows = 8ull * n_seqs * n_q_heads + 512ull * l.parts, slots = ((uint64_t)l.own.parts + n_seqs) * 2;   // two results per slot of an E4M3 pool
+    const uint64_t rows = (uint64_t)n_seqs * n_q_heads + 256ull * l.parts, slots = (uint64_t)l.own.parts + n_seqs;
     l.pre_ml = up(4ull * (n_groups + 2ull), 256);
     l.pre_o = l.pre_ml + up(rows * 8, 256);
     l.own_plan = l.pre_o + up(rows * head_dim * 4, 256);
@@ -957,7 +935,6 @@ int32_t tkv_prefix_attn_enqueue(const TkvPool* pool, const TkvPrefixAttn* p, voi
     j.n_q_heads = a.n_q_heads;
     j.n_kv_heads = a.n_kv_heads;
     j.group = a.group;
-    j.subs = tkv_rows::subs_of(fp8, false);
 
     CUtensorMap mk{}, mv{};
     if (!fp8 && (!make_map(&mk, kp, pool->total_blocks, pool->n_kv_heads, pool->head_dim) || !make_map(&mv, vp, pool->total_blocks, pool->n_kv_heads, pool->head_dim)))

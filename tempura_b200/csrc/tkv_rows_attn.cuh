@@ -21,13 +21,12 @@
 // rides in the four spare columns of the same MMAs, else it is a second set of them.
 //
 // A block costs a consumer a chain of dependent steps (wait, fragments, eight MMAs, exp2, transposes, eight MMAs).  For an F16 block the
-// chain is shorter than the time in which HBM delivers the block; for an E4M3 block, with half the bytes and a conversion in the
-// chain, it is longer, so two consumers take its blocks in turns, each with its own partial result (F32 operands need the registers
-// of both).  Stages then come in pairs: a stage always belongs to the same consumer, whose wait for a barrier's phase would otherwise
-// be answered by the phase before the one that its partner waits for.
+// chain is shorter than the time in which HBM delivers the block (131 071 tokens of 8 heads: 97 us, 5.6 TB/s); for an E4M3 block, with half
+// the bytes and a conversion in the chain, it is the bound (64 sequences of up to 4 096 tokens: 56 us, 4.8 TB/s).  Two consumers per head on
+// alternate blocks did not help: the same 71 us for the whole call, and 91 against 75 us for one context of 131 071 tokens.
 //
 // Work split: the batch's blocks, sequence after sequence, are cut into `parts` equal shares that may span sequences; part p and
-// sequence s meet in partial slot p + s (subs_of results each), which is unique because both only grow along the batch.
+// sequence s meet in partial slot p + s, which is unique because both only grow along the batch.
 #pragma once
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -40,9 +39,7 @@ namespace tkv_rows {
 
 constexpr int BS = 16;                       // tokens per block
 constexpr int WARPS = 8;                     // consumer warps of a share of the blocks
-// consumers of a kv head, on alternate blocks: partial results per slot
-__host__ __device__ constexpr int subs_of(bool fp8, bool f32) { return fp8 && !f32 ? 2 : 1; }
-__host__ __device__ constexpr int threads_of(bool fp8, bool f32) { return (WARPS * subs_of(fp8, f32) + 1) * 32; }   // and the producer
+constexpr int THREADS = (WARPS + 1) * 32;    // and the producer
 constexpr int MAX_STAGES = 8;
 constexpr uint32_t PAD = 32;                 // bytes between runs of four tokens
 constexpr uint32_t SCALE_BYTES = 2 * WARPS * 4;
@@ -56,7 +53,7 @@ struct Args {
     const void* q;                           // f16 or f32 [n_seqs][n_q_heads][D]
     const uint32_t *tables, *kv_lens;
     const uint32_t *group_starts, *prefix_lens;   // shared-prefix groups, or null: ranges begin at token 0
-    float *part_o, *part_ml;                 // [slot][sub][n_q_heads][D], [slot][sub][n_q_heads][2]
+    float *part_o, *part_ml;                 // [slot][n_q_heads][D], [slot][n_q_heads][2]
     float* logits;                           // [n_seqs][n_q_heads][logit_stride], or null
     uint32_t* plan;                          // [0] blocks per part, [1 + s] blocks before sequence s (n_seqs + 1 entries)
     uint32_t* status;
@@ -178,9 +175,9 @@ struct Cursor {
 // F32: q and out are F32 and q is used as two F16 terms (22 bits); else both are F16.
 // WIDE: more than four query heads per kv head (the second term of the probabilities then takes MMAs of its own).
 template <int D, bool FP8, bool F32, bool WIDE>
-__global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args a) {
+__global__ void __launch_bounds__(THREADS, 1) rows_attn(const Args a) {
     using S = Shape<D, FP8>;
-    constexpr int THREADS = threads_of(FP8, F32), NWARPS = THREADS / 32;
+    constexpr int NWARPS = THREADS / 32;
     constexpr int KS = S::KS, MT = S::MT;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     extern __shared__ __align__(128) unsigned char ring[];
@@ -395,9 +392,8 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
         return;
     }
 
-    // ---- consumer: one kv head of one stream, every block or every second one ----
-    constexpr uint32_t STEP = subs_of(FP8, F32);
-    const uint32_t sub = warp / WARPS, x_stream = (warp % WARPS) / a.heads, h = (warp % WARPS) % a.heads, stream = blockIdx.x * a.streams + x_stream;
+    // ---- consumer: one kv head of one stream ----
+    const uint32_t x_stream = warp / a.heads, h = warp % a.heads, stream = blockIdx.x * a.streams + x_stream;
     const uint32_t part = stream / a.head_groups, kvh = (stream % a.head_groups) * a.heads + h;
     if (x_stream >= a.streams || kvh >= a.n_kv_heads) return;
     const uint32_t n_mine = part_blocks(part);
@@ -408,8 +404,7 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
     const uint32_t tok_v0 = 4 * j, tok_v1 = 4 * (j ^ 2u) + 1;   // of k indices 2j, 2j + 1; of 2j + 8, 2j + 9: two more
 
     const bool scaled = FP8 && a.k_scales != nullptr;
-    uint32_t slot = sub, phase = 0;                             // ring stage of this consumer's next block
-    uint32_t turn = sub;                                        // blocks until it, counted from c.block
+    uint32_t slot = 0, phase = 0;                               // ring stage of the next block
     const uint32_t ring_base = smem_addr(ring) + x_stream * a.stages * stage_bytes;
     const uint32_t k_off = ring_base + h * S::ROW + run_k * run_smem + (grp & 1u) * row_smem + j * 16, half = 2 * row_smem;
     const uint32_t v_off = ring_base + plane + h * S::ROW + grp * S::VPB;
@@ -448,7 +443,7 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
                                                                 // it, and P x scale / v_ref stays in F16's range
         float* lg = a.logits ? a.logits + ((size_t)c.seq * a.n_q_heads + kvh * a.group + 2 * j) * a.logit_stride + c.block * BS + tok_k : nullptr;
         const uint32_t n = c.left;
-        for (; turn < n; turn += STEP) {
+        for (uint32_t turn = 0; turn < n; turn++) {
             if (!bar_wait(smem_addr(&full[x_stream][slot]), phase, &fail)) {
                 if (lane == 0) {
                     atomicCAS(&fail, 0u, 4u);
@@ -602,16 +597,14 @@ __global__ void __launch_bounds__(threads_of(FP8, F32), 1) rows_attn(const Args 
             }
             __syncwarp();                                       // every lane's reads of the stage are done
             if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&empty[x_stream][slot])) : "memory");
-            slot += STEP;
-            if (slot >= a.stages) {
-                slot -= a.stages;
+            if (++slot == a.stages) {
+                slot = 0;
                 phase ^= 1u;
             }
         }
-        turn -= n;
 
-        // ---- partial results of (part, sequence); a consumer that had no block says so with an empty sum ----
-        const size_t at_slot = ((size_t)part + c.seq) * STEP + sub;
+        // ---- partial results of (part, sequence) ----
+        const size_t at_slot = (size_t)part + c.seq;
         if (!WIDE) {                                            // first and second terms of a head together
 #pragma unroll
             for (int t = 0; t < MT; t++)
@@ -648,8 +641,9 @@ struct Split {
     uint32_t parts, min_share, grid;
 };
 // Streams of at most eight kv heads, as even as they come; parts for a batch of at most `blocks` cached blocks: one CTA per SM, and no
-// part shorter than MIN_SHARE blocks (a part costs the joining kernel a partial result per query head).
-constexpr uint32_t MIN_SHARE = 4;
+// part shorter than MIN_SHARE blocks (a part costs the joining kernel a partial result per query head; scored attention of one sequence of 200 tokens:
+// 12.3 us with 2, 14.3 with 4, 16.4 with 8, and no difference for batches that fill the machine).
+constexpr uint32_t MIN_SHARE = 2;
 inline Split split_for(uint64_t blocks, uint32_t n_kv_heads, uint32_t ctas) {
     Split s;
     s.head_groups = (n_kv_heads + WARPS - 1) / WARPS;
@@ -672,8 +666,7 @@ template <int D, bool FP8, bool F32, bool WIDE> cudaError_t launch_one(Args a, c
     a.parts = sp.parts;
     a.min_share = sp.min_share;
     const uint32_t stage = 2 * (BS * sp.heads * S::ROW + 4 * PAD) + (FP8 ? SCALE_BYTES : 0), fit = RING_BYTES / (sp.streams * stage);
-    a.stages = (fit < (uint32_t)MAX_STAGES ? fit : (uint32_t)MAX_STAGES) / subs_of(FP8, F32) * subs_of(FP8, F32);   // at least 3 (eight heads of 128
-                                                                                                    // F16 dims: 65 KB each), in pairs for pairs
+    a.stages = fit < (uint32_t)MAX_STAGES ? fit : (uint32_t)MAX_STAGES;   // at least 3 (eight heads of 128 F16 dims: 65 KB each)
     const size_t smem = (size_t)sp.streams * a.stages * stage;
     auto kernel = rows_attn<D, FP8, F32, WIDE>;
     static std::atomic<uint64_t> granted{0};                    // devices on which this kernel may use the ring's shared memory
@@ -688,7 +681,7 @@ template <int D, bool FP8, bool F32, bool WIDE> cudaError_t launch_one(Args a, c
     }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(sp.grid);
-    cfg.blockDim = dim3(threads_of(FP8, F32));
+    cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute at[1];

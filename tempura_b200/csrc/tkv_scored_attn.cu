@@ -33,15 +33,15 @@ struct FinishArgs {
     const uint32_t *plan, *kv_lens;
     float* scores;
     void* out;
-    uint32_t n_seqs, n_q_heads, n_kv_heads, group, logit_stride, score_stride, max_kv_len, tasks, subs, v4;
+    uint32_t n_seqs, n_q_heads, n_kv_heads, group, logit_stride, score_stride, max_kv_len, tasks, v4;
     float decay;
 };
 
-// Tokens per thread of the second kernel: their scores of all G query heads wait in registers.
+// Tokens per thread of the second kernel: their scores of all G query heads wait in registers (16 sequences of up to 4 096 tokens: 2 with
+// eight query heads 47 us for the whole call, 4 49 us; with four query heads 42.6 and 42.3).
 __host__ __device__ constexpr int tokens_of(int g) { return g > 4 ? 2 : 4; }
 
-// One CTA per (sequence, kv head, task): the first G tasks join the partial results of one query head each (the first one those of all
-// heads, a warp each, when they are few), the others turn the scores of 256 x TOK tokens into weights.  Bound by latency and L2:
+// One CTA per (sequence, kv head, task): the first G tasks join the partial results of one query head each, the others turn the scores of 256 x TOK tokens into weights.  Bound by latency and L2:
 // everything it reads was written just before, so a thread asks for its scores before it joins the maxima and sums, and asks
 // for all of those at once.  V: rows of scores are aligned to a thread's tokens.
 template <int D, bool F32, int G> __global__ void __launch_bounds__(256) scored_finish(const FinishArgs a) {
@@ -77,12 +77,10 @@ template <int D, bool F32, int G> __global__ void __launch_bounds__(256) scored_
     float x[G][TOK];
     if (!join) read(x, t0);
     if (!join && t0 >= len) return;
-    const uint32_t p0 = hi > lo ? lo / share : 0u, n = hi > lo ? ((hi - 1) / share - p0 + 1) * a.subs : 0u;
-    const size_t first = (size_t)(p0 + s) * a.subs;             // partial results first .. first + n - 1
-    const bool few = n <= 16;
-    if (join && few && task) return;
+    const uint32_t p0 = hi > lo ? lo / share : 0u, n = hi > lo ? ((hi - 1) / share - p0 + 1) : 0u;
+    const size_t first = p0 + s;                               // partial results first .. first + n - 1
     __shared__ float top[8], inv[8];
-    if (warp < (uint32_t)G && (!join || few || warp == task)) { // warp g: maximum and sum of query head g
+    if (warp < (uint32_t)G && (!join || warp == task)) { // warp g: maximum and sum of query head g
         float m = -INFINITY, l = 0.0f;
         const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + first * a.n_q_heads + kvh * G + warp;
         for (uint32_t i0 = 0; i0 < n; i0 += 256) {
@@ -117,12 +115,10 @@ template <int D, bool F32, int G> __global__ void __launch_bounds__(256) scored_
         float acc[PER];
 #pragma unroll
         for (int i = 0; i < PER; i++) acc[i] = 0.0f;
-        const uint32_t head = few ? warp : task;
-        if (head >= (uint32_t)G) return;
+        const uint32_t head = task;
         const float m = top[head];
-        const uint32_t step = few ? 1u : 8u;
 #pragma unroll 8
-        for (uint32_t i = few ? 0u : warp; i < n; i += step) {
+        for (uint32_t i = warp; i < n; i += 8) {
             const size_t r = (first + i) * a.n_q_heads + kvh * G + head;
             const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + r * 2);
             float v[PER];
@@ -133,15 +129,6 @@ template <int D, bool F32, int G> __global__ void __launch_bounds__(256) scored_
             for (int k = 0; k < PER; k++) acc[k] = ml.x != -INFINITY || ml.y != 0.0f ? __fmaf_rn(f, v[k], acc[k]) : acc[k];   // an empty part's O counts for nothing
         }
         const size_t at = ((size_t)s * a.n_q_heads + kvh * G + head) * D;
-        if (few) {
-#pragma unroll
-            for (int k = 0; k < PER; k++) {
-                const float v = acc[k] * inv[head];
-                if (F32) reinterpret_cast<float*>(a.out)[at + k * 32 + lane] = v;
-                else reinterpret_cast<__half*>(a.out)[at + k * 32 + lane] = __float2half_rn(v);
-            }
-            return;
-        }
         __shared__ float part[8][D];
 #pragma unroll
         for (int k = 0; k < PER; k++) part[warp][k * 32 + lane] = acc[k];
@@ -333,7 +320,6 @@ int32_t tkv_scored_attn_enqueue(const TkvPool* pool, const TkvScoredAttn* p, voi
     f.max_kv_len = p->max_kv_len;
     f.tasks = tasks;
     f.v4 = p->scores % 16 == 0 && p->score_stride % 4 == 0;
-    f.subs = tkv_rows::subs_of(es == 1, p->q_dtype == TKV_DTYPE_F32);
     f.decay = p->decay;
 
     int prev = -1;
