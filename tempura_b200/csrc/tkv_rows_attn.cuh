@@ -21,7 +21,7 @@
 // rides in the four spare columns of the same MMAs, else it is a second set of them.
 //
 // A block costs a consumer a chain of dependent steps (wait, fragments, eight MMAs, exp2, transposes, eight MMAs).  For an F16 block the
-// chain is shorter than the time in which HBM delivers the block (131 071 tokens of 8 heads: 97 us, 5.6 TB/s); for an E4M3 block, with half
+// chain is shorter than the time in which HBM delivers the block (131 071 tokens of 8 heads: 92 us, 5.9 TB/s); for an E4M3 block, with half
 // the bytes and a conversion in the chain, it is the bound (64 sequences of up to 4 096 tokens: 56 us, 4.8 TB/s).  Two consumers per head on
 // alternate blocks did not help: the same 71 us for the whole call, and 91 against 75 us for one context of 131 071 tokens.
 //
