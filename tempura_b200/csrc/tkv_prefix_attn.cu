@@ -16,13 +16,14 @@
 // tile: 4 800 cycles per tile of both streams.)  A softmax thread owns a row: no exchange between threads.  P goes back to tensor memory, over
 // the S it was made from, as the A operand of the second product, so shared memory holds Q and the K and V tiles only.  The row maximum in use
 // is raised, and O rescaled, only when a score exceeds it by 2^6.
-// Measured: 128 sequences on 16 384 tokens, 64 query heads: 85 us of the call's 117, 0.49 of the measured bf16 rate.  A step of 64 tokens takes
-// both streams some 1 800 cycles, of which the products are 1 260 and the rest hand-offs between softmax and issuers.
+// Measured: 128 sequences on 16 384 tokens, 64 query heads: 131 us for the call, 529 TFLOP/s of useful products (0.32 of the measured bf16 rate; with
+// the second terms counted 0.48).  A step of 64 tokens takes both streams some 2 200 cycles, of which the products are 1 790 (N = 64 from shared
+// memory 48 cycles each, with A in tensor memory 64) and the rest hand-offs between softmax and issuers.
 // An F16 pool's tiles arrive as tensor-map boxes, in the 128-byte swizzle the MMA reads.  An E4M3 pool's tiles are widened to F16
 // on the way by four warps (exact); K's block scale multiplies the scores, V's the probabilities, in units of a power of two above every
-// scale met so far.  Both operands of both products are then F16 and the products exact.  With up to 128 rows, where the tensor cores
-// wait for the softmax, a probability is two F16 terms (22 bits: 0.21e-3 off 64 bits, what the rounding of the output alone gives, against
-// 0.32e-3 with one term); with more, where a second set of products would be on the bound, it is rounded to F16 once, 2^-11 of its value at most.
+// scale met so far.  Both operands of both products are then F16 and the products exact.  A probability is
+// two F16 terms (22 bits), the second with products of its own: 0.21e-3 off 64 bits, which is the rounding of the output alone, against 0.29e-3
+// with one term.  That costs 118 -> 131 us on the largest case below and nothing where the products are not the bound.
 //
 // Work split: the cached tiles of all (group, kv head, row block) items, one after another, in equal shares, one per CTA; a share may
 // begin and end inside an item.  The partial rows of item i and share c start at (rows before item i) + 256 * c, which keeps them
@@ -253,7 +254,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             auto uni = [](uint32_t v) { return __shfl_sync(0xFFFFFFFFu, v, 0); };
             const uint32_t x = uni(warp - (SM + FEED)), s_x = uni(n_steps), n_t = uni(it.n_tiles);
             const uint32_t done = uni(tiles_done), n_left = uni(n_blocks - it.tile * 8u);
-            const bool two = uni(few ? 1u : 0u) != 0, idle = two && x != 0;   // two terms per probability; a stream without rows
+            const bool idle = uni(few ? 1u : 0u) != 0 && x != 0;   // a stream without rows
             auto blocks_at = [&](uint32_t i) { return min(8u, n_left - i * 8u); };
             const uint32_t q_lo = (smem_u32(q_tile) >> 4) + x * (TILE >> 4), k_lo = smem_u32(k_ring) >> 4, v_lo = smem_u32(v_ring) >> 4;
             const uint32_t ts = TM_S + x * 128, to = TM_O + x * 128;
@@ -303,11 +304,9 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
 #pragma unroll
                         for (uint32_t ks = 0; ks < 4; ks++)                // a block is one k-step: blocks behind the prefix are left out
                             if (ks < nb) mma_ts(to, ts + b * ST + ks * 8, v_desc + ks * (2048u >> 4), IDESC_PV, (np > s_x || ks > 0) ? 1u : 0u);
-                        if (two) {                                         // the second terms of the probabilities
 #pragma unroll
-                            for (uint32_t ks = 0; ks < 4; ks++)
-                                if (ks < nb) mma_ts(to, ts + b * ST + 32 + ks * 8, v_desc + ks * (2048u >> 4), IDESC_PV, 1u);
-                        }
+                        for (uint32_t ks = 0; ks < 4; ks++)                // the second terms of the probabilities
+                            if (ks < nb) mma_ts(to, ts + b * ST + 32 + ks * 8, v_desc + ks * (2048u >> 4), IDESC_PV, 1u);
                     }
                     tc_commit(&c->pv_done[x][b]);
                     if (last) tc_commit(c->v_empty + st);
@@ -477,8 +476,8 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         const int left = (int)min(limit > t0 ? limit - t0 : 0u, (uint32_t)ST);   // tokens of the step that the row attends to
                         const uint32_t tb = ts + b * ST;
                         const float* sc = c->scales[slot] + 4 * h;
-                        auto step = [&](auto masked_type, auto two_type) {
-                            constexpr bool MASKED = decltype(masked_type)::value, TWO = decltype(two_type)::value;
+                        auto step = [&](auto masked_type) {
+                            constexpr bool MASKED = decltype(masked_type)::value;
                             constexpr int NB = ST / BS;
                             uint32_t v[NB][16];
 #pragma unroll
@@ -547,26 +546,19 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                                     }
                                     const __half2 hp = __floats2half2_rn(p0, p1);
                                     first[k / 2] = *reinterpret_cast<const uint32_t*>(&hp);
-                                    if (TWO) {
-                                        const float2 fp = __half22float2(hp);
-                                        const __half2 lp = __floats2half2_rn(p0 - fp.x, p1 - fp.y);
-                                        second[k / 2] = *reinterpret_cast<const uint32_t*>(&lp);
-                                    }
+                                    const float2 fp = __half22float2(hp);
+                                    const __half2 lp = __floats2half2_rn(p0 - fp.x, p1 - fp.y);
+                                    second[k / 2] = *reinterpret_cast<const uint32_t*>(&lp);
                                 }
                                 tmem_st8(tb + q * 8, first);
-                                if (TWO) tmem_st8(tb + 32 + q * 8, second);
+                                tmem_st8(tb + 32 + q * 8, second);
                             }
                             tmem_wait_st();
                             l += sum;
                         };
                         const bool masked = __any_sync(0xFFFFFFFFu, left < ST);
-                        if (few) {
-                            if (masked) step(std::true_type{}, std::true_type{});
-                            else step(std::false_type{}, std::true_type{});
-                        } else {
-                            if (masked) step(std::true_type{}, std::false_type{});
-                            else step(std::false_type{}, std::false_type{});
-                        }
+                        if (masked) step(std::true_type{});
+                        else step(std::false_type{});
                         tc_fence_before();
                     }
                     __syncwarp();
