@@ -17,13 +17,13 @@
 // the S it was made from, as the A operand of the second product, so shared memory holds Q and the K and V tiles only.  The row maximum in use
 // is raised, and O rescaled, only when a score exceeds it by 2^6.
 // Measured: 128 sequences on 16 384 tokens, 64 query heads: 131 us for the call, 529 TFLOP/s of useful products (0.32 of the measured bf16 rate; with
-// the second terms counted 0.48).  A step of 64 tokens takes both streams some 2 200 cycles, of which the products are 1 790 (N = 64 from shared
+// the second terms counted 0.48).  A step of 64 tokens takes both streams some 2 100 cycles, of which the products are 1 790 (N = 64 from shared
 // memory 48 cycles each, with A in tensor memory 64) and the rest hand-offs between softmax and issuers.
 // An F16 pool's tiles arrive as tensor-map boxes, in the 128-byte swizzle the MMA reads.  An E4M3 pool's tiles are widened to F16
 // on the way by four warps (exact); K's block scale multiplies the scores, V's the probabilities, in units of a power of two above every
 // scale met so far.  Both operands of both products are then F16 and the products exact.  A probability is
 // two F16 terms (22 bits), the second with products of its own: 0.21e-3 off 64 bits, which is the rounding of the output alone, against 0.29e-3
-// with one term.  That costs 118 -> 131 us on the largest case below and nothing where the products are not the bound.
+// with one term.  That costs 118 -> 131 us on that case and nothing where the products are not the bound.
 //
 // Work split: the cached tiles of all (group, kv head, row block) items, one after another, in equal shares, one per CTA; a share may
 // begin and end inside an item.  The partial rows of item i and share c start at (rows before item i) + 256 * c, which keeps them
