@@ -15,14 +15,14 @@
 // step are there when the softmax of this one ends.  (One buffer of 128 tokens per stream left the softmax warps waiting for two products per
 // tile: 4 800 cycles per tile of both streams.)  A softmax thread owns a row: no exchange between threads.  P goes back to tensor memory, over
 // the S it was made from, as the A operand of the second product, so shared memory holds Q and the K and V tiles only.  The row maximum in use
-// is raised, and O rescaled, only when a score exceeds it by 2^6.
+// is raised, and O rescaled, only when a score is 14 above a reference that lies 8 below the maximum it was set from.
 // Measured: 128 sequences on 16 384 tokens, 64 query heads: 131 us for the call, 529 TFLOP/s of useful products (0.32 of the measured bf16 rate; with
 // the second terms counted 0.48).  A step of 64 tokens takes both streams some 2 100 cycles, of which the products are 1 790 (N = 64 from shared
 // memory 48 cycles each, with A in tensor memory 64) and the rest hand-offs between softmax and issuers.
 // An F16 pool's tiles arrive as tensor-map boxes, in the 128-byte swizzle the MMA reads.  An E4M3 pool's tiles are widened to F16
-// on the way by four warps (exact); K's block scale multiplies the scores, V's the probabilities, in units of a power of two above every
-// scale met so far.  Both operands of both products are then F16 and the products exact.  A probability is
-// two F16 terms (22 bits), the second with products of its own: 0.21e-3 off 64 bits, which is the rounding of the output alone, against 0.29e-3
+// on the way by four warps (exact); K's block scale multiplies the scores, V's the probabilities, in units of a power of two per row that goes by
+// the largest probability times scale met so far (tkv_rows_attn.cuh).  Both operands of both products are then F16 and the products exact.  A
+// probability is two F16 terms (22 bits), the second with products of its own: 0.21e-3 off 64 bits, which is the rounding of the output alone, against 0.29e-3
 // with one term.  That costs 118 -> 131 us on that case and nothing where the products are not the bound.
 //
 // Work split: the cached tiles of all (group, kv head, row block) items, one after another, in equal shares, one per CTA; a share may
@@ -55,7 +55,8 @@ using tkv_rows::bar_wait;
 constexpr uint32_t CTAS = 148;               // one per SM of the part this is built for; partial results are sized by it
 constexpr int BS = 16, KT = 128, ST = 64;    // tokens of a block, of a cached tile, of a step
 constexpr int GROUP_BYTES = 128 * 128;       // a [128 rows][128 B] swizzled column group of an operand tile
-constexpr float RAISE = 6.0f;
+using tkv_rows::HEAD;
+using tkv_rows::RAISE;
 // Cached tiles of a share: at least two where there are shares for more than half of the SMs, so that the kernel for the tokens behind the prefix
 // finds SMs beside this one (64 sequences on 2 048 tokens: 41 us with 2, 53 with 1), else one (3 on 48: 14 us, 18 with 2).
 __host__ __device__ __forceinline__ uint32_t min_share(uint64_t tiles) { return 2 * tiles > CTAS ? 2u : 1u; }
@@ -81,7 +82,7 @@ struct Control {
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
     uint64_t q_ready[2], s_full[2][2], p_full[2][2], pv_done[2][2], drained[2];   // [stream][S buffer]
     uint32_t tmem, fail;
-    float scales[4][16];                     // per cached tile (mod 4): K scales of its 8 blocks, V scales
+    float scales[4][24];                     // per cached tile (mod 4): of its 8 blocks K scale x scale_log2, V scale, log2 of V scale
 };
 constexpr uint32_t CTRL_BYTES = 1024;
 static_assert(sizeof(Control) <= CTRL_BYTES, "control block");
@@ -421,7 +422,8 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     const uint32_t t = tiles_done + i, st = t & 1u;
                     if (t >= 2) ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(c->k_empty + st), ((t >> 1) - 1u) & 1u, fail));
                     if (!ok) break;
-                    if (t128 < 16) c->scales[t & 3u][t128] = sc;
+                    if (t128 < 16) c->scales[t & 3u][t128] = t128 < 8 ? sc * a.scale_log2 : sc;
+                    if (t128 >= 8 && t128 < 16) c->scales[t & 3u][t128 + 8] = fast_log2(fabsf(sc));
                     widen(k_ring + st * TILE, 0);
                     if (lane == 0) mbar_arrive(c->k_full + st);
                     load_scales();
@@ -463,7 +465,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 if (lane == 0) mbar_arrive(c->q_ready + x);
             }
             const uint32_t lanes = ((warp & 3u) * 32u) << 16, ts = tmem + TM_S + x * 128 + lanes, to = tmem + TM_O + x * 128 + lanes;
-            float m = -INFINITY, l = 0.0f, v_ref = FP8 ? 0x1p-100f : 1.0f, v_inv = FP8 ? 0x1p+100f : 1.0f;
+            float m = -INFINITY, l = 0.0f, unit = FP8 ? tkv_rows::UNIT_MOST : 1.0f;   // O is in units of 1 / unit
             uint32_t n = s_x;                                   // steps of this stream so far
             for (uint32_t i = 0; i < it.n_tiles && ok; i++) {
                 const uint32_t slot = (tiles_done + i) & 3u, h_end = steps_in(i);
@@ -483,31 +485,31 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
 #pragma unroll
                             for (int q = 0; q < NB; q++) tmem_ld16(tb + q * 16, v[q]);
                             tmem_wait_ld();
-                            float mx = -INFINITY;               // neither scale is negative: the maximum commutes with them
+                            float mx = -INFINITY, mv = -INFINITY;   // no scale is negative: the maximum commutes with them; mv: with V's scale
 #pragma unroll
                             for (int q = 0; q < NB; q++) {      // a block
                                 float top = -INFINITY;
 #pragma unroll
                                 for (int k = 0; k < 16; k++) top = fmaxf(top, MASKED && q * 16 + k >= left ? -INFINITY : __uint_as_float(v[q][k]));
-                                mx = FP8 ? fmaxf(mx, top == -INFINITY ? top : top * sc[q]) : fmaxf(mx, top);
+                                if (FP8) {
+                                    top *= sc[q];               // -inf x 0 is NaN, which no maximum takes
+                                    mv = fmaxf(mv, top + sc[16 + q]);
+                                }
+                                mx = fmaxf(mx, top);
                             }
-                            mx = mx == -INFINITY ? mx : mx * a.scale_log2;
-                            // ---- a raised maximum or V scale rescales the row of O, once the product of the step before is done ----
+                            if (!FP8) mx = mx == -INFINITY ? mx : mx * a.scale_log2;
+                            // ---- a raised reference rescales the row of O, once the product of the step before is done ----
                             float factor = 1.0f;
-                            if (mx > m + RAISE) {
-                                factor = m == -INFINITY ? 0.0f : fast_exp2(m - mx);
-                                m = mx;
+                            if (mx > m + RAISE || (FP8 && mv + tkv_rows::log2_of_power(unit) > m + RAISE)) {
+                                const float m_new = fmaxf(m, mx - HEAD);
+                                const float up = m_new - m;
+                                factor = m == -INFINITY ? 0.0f : fast_exp2(-up);
+                                m = m_new;
                                 l *= factor;
-                            }
-                            if (FP8) {
-                                float top = sc[8];
-#pragma unroll
-                                for (int q = 1; q < NB; q++) top = fmaxf(top, sc[8 + q]);
-                                if (top > v_ref) {              // the same in every thread
-                                    const float up = __uint_as_float(min((__float_as_uint(top) >> 23) + 1u, 253u) << 23);
-                                    factor *= v_ref / up;
-                                    v_ref = up;
-                                    v_inv = 1.0f / up;
+                                if (FP8) {
+                                    const float u = tkv_rows::next_unit(unit, up, mv == -INFINITY ? mv : mv - m);
+                                    factor *= u * tkv_rows::inverse_of_power(unit);
+                                    unit = u;
                                 }
                             }
                             if (n > s_x && __any_sync(0xFFFFFFFFu, factor != 1.0f)) {
@@ -529,7 +531,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                             float sum = 0.0f;
 #pragma unroll
                             for (int q = 0; q < NB; q++) {
-                                const float ks = FP8 ? a.scale_log2 * sc[q] : a.scale_log2, vn = FP8 ? sc[8 + q] * v_inv : 1.0f;
+                                const float ks = FP8 ? sc[q] : a.scale_log2, vn = FP8 ? sc[8 + q] * unit : 1.0f;
                                 uint32_t first[8], second[8];
 #pragma unroll
                                 for (int k = 0; k < 16; k += 2) {
@@ -578,6 +580,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     constexpr int DH = D / 2, CH = DH / 4;      // dims of a pass; its 16-byte chunks per row
                     unsigned char* stage = q_tile + x * TILE + (warp & 3u) * (TILE / 4);
                     const uint32_t n_live = (uint32_t)__popc(__ballot_sync(0xFFFFFFFFu, live));
+                    const float inv_unit = tkv_rows::inverse_of_power(unit);
                     float* rows_out = a.part_o + (dst - lane) * D;             // (the warp's first row is alive if any is)
 #pragma unroll 1
                     for (int d0 = 0; d0 < D; d0 += DH) {
@@ -589,8 +592,8 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
 #pragma unroll
                             for (int k = 0; k < 8; k++)
                                 *reinterpret_cast<float4*>(stage + lane * (DH * 4) + (((c0 / 4 + k) ^ (lane % CH)) * 16)) =
-                                    make_float4(__uint_as_float(o[4 * k]) * v_ref, __uint_as_float(o[4 * k + 1]) * v_ref, __uint_as_float(o[4 * k + 2]) * v_ref,
-                                                __uint_as_float(o[4 * k + 3]) * v_ref);
+                                    make_float4(__uint_as_float(o[4 * k]) * inv_unit, __uint_as_float(o[4 * k + 1]) * inv_unit, __uint_as_float(o[4 * k + 2]) * inv_unit,
+                                                __uint_as_float(o[4 * k + 3]) * inv_unit);
                         }
                         __syncwarp();
 #pragma unroll 8

@@ -2,7 +2,7 @@
 // head_dim 64 or 128, F16 or E4M3 blocks: the part that the scored decode attention and the shared-prefix attention have in
 // common (the latter runs it over the tokens behind the prefix).
 //
-//   x[t] = scale * log2(e) * k_scale * (q . k_t),   m >= max x - 6,   l = sum 2^(x[t] - m),   O = sum 2^(x[t] - m) * v_t
+//   x[t] = scale * log2(e) * k_scale * (q . k_t),   m >= max x - 14,   l = sum 2^(x[t] - m),   O = sum 2^(x[t] - m) * v_t
 //
 // and (m, l, O) of a token range is one partial result; ranges are joined by a second kernel.
 //
@@ -16,9 +16,13 @@
 // 16-byte fragment reads of K (four lanes side by side in each of two tokens) and of V (two lanes side by side in each of four tokens)
 // are free of bank conflicts.  The order of the dims inside a contraction is free too: a lane's fragment is a 16-byte run.
 // Both contractions run on mma.sync m16n8k16 with the tokens (K) or the dims (V) as the 16 rows and the query heads as the 8
-// columns; the maximum is only raised, for all lanes at once after a vote, when a score exceeds it by 2^6, so the common step has
-// no shuffle in it.  Probabilities are used as two F16 terms (22 bits): with up to four query heads per kv head the second term
-// rides in the four spare columns of the same MMAs, else it is a second set of them.
+// columns; the reference m lies 8 below a maximum that it is set from and is only raised, for all lanes at once after a vote, when a score
+// exceeds it by 14, so the common step has no shuffle in it.  Probabilities are used as two F16 terms: with up to four query heads per kv
+// head the second term rides in the four spare columns of the same MMAs, else it is a second set of them.  Between 2^8 (or more) for the
+// largest and F16's smallest step of 2^-24 they keep 22 bits down to 2^-10 of the largest and are off by 2^-33 of it below.
+// In a scaled E4M3 pool what the MMA takes is 2^(x - m) * v_scale * unit, with a power of two `unit` per query head that holds the largest such
+// product met so far (not the largest scale: a block that is large but not attended to must not push the others among F16's subnormals)
+// where the largest probability would be.
 //
 // A block costs a consumer a chain of dependent steps (wait, fragments, eight MMAs, exp2, transposes, eight MMAs).  For an F16 block the
 // chain is shorter than the time in which HBM delivers the block (131 071 tokens of 8 heads: 92 us, 5.9 TB/s); for an E4M3 block, with half
@@ -45,7 +49,17 @@ constexpr uint32_t PAD = 32;                 // bytes between runs of four token
 constexpr uint32_t SCALE_BYTES = 2 * WARPS * 4;
 constexpr uint32_t RING_BYTES = 208 * 1024;  // of all streams of a CTA
 constexpr uint32_t SEQ_CACHE = 1024;         // sequences whose ranges a CTA keeps in shared memory (more are looked up again)
-constexpr float RAISE = 6.0f;                // log2: probabilities reach 2^6, far inside F16
+constexpr float HEAD = 8.0f, RAISE = 14.0f;  // log2: what is largest is put at 2^8 and may grow to 2^14 (F16 ends below 2^16) before it is put there again
+constexpr float UNIT_MOST = 0x1p+100f;
+// of a power of two
+__device__ __forceinline__ float log2_of_power(float u) { return (float)((int)(__float_as_uint(u) >> 23) - 127); }
+__device__ __forceinline__ float inverse_of_power(float u) { return __uint_as_float(0x7F000000u - __float_as_uint(u)); }
+// The unit of a row whose reference was just raised by `up`; `top` is the largest probability times V scale at hand as a power of two (-inf: none).
+// Measured absolutely a unit only falls, as a maximum only rises.  (up <= 126: what O is multiplied by stays a number.)
+__device__ __forceinline__ float next_unit(float unit, float up, float top) {
+    const float e = fminf(log2_of_power(unit) + fminf(up, 126.0f), HEAD - top);
+    return __uint_as_float((uint32_t)((int)floorf(fminf(fmaxf(e, -110.0f), 100.0f)) + 127) << 23);
+}
 
 struct Args {
     const char *k_base, *v_base;             // layer tensors
@@ -70,6 +84,11 @@ __device__ __forceinline__ void report(uint32_t* status, uint32_t code) {
 __device__ __forceinline__ float exp2_fast(float x) {          // 2^x, relative error 2^-22, 2^-inf = 0
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float log2_fast(float x) {
+    float r;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
@@ -439,8 +458,7 @@ __global__ void __launch_bounds__(THREADS, 1) rows_attn(const Args a) {
         float o[MT][4], m2[2] = {-INFINITY, -INFINITY}, l2[2] = {0.0f, 0.0f};   // o[t]: dims 2t, 2t + 1 of this lane's run, columns 2j, 2j + 1
 #pragma unroll
         for (int t = 0; t < MT; t++) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
-        float v_ref = FP8 ? 0x1p-100f : 1.0f, v_inv = FP8 ? 0x1p+100f : 1.0f;   // a power of two above every V scale met so far: O is in units of
-                                                                // it, and P x scale / v_ref stays in F16's range
+        float unit[2] = {scaled ? UNIT_MOST : 1.0f, scaled ? UNIT_MOST : 1.0f};   // O is in units of 1 / unit
         float* lg = a.logits ? a.logits + ((size_t)c.seq * a.n_q_heads + kvh * a.group + 2 * j) * a.logit_stride + c.block * BS + tok_k : nullptr;
         const uint32_t n = c.left;
         for (uint32_t turn = 0; turn < n; turn++) {
@@ -502,34 +520,37 @@ __global__ void __launch_bounds__(THREADS, 1) rows_attn(const Args a) {
                 if (col1 && lo) at[0] = x[1];
                 if (col1 && hi) at[2] = x[3];
             }
-            // the maxima in use are raised, for all lanes together, once a score is 2^6 above
-            const bool over = fmaxf(x[0], x[2]) > m2[0] + RAISE || fmaxf(x[1], x[3]) > m2[1] + RAISE;
+            // the references in use are raised, for all lanes together, once a score (or a score and its V scale) is too far above
+            float room[2] = {RAISE, RAISE}, vs_log2 = 0.0f;
+            if (FP8 && scaled) {
+                vs_log2 = log2_fast(fabsf(vs));
+                room[0] -= fmaxf(vs_log2 + log2_of_power(unit[0]), 0.0f);
+                room[1] -= fmaxf(vs_log2 + log2_of_power(unit[1]), 0.0f);
+            }
+            const bool over = fmaxf(x[0], x[2]) > m2[0] + room[0] || fmaxf(x[1], x[3]) > m2[1] + room[1];
             if (__any_sync(0xFFFFFFFFu, over)) {
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    float mx = fmaxf(m2[e], fmaxf(x[e], x[2 + e]));
+                    float mx = fmaxf(x[e], x[2 + e]);
                     mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
-                    const float keep = m2[e] == -INFINITY ? 0.0f : exp2_fast(m2[e] - mx);
-                    m2[e] = mx;
+                    const float m_new = fmaxf(m2[e], mx - HEAD);
+                    const float up = m_new - m2[e];
+                    float keep = m2[e] == -INFINITY ? 0.0f : exp2_fast(-up);
+                    m2[e] = m_new;
                     l2[e] *= keep;
+                    if (FP8 && scaled) {
+                        const float u = next_unit(unit[e], up, mx == -INFINITY ? mx : mx - m_new + vs_log2);
+                        keep *= u * inverse_of_power(unit[e]);
+                        unit[e] = u;
+                    }
 #pragma unroll
                     for (int t = 0; t < MT; t++) {
                         o[t][e] *= keep;
                         o[t][2 + e] *= keep;
                     }
                 }
-            }
-            if (FP8 && vs > v_ref) {                            // the same in every lane
-                const float up = __uint_as_float(min((__float_as_uint(vs) >> 23) + 1u, 253u) << 23);
-                const float keep = v_ref / up;
-                v_ref = up;
-                v_inv = 1.0f / up;
-#pragma unroll
-                for (int t = 0; t < MT; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) o[t][i] *= keep;
             }
             const float sub0 = m2[0] == -INFINITY ? 0.0f : m2[0], sub1 = m2[1] == -INFINITY ? 0.0f : m2[1];
             // probabilities, and O += V^T P
@@ -540,10 +561,10 @@ __global__ void __launch_bounds__(THREADS, 1) rows_attn(const Args a) {
             p[3] = exp2_fast(x[3] - sub1);
             l2[0] += p[0] + p[2];
             l2[1] += p[1] + p[3];
-            if (FP8) {
-                const float vn = vs * v_inv;
+            if (FP8 && scaled) {
+                const float vn[2] = {vs * unit[0], vs * unit[1]};
 #pragma unroll
-                for (int i = 0; i < 4; i++) p[i] *= vn;
+                for (int i = 0; i < 4; i++) p[i] *= vn[i & 1];
             }
             __half2 pl = __floats2half2_rn(p[0], p[1]), ph = __floats2half2_rn(p[2], p[3]);
             const float2 fl = __half22float2(pl), fh = __half22float2(ph);
@@ -618,6 +639,7 @@ __global__ void __launch_bounds__(THREADS, 1) rows_attn(const Args a) {
             l += __shfl_xor_sync(0xFFFFFFFFu, l, 8);
             l += __shfl_xor_sync(0xFFFFFFFFu, l, 16);
             const uint32_t head = 2 * j + e;
+            const float inv_unit = inverse_of_power(unit[e]);
             if (head < a.group) {
                 const size_t row = at_slot * a.n_q_heads + kvh * a.group + head;
                 if (grp == 0) *reinterpret_cast<float2*>(a.part_ml + row * 2) = make_float2(m2[e], l);
@@ -626,7 +648,7 @@ __global__ void __launch_bounds__(THREADS, 1) rows_attn(const Args a) {
                 for (int t = 0; t < MT; t++) {
                     constexpr int RUN = S::VPB / S::ES;         // dims of a piece
                     const int i = 2 * t, dim = (i / RUN) * (8 * RUN) + (int)grp * RUN + i % RUN;
-                    *reinterpret_cast<float2*>(dst + dim) = make_float2(o[t][e] * v_ref, o[t][2 + e] * v_ref);
+                    *reinterpret_cast<float2*>(dst + dim) = make_float2(o[t][e] * inv_unit, o[t][2 + e] * inv_unit);
                 }
             }
         }
