@@ -1,10 +1,12 @@
 """How exact the attention operators of the cache are, judged against the size of what is summed rather than against the largest V.
 
-With w in 64 bits, A the largest sum of |scale log2(e) q_i k_i| of a row and n its tokens, an element of out may be off by
+V is made so that a row's weighted sum nearly cancels: the rounding of the output to F16, 2^-11 of it, is then small, and what is left is the error
+of the weights.  With w in 64 bits, A the largest sum of |scale log2(e) q_i k_i| of a row and n its tokens, an element of out may be off by
     2^-11 |out| + 2^-25 + sum_t w_t |v_t| * c,   c = 2 ln 2 A (D / 16 + 6) 2^-23 + (n / 8 + 24) 2^-23 + 2^-21:
 a score is D / 16 truncating MMA steps and at most six roundings of terms whose sum of magnitudes is A (twice: in the weight and in the sum that it
 is divided by); a row of O is two MMA steps per 16 tokens and at most 24 roundings (rescaling, joining, the sum's own); a probability of
-22 bits and exp2 are 2^-23 and 2^-22 each, at both places."""
+22 bits and exp2 are 2^-23 and 2^-22 each, at both places.  A probability of one F16 term is off by up to 2^-11: the tests plant that in a plain
+implementation and require that the bound catches it."""
 import math
 
 import pytest
@@ -33,11 +35,25 @@ def weights(q, k, scale):
     return torch.softmax(q @ k.T * scale, dim=1), float((q.abs() @ k.abs().T).max()) * abs(scale) * LOG2E
 
 
+def cancel(w, v, to):
+    """Row `to` of v so that w @ v is about zero (w: one row of weights)."""
+    rest = w @ v - w[to] * v[to]
+    v[to] = -rest / w[to]
+
+
 def bound(w, v, a, dim):
     """Per element of w @ v, see above."""
     n = v.shape[0]
     c = 2 * math.log(2) * a * (dim / 16 + 6) * 2.0 ** -23 + (n / 8 + 24) * 2.0 ** -23 + 2.0 ** -21
     return 2.0 ** -11 * (w @ v).abs() + 2.0 ** -25 + c * (w @ v.abs())
+
+
+def one_term(q, k, v, scale):
+    """The same attention with every probability rounded to F16 once, relative to its row's largest."""
+    import torch
+    x = q @ k.T * scale
+    p = torch.exp(x - x.amax(dim=1, keepdim=True))
+    return p.to(torch.float16).double() @ v / p.sum(dim=1, keepdim=True)
 
 
 class Case:
@@ -76,14 +92,72 @@ class Case:
             self.v.append(torch.cat(kept[1]))
 
 
-def judge(out, q, case, s, h, group, scale):
-    """Checks query heads of kv head h of sequence s."""
+def cancelling_rows(q, n, kv_heads, dim, g, dtype, scale):
+    """K and V [n, kv_heads, dim] for which a query row q [dim] attends to a sum of about zero."""
+    import torch
+    k = torch.randn((n, kv_heads, dim), generator=g, dtype=torch.float64)
+    v = torch.randn((n, kv_heads, dim), generator=g, dtype=torch.float64)
+    k, v = k.to(torch.float16).double(), v.to(torch.float16).double()
+    for h in range(kv_heads):
+        w, _ = weights(q[None], k[:, h], scale)
+        cancel(w[0], v[:, h], int(w[0].argmax()))
+    return k, v
+
+
+def judge(out, q, case, s, h, group, scale, planted=None):
+    """Checks query heads of kv head h of sequence s; `planted` collects how far a one-term form is outside of the bound."""
     k, v = case.k[s][:, h], case.v[s][:, h]
     rows = slice(h * group, (h + 1) * group)
     w, a = weights(q[s][rows].double(), k, scale)
     b = bound(w, v, a, case.dim)
     err = (out[s][rows].double().cpu() - w @ v).abs()
     assert (err <= b).all(), f"sequence {s}, kv head {h}: off by {(err / b).max():.2f} of the bound"
+    if planted is not None:
+        planted.append(float(((one_term(q[s][rows].double(), k, v, scale) - w @ v).abs() / b).max()))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "e4m3", "e4m3 unscaled"])
+@pytest.mark.parametrize("kv_heads,dim,group", [(2, 128, 4), (3, 64, 8), (1, 128, 2)])
+def test_scored_attention_keeps_both_terms_of_a_probability(H, dtype, kv_heads, dim, group):
+    import torch
+    g = torch.Generator().manual_seed(dim + group)
+    lens, scale = [2, 3, 7, 16, 20, 40], 1 / math.sqrt(dim)
+    q1 = torch.randn((len(lens), dim), generator=g).to(torch.float16)
+    rows = [cancelling_rows(q1[s].double(), n, kv_heads, dim, g, dtype, scale) for s, n in enumerate(lens)]
+    case = Case(H, dtype, kv_heads, dim, rows)
+    q = q1[:, None].repeat(1, kv_heads * group, 1)
+    scores = torch.zeros((1, len(lens), kv_heads, 48)).cuda()
+    attn = H.ScoredDecodeAttention(case.pool, q.cuda(), case.tables.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), scores, 48)
+    out, planted = attn.enqueue(0), []
+    assert int(attn.status.item()) == 0
+    for s in range(len(lens)):
+        for h in range(kv_heads):
+            judge(out, q, case, s, h, group, scale, planted)
+    assert max(planted) > 2                                           # what is tested for would show
+
+
+@pytest.mark.parametrize("dtype", ["f16", "e4m3", "e4m3 unscaled"])
+@pytest.mark.parametrize("kv_heads,dim,group,members", [(2, 128, 4, 3), (3, 64, 8, 20), (1, 128, 2, 140)])
+def test_prefix_attention_keeps_both_terms_of_a_probability(H, dtype, kv_heads, dim, group, members):
+    """Groups that are nothing but their prefix: one tile, a short tile, and several steps."""
+    import torch
+    g = torch.Generator().manual_seed(dim + group + members)
+    prefixes, scale = [16, 48, 64], 1 / math.sqrt(dim)
+    q1 = torch.randn((len(prefixes), dim), generator=g).to(torch.float16)
+    rows = [cancelling_rows(q1[i].double(), n, kv_heads, dim, g, dtype, scale) for i, n in enumerate(prefixes)]
+    case = Case(H, dtype, kv_heads, dim, rows)
+    of = torch.arange(len(prefixes)).repeat_interleave(members)
+    case.k, case.v = [case.k[i] for i in of], [case.v[i] for i in of]
+    q = q1[of][:, None].repeat(1, kv_heads * group, 1)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+    attn = H.PrefixAttention(case.pool, q.cuda(), case.tables[of].contiguous().cuda(), i32([prefixes[i] for i in of]),
+                             i32([members * i for i in range(len(prefixes) + 1)]), i32(prefixes), max(prefixes), max(prefixes))
+    out, planted = attn.enqueue(0), []
+    assert int(attn.status.item()) == 0
+    for s in range(0, len(of), max(1, members // 3)):
+        for h in range(kv_heads):
+            judge(out, q, case, s, h, group, scale, planted)
+    assert max(planted) > 2
 
 
 def spread_rows(n, loud, ratio, dim, g, q):
