@@ -450,7 +450,7 @@ int32_t tkv_evict_select_enqueue(const TkvEvictSelect* p, void* stream) {
     while (cluster < MAX_CLUSTER && p->max_kv_len / cluster > 32768) cluster *= 2;
     if (rows * cluster > 0x7FFFFFFFull) return fail(TKV_ERR_INVALID_CONFIG, "%llu rows: batch too large", rows);
     if (p->new_lens == p->kv_lens) return fail(TKV_ERR_INVALID_CONFIG, "new_lens must not be kv_lens: every row reads the old length");
-    const uint32_t slice = (p->max_kv_len + cluster - 1) / cluster;
+    const uint32_t slice = (uint32_t)(((uint64_t)p->max_kv_len + cluster - 1) / cluster);   // (a bound near 2^32 must not wrap to a small slice)
     SelectArgs a{};
     a.scores = reinterpret_cast<const float*>(p->scores);
     a.kv_lens = reinterpret_cast<const uint32_t*>(p->kv_lens);

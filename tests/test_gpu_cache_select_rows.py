@@ -1,8 +1,12 @@
 """Select at the row lengths where its work is split differently: one CTA, staged clusters of two, four and eight, a cluster whose slices do not fit
 shared memory; several rows per launch, short and uncut rows inside a clustered launch."""
 
+import ctypes
+
 import numpy as np
 import pytest
+
+from tempura_b200 import _native as N
 
 from test_gpu_cache_eviction import H, check_choice  # noqa: F401  (H is the fixture)
 
@@ -36,3 +40,18 @@ def test_rows_of_one_cta(H, shape, lens):  # noqa: F811
     scores = tied(shape, shape[3])
     for budget in (100, shape[3] // 3, shape[3] - 5):
         check_choice(H, scores, lens, [0] * len(lens), budget, 64)
+
+
+@pytest.mark.parametrize("bound", [0xFFFFFFFF, 0xFFFFFFF9, 0xFFFFFFF8, 1 << 31])
+def test_a_length_bound_at_the_end_of_32_bits(H, bound):  # noqa: F811
+    """One row whose length is far below a bound that no row could reach: the bound decides how a row is split, and must not wrap."""
+    import torch
+    scores = torch.rand(500, generator=torch.Generator().manual_seed(1)).cuda()
+    lens, kept, new, status = (torch.zeros(n, dtype=torch.int32).cuda() for n in (1, 64, 1, 1))
+    lens.fill_(500)
+    args = N.TkvEvictSelect(0, 1, 1, 1, bound, bound, 64, 64, 8, 0, scores.data_ptr(), lens.data_ptr(), 0, kept.data_ptr(), new.data_ptr(), status.data_ptr())
+    torch.cuda.synchronize()
+    assert N.lib().tkv_evict_select_enqueue(ctypes.byref(args), None) == 0
+    torch.cuda.synchronize()
+    top = sorted(torch.topk(scores[:492], 56).indices.tolist()) + list(range(492, 500))
+    assert int(status) == 0 and int(new) == 64 and kept.tolist() == top
