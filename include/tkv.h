@@ -493,7 +493,7 @@ typedef struct TkvEvictSelect {
     uint64_t kv_lens;             /* u32 [n_seqs]                                                                   */
     uint64_t protect;             /* u32 [n_seqs], or 0: nothing protected                                          */
     uint64_t kept;                /* u32 [n_layers][n_seqs][n_kv_heads][kept_stride]                                */
-    uint64_t new_lens;            /* u32 [n_seqs], not kv_lens itself                                               */
+    uint64_t new_lens;            /* u32 [n_seqs], memory of its own: no part of kv_lens or protect                 */
     uint64_t status;              /* 0, or a device u32 (zero it before the launch): TKV_ERR_INVALID_CONFIG if kv_lens held a value
                                      above max_kv_len (clamped to it) or kept is too narrow for a sequence, which then is not cut */
 } TkvEvictSelect;

@@ -449,7 +449,10 @@ int32_t tkv_evict_select_enqueue(const TkvEvictSelect* p, void* stream) {
     uint32_t cluster = 1;
     while (cluster < MAX_CLUSTER && p->max_kv_len / cluster > 32768) cluster *= 2;
     if (rows * cluster > 0x7FFFFFFFull) return fail(TKV_ERR_INVALID_CONFIG, "%llu rows: batch too large", rows);
-    if (p->new_lens == p->kv_lens) return fail(TKV_ERR_INVALID_CONFIG, "new_lens must not be kv_lens: every row reads the old length");
+    // every row reads its sequence's length and protection; the first one of a layer writes the new length
+    const uint64_t lens_bytes = 4ull * p->n_seqs;
+    auto meets = [&](uint64_t other) { return other && p->new_lens < other + lens_bytes && other < p->new_lens + lens_bytes; };
+    if (meets(p->kv_lens) || meets(p->protect)) return fail(TKV_ERR_INVALID_CONFIG, "new_lens must not share memory with kv_lens or protect: every row reads those");
     const uint32_t slice = (uint32_t)(((uint64_t)p->max_kv_len + cluster - 1) / cluster);   // (a bound near 2^32 must not wrap to a small slice)
     SelectArgs a{};
     a.scores = reinterpret_cast<const float*>(p->scores);

@@ -137,3 +137,17 @@ def test_workspaces_grow_with_what_they_hold(L):
     p = L.tkv_prefix_attn_scratch_bytes
     assert p(0, 1, 8, 4, 64, 100, 64) == 0 and p(1, 0, 8, 4, 64, 100, 64) == 0
     assert 0 < p(1, 1, 8, 4, 64, 0, 0) <= p(1, 1, 8, 4, 64, 1000, 512) < p(64, 1, 8, 4, 64, 1000, 512) < p(64, 1, 8, 4, 128, 1000, 512)
+
+
+@pytest.mark.parametrize("change", [{"protect": A + 4096}, {"protect": A + 4096 + 4}, {"protect": A + 4096 - 4}, {"kv_lens": A + 4096 + 4}, {"kv_lens": A + 4096 - 4}])
+def test_select_refuses_new_lens_that_share_memory_with_what_every_row_reads(L, change):
+    assert L.tkv_evict_select_enqueue(C.byref(select(new_lens=A + 4096, **change)), None) == BAD
+    text = C.create_string_buffer(256)
+    L.tkv_last_error(text, 256)
+    assert b"new_lens" in text.value
+
+
+def test_select_takes_neighbouring_buffers(L):
+    """Side by side in one allocation is no overlap: the call goes on to the device (or, without one, to its error)."""
+    for change in ({"protect": A + 4096 + 8}, {"protect": A + 4096 - 8}, {"kv_lens": A + 4096 + 8}, {"kv_lens": A + 4096 - 8}):
+        assert L.tkv_evict_select_enqueue(C.byref(select(device=1 << 20, new_lens=A + 4096, **change)), None) == N.ERR_CUDA
