@@ -418,14 +418,18 @@ int32_t fail(int32_t code, const char* fmt, unsigned long long x = 0, unsigned l
     return tkv_internal::set_error(code, 0, buf);
 }
 int32_t launch_error(const char* what, cudaError_t e) {
+    cudaGetLastError();                                         // reported here, not by whoever asks next
     char buf[256];
     snprintf(buf, sizeof buf, "%s launch: %s (cuda error %d)", what, cudaGetErrorString(e), (int)e);
     return tkv_internal::set_error(TKV_ERR_CUDA, (int32_t)e, buf);
 }
 
-template <int ROW> void launch_compact(bool scaled, const CompactArgs& a, dim3 grid, cudaStream_t st) {
-    if (scaled) evict_compact<ROW, true><<<grid, CMP_THREADS, 0, st>>>(a);
-    else evict_compact<ROW, false><<<grid, CMP_THREADS, 0, st>>>(a);
+template <int ROW, bool SCALED> cudaError_t launch_compact(const CompactArgs& a, dim3 grid, cudaStream_t st) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(CMP_THREADS);
+    cfg.stream = st;
+    return cudaLaunchKernelEx(&cfg, evict_compact<ROW, SCALED>, a);
 }
 
 }  // namespace
@@ -558,10 +562,9 @@ int32_t tkv_evict_compact_enqueue(const TkvPool* pool, const TkvEvictCompact* p,
         const dim3 grid((unsigned)per_layer, n, a.scores ? 3 : 2);
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         const bool scaled = a.k_scales != nullptr;
-        if (row == 256) evict_compact<256, false><<<grid, CMP_THREADS, 0, st>>>(a);     // 128 F16 dims
-        else if (row == 128) launch_compact<128>(scaled, a, grid, st);
-        else launch_compact<64>(scaled, a, grid, st);
-        e = cudaGetLastError();
+        if (row == 256) e = launch_compact<256, false>(a, grid, st);                    // 128 F16 dims
+        else if (row == 128) e = scaled ? launch_compact<128, true>(a, grid, st) : launch_compact<128, false>(a, grid, st);
+        else e = scaled ? launch_compact<64, true>(a, grid, st) : launch_compact<64, false>(a, grid, st);
     }
     if (prev >= 0 && prev != pool->device) cudaSetDevice(prev);
     return e == cudaSuccess ? TKV_OK : launch_error("evict compact", e);

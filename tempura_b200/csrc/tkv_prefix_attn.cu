@@ -788,8 +788,12 @@ template <int D, bool FP8> cudaError_t launch_prefix(const CUtensorMap& mk, cons
         if (e != cudaSuccess) return e;
         granted.fetch_or(bit, std::memory_order_relaxed);
     }
-    kernel<<<a.parts, threads_of(FP8), smem, st>>>(mk, mv, a);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(a.parts);
+    cfg.blockDim = dim3(threads_of(FP8));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    return cudaLaunchKernelEx(&cfg, kernel, mk, mv, a);
 }
 template <int D> cudaError_t launch_join(const JoinArgs& a, cudaStream_t st) {
     const uint64_t rows = (uint64_t)a.n_seqs * a.n_q_heads;
@@ -946,6 +950,7 @@ int32_t tkv_prefix_attn_enqueue(const TkvPool* pool, const TkvPrefixAttn* p, voi
     }
     if (prev >= 0 && prev != pool->device) cudaSetDevice(prev);
     if (e != cudaSuccess) {
+        cudaGetLastError();                                     // reported here, not by whoever asks next
         char buf[256];
         snprintf(buf, sizeof buf, "shared-prefix attention launch: %s (cuda error %d)", cudaGetErrorString(e), (int)e);
         return tkv_internal::set_error(TKV_ERR_CUDA, (int32_t)e, buf);

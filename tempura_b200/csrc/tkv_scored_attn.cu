@@ -337,6 +337,7 @@ int32_t tkv_scored_attn_enqueue(const TkvPool* pool, const TkvScoredAttn* p, voi
     }
     if (prev >= 0 && prev != pool->device) cudaSetDevice(prev);
     if (e != cudaSuccess) {
+        cudaGetLastError();                                     // reported here, not by whoever asks next
         char buf[256];
         snprintf(buf, sizeof buf, "scored attention launch: %s (cuda error %d)", cudaGetErrorString(e), (int)e);
         return tkv_internal::set_error(TKV_ERR_CUDA, (int32_t)e, buf);
