@@ -456,6 +456,31 @@ def decode_attention(pool: Pool, layer: int, q: torch.Tensor, tables: torch.Tens
     return out
 
 
+class _Buffers:
+    """What a handle made for itself on the stream that was current then.  Another stream's first call waits until that is done, and the
+    allocator hands none of it out again before that stream's work has ended, however early the handle is dropped.  (A stream that is being
+    captured waits for nothing: the graph's owner keeps the handle, and a capture begins on an idle device.)"""
+
+    def __init__(self, device: int, *tensors: torch.Tensor):
+        home = torch.cuda.current_stream(device)
+        self._tensors, self._known = tensors, {home.cuda_stream}
+        self._made = None if self._capturing(home) else home.record_event()
+
+    @staticmethod
+    def _capturing(stream: torch.cuda.Stream) -> bool:
+        with torch.cuda.stream(stream):
+            return torch.cuda.is_current_stream_capturing()
+
+    def use(self, stream: torch.cuda.Stream) -> None:
+        if stream.cuda_stream in self._known or self._capturing(stream):
+            return
+        if self._made is not None:
+            stream.wait_event(self._made)
+        for t in self._tensors:
+            t.record_stream(stream)
+        self._known.add(stream.cuda_stream)
+
+
 class ScoredDecodeAttention:
     """Decode attention that also accumulates, per cached token and kv head, the softmax weight the token received:
     ``scores[layer, s, h, t] = decay * scores[layer, s, h, t] + sum of the weights of the query heads that read kv head h``
@@ -477,6 +502,7 @@ class ScoredDecodeAttention:
         need = int(lib().tkv_scored_attn_scratch_bytes(n_seqs, n_q_heads, pool.n_kv_heads, head_dim, max_kv_len))
         self.scratch = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=q.device)
+        self._buffers = _Buffers(pool.device, self.out, self.scratch, self.status)
         self._pool_c = pool.c_struct()
         self._args = {}
         row = n_seqs * pool.n_kv_heads * scores.shape[3] * 4
@@ -490,6 +516,7 @@ class ScoredDecodeAttention:
         args = self._args.get(layer)
         if args is None:
             args = self._args[layer] = C.byref(self._mk(layer))
+        self._buffers.use(stream)
         check(lib().tkv_scored_attn_enqueue(C.byref(self._pool_c), args, C.c_void_p(stream.cuda_stream)))
         return self.out
 
@@ -518,6 +545,7 @@ class PrefixAttention:
         need = int(lib().tkv_prefix_attn_scratch_bytes(n_seqs, n_groups, n_q_heads, pool.n_kv_heads, head_dim, max_kv_len, max_prefix_len))
         self.scratch = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=q.device)
+        self._buffers = _Buffers(pool.device, self.out, self.scratch, self.status)
         self._pool_c = pool.c_struct()
         self._args = {}
         self._mk = lambda layer: N.TkvPrefixAttn(n_seqs, n_groups, n_q_heads, tables.shape[1], layer, max_kv_len, max_prefix_len, self.sm_scale,
@@ -530,6 +558,7 @@ class PrefixAttention:
         args = self._args.get(layer)
         if args is None:
             args = self._args[layer] = C.byref(self._mk(layer))
+        self._buffers.use(stream)
         check(lib().tkv_prefix_attn_enqueue(C.byref(self._pool_c), args, C.c_void_p(stream.cuda_stream)))
         return self.out
 
@@ -553,6 +582,7 @@ class CacheEviction:
         assert scores.is_cuda and scores.dtype == torch.float32 and scores.is_contiguous() and scores.dim() == 4
         n_layers, n_seqs, n_kv_heads, stride = scores.shape
         dev = scores.device
+        made = [x is None for x in (kept, new_lens)]
         if kept is None:
             kept = torch.zeros((n_layers, n_seqs, n_kv_heads, min(stride, max(budget, recent))), dtype=torch.int32, device=dev)
         if new_lens is None:
@@ -566,6 +596,7 @@ class CacheEviction:
         self.kept, self.new_lens = kept, new_lens
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         self._device = dev.index
+        self._buffers = _Buffers(dev.index, self.status, *(x for x, own in zip((kept, new_lens), made) if own))
         self._select = N.TkvEvictSelect(dev.index, n_layers, n_seqs, n_kv_heads, stride, stride, kept.shape[3], budget, recent, 0, scores.data_ptr(),
                                         kv_lens.data_ptr(), protect.data_ptr() if protect is not None else 0, kept.data_ptr(), new_lens.data_ptr(),
                                         self.status.data_ptr())
@@ -576,7 +607,9 @@ class CacheEviction:
                                               kv_lens.data_ptr(), kept.data_ptr(), new_lens.data_ptr(), scores.data_ptr(), self.status.data_ptr())
 
     def _stream(self, stream):
-        return C.c_void_p((stream or torch.cuda.current_stream(self._device)).cuda_stream)
+        stream = stream or torch.cuda.current_stream(self._device)
+        self._buffers.use(stream)
+        return C.c_void_p(stream.cuda_stream)
 
     def select(self, stream: Optional[torch.cuda.Stream] = None):
         """Fills and returns ``(kept, new_lens)``."""

@@ -1,5 +1,7 @@
-"""Calls of the cache operators that their documentation allows and that are easy to get wrong."""
+"""Calls of the cache operators that their documentation allows and that are easy to get wrong: handles used on another stream than they were made on,
+a call after one that failed."""
 import ctypes
+import gc
 
 import pytest
 
@@ -30,6 +32,57 @@ def batch(H, lens, kv_heads=2, head_dim=64, dtype="f16", seed=0, layers=1):
     tables = torch.arange(len(lens) * width, dtype=torch.int32).view(len(lens), width).cuda()
     q = torch.randn((len(lens), kv_heads * 2, head_dim), generator=g).to(torch.float16).cuda()
     return pool, tables, q, torch.tensor(lens, dtype=torch.int32).cuda()
+
+
+def test_handles_used_at_once_on_another_stream_than_they_were_made_on(H):
+    """The stream on which a handle is made is busy; the call goes to another one, whose order with the caller's tensors is the caller's business but
+    which cannot know of the handle's own buffers.  A first round loads the kernels and fills the allocator, so that nothing else waits."""
+    import torch
+    pool, tables, q, lens = batch(H, [60, 200, 33])
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+    starts, prefixes = i32([0, 3]), i32([32])
+    scores, into = torch.rand((1, 3, 2, 208), generator=torch.Generator().manual_seed(1)).cuda(), torch.zeros((1, 3, 2, 208)).cuda()
+    bad = tables.clone()
+    bad[:, 1] = 1 << 24
+    side = torch.cuda.Stream()
+    for busy in (False, True):
+        torch.cuda.synchronize()
+        if busy:
+            torch.cuda._sleep(400_000_000)                             # some 0.2 s
+        ev = H.CacheEviction(None, None, lens, scores, 40, 8)
+        ev.select(side)
+        handles = [H.ScoredDecodeAttention(pool, q, bad, lens, into, 200), H.PrefixAttention(pool, q, bad, lens, starts, prefixes, 200, 32)]
+        for h in handles:
+            h.enqueue(0, side)
+        torch.cuda.synchronize()
+        kept, new, told = ev.kept.clone(), ev.new_lens.clone(), [int(h.status.item()) for h in handles]
+        if not busy:
+            want = kept, new
+        del ev, handles, h
+    assert torch.equal(kept, want[0]) and torch.equal(new, want[1]) and new.tolist() == [40, 40, 33]
+    assert told == [N.ERR_INVALID_CONFIG] * 2                          # what the kernels reported is still there
+
+
+def test_a_handle_dropped_while_its_call_runs_on_another_stream_keeps_its_workspace(H):
+    import torch
+    pool, tables, q, lens = batch(H, [60, 200, 33])
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+    starts, prefixes = i32([0, 3]), i32([32])
+    side = torch.cuda.Stream()
+    first = H.PrefixAttention(pool, q, tables, lens, starts, prefixes, 200, 32)
+    want, size = first.enqueue(0).clone(), first.scratch.numel()
+    h = H.PrefixAttention(pool, q, tables, lens, starts, prefixes, 200, 32)
+    h.enqueue(0, side)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)
+    out, at = h.enqueue(0, side), h.scratch.data_ptr()
+    del h
+    gc.collect()                                                       # (a handle refers to itself)
+    again = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(100)]   # the allocator must not hand out what the call still uses
+    assert all(x.data_ptr() >= at + size or x.data_ptr() + size <= at for x in again)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
 
 
 def test_a_call_that_fails_on_its_device_spoils_nothing_after_it(H):
