@@ -447,8 +447,8 @@ int32_t tkv_scored_attn_enqueue(const TkvPool* pool, const TkvScoredAttn* args, 
  * tokens behind them as in tkv_decode_attn_enqueue.  Sequences group_starts[g] .. group_starts[g + 1] - 1 are group g; their first
  * prefix_lens[g] tokens (whole blocks) are those that the table row of the group's FIRST sequence names.  The result is that of
  * attending every sequence to its own kv_lens[s] tokens; a sequence shorter than its group's prefix attends to as much of it.
- * Sequences outside [group_starts[0], group_starts[n_groups]) are not computed and their rows of out are left as they were (a padded
- * batch); a sequence of length 0 inside gets zeros.  No counterpart in the reference.  F16 or E4M3 pool (per-block scales applied),
+ * Sequences outside [group_starts[0], group_starts[n_groups]) are not computed, whatever their lengths and table rows hold, and their
+ * rows of out are left as they were (a padded batch); a sequence of length 0 inside gets zeros.  No counterpart in the reference.  F16 or E4M3 pool (per-block scales applied),
  * F16 q and out, 16-token blocks, head_dim 64 or 128, 1..8 query heads per kv head.  Lengths and groups are device memory read when the
  * kernels run.  Calls that share scratch have to be ordered, two graphs that were captured with the same scratch included.            */
 typedef struct TkvPrefixAttn {
@@ -466,7 +466,7 @@ typedef struct TkvPrefixAttn {
     uint64_t scratch_bytes;
     uint64_t status;              /* 0, or a device u32 (zero it before the launch): TKV_ERR_TIMEOUT if a bounded wait gave up,
                                      TKV_ERR_INVALID_CONFIG if the groups do not ascend, a prefix is no whole number of blocks or above
-                                     its bound (nothing is computed then), a length is above its bound (clamped) or a table entry
+                                     its bound (nothing is computed then), a member's length is above its bound (clamped) or a table entry
                                      names a block outside the pool (never read); out is then not valid            */
 } TkvPrefixAttn;
 uint64_t tkv_prefix_attn_scratch_bytes(uint32_t n_seqs, uint32_t n_groups, uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t head_dim,

@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(THREADS, 1) rows_attn(const Args a) {
             const uint2 r = own_range(a, s);
             if (s < SEQ_CACHE) seq_info[s] = r;
             mine += blocks_of(r);
-            if (blockIdx.x == 0 && a.kv_lens[s] > a.max_kv_len) report(a.status, 2u);
+            if (blockIdx.x == 0 && a.kv_lens[s] > a.max_kv_len && (!a.group_starts || group_of(a.group_starts, a.n_groups, s) < a.n_groups)) report(a.status, 2u);
         }
     }
     uint32_t incl = mine;

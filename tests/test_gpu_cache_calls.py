@@ -1,5 +1,5 @@
 """Calls of the cache operators that their documentation allows and that are easy to get wrong: handles used on another stream than they were made on,
-a call after one that failed."""
+padded batches, a call after one that failed."""
 import ctypes
 import gc
 
@@ -83,6 +83,23 @@ def test_a_handle_dropped_while_its_call_runs_on_another_stream_keeps_its_worksp
     assert all(x.data_ptr() >= at + size or x.data_ptr() + size <= at for x in again)
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+def test_lengths_of_rows_outside_the_groups_are_nobodys_business(H):
+    """A padded batch: what stands in kv_lens (and the tables) behind the last group, and before the first, is not looked at."""
+    import torch
+    pool, tables, q, lens = batch(H, [60, 200, 33, 40, 90])
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+    starts, prefixes = i32([1, 3]), i32([0])
+    attn = H.PrefixAttention(pool, q, tables, lens, starts, prefixes, 200, 16)
+    want = attn.enqueue(0).clone()
+    assert int(attn.status.item()) == 0
+    lens[0], lens[3], lens[4] = -1, 100000, -7
+    tables[3:] = -1
+    attn.out.fill_(7.5)
+    out = attn.enqueue(0)
+    assert int(attn.status.item()) == 0
+    assert torch.equal(out[1:3], want[1:3]) and (out[0] == 7.5).all() and (out[3:] == 7.5).all()
 
 
 def test_a_call_that_fails_on_its_device_spoils_nothing_after_it(H):
