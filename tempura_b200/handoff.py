@@ -580,6 +580,9 @@ class CacheEviction:
     def __init__(self, pool: Optional[Pool], tables: Optional[torch.Tensor], kv_lens: torch.Tensor, scores: torch.Tensor, budget: int, recent: int,
                  protect: Optional[torch.Tensor] = None, kept: Optional[torch.Tensor] = None, new_lens: Optional[torch.Tensor] = None):
         assert scores.is_cuda and scores.dtype == torch.float32 and scores.is_contiguous() and scores.dim() == 4
+        if budget < 0 or recent < 0:
+            raise TkvError(N.ERR_INVALID_CONFIG, f"budget and recent must not be negative ({budget}, {recent})")
+        budget, recent = min(budget, 0xFFFFFFFF), min(recent, 0xFFFFFFFF)    # what no sequence reaches cuts none
         n_layers, n_seqs, n_kv_heads, stride = scores.shape
         dev = scores.device
         made = [x is None for x in (kept, new_lens)]

@@ -1,7 +1,8 @@
 """Calls of the cache operators that their documentation allows and that are easy to get wrong: handles used on another stream than they were made on,
-padded batches, a call after one that failed."""
+padded batches, bounds without a limit, a call after one that failed."""
 import ctypes
 import gc
+import sys
 
 import pytest
 
@@ -100,6 +101,24 @@ def test_lengths_of_rows_outside_the_groups_are_nobodys_business(H):
     out = attn.enqueue(0)
     assert int(attn.status.item()) == 0
     assert torch.equal(out[1:3], want[1:3]) and (out[0] == 7.5).all() and (out[3:] == 7.5).all()
+
+
+@pytest.mark.parametrize("budget,recent", [(1 << 32, 4), (sys.maxsize, 0), (4, 1 << 32), (4, sys.maxsize)])
+def test_a_budget_without_a_limit_cuts_nothing(H, budget, recent):
+    import torch
+    scores = torch.rand((1, 2, 1, 64)).cuda()
+    ev = H.CacheEviction(None, None, torch.tensor([64, 50], dtype=torch.int32).cuda(), scores, budget, recent)
+    kept, new = ev.select()
+    assert int(ev.status.item()) == 0 and new.tolist() == [64, 50]
+    assert kept[0, 0, 0].tolist() == list(range(64))
+
+
+def test_negative_budgets_are_refused(H):
+    import torch
+    scores, lens = torch.rand((1, 1, 1, 64)).cuda(), torch.tensor([64], dtype=torch.int32).cuda()
+    for budget, recent in ((-1, 0), (8, -1)):
+        with pytest.raises(H.TkvError):
+            H.CacheEviction(None, None, lens, scores, budget, recent)
 
 
 def test_a_call_that_fails_on_its_device_spoils_nothing_after_it(H):
