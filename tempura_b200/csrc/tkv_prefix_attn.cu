@@ -348,14 +348,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         }
                     }
                 }
-                if (!ok) {
-                    if (lane == 0) atomicCAS(&c->fail, 0u, 4u);
-                    // no copy is in flight when the CTA's shared memory goes: the last two of each ring are waited for
-#pragma unroll
-                    for (int kv = 0; kv < 2; kv++)
-                        for (uint32_t t = issued[kv] > 2 ? issued[kv] - 2 : 0u; t < issued[kv]; t++)
-                            for (uint32_t n = 0; n < (1u << 20) && !mbar_test((kv ? c->v_full : c->k_full) + (t & 1u), (t >> 1) & 1u); n++) {}
-                }
+                if (!ok && lane == 0) atomicCAS(&c->fail, 0u, 4u);
             } else {
                 // ---- widening: 128 threads, 16 bytes of a token at a time.  The bytes arrive a tile ahead by asynchronous copies; a thread copies
                 // what it will widen, so its own wait is enough.  (In registers they did not fit beside the softmax's share of them.) ----
@@ -616,6 +609,12 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         const uint32_t cut = 2 - steps_in(it.n_tiles - 1);      // only a prefix's last tile may hold one half
         n_steps += 2 * it.n_tiles - cut;
         u += it.n_tiles;
+    }
+    if (!FP8 && warp == SM && *fail) {                          // whichever role gave up, no copy is in flight when the CTA's shared memory goes
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++)                          // the last two of each ring
+            for (uint32_t t = issued[kv] > 2 ? issued[kv] - 2 : 0u; t < issued[kv]; t++)
+                for (uint32_t n = 0; n < (1u << 20) && !mbar_test((kv ? c->v_full : c->k_full) + (t & 1u), (t >> 1) & 1u); n++) {}
     }
     if (warp >= SM + FEED && lane == 0) {                       // whatever ended the loop, no product is under way when tensor memory is given back
         uint64_t* bar = c->drained + (warp - (SM + FEED));

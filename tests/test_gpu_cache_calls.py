@@ -150,3 +150,23 @@ def test_a_call_that_fails_on_its_device_spoils_nothing_after_it(H):
         good()
     torch.cuda.synchronize()
     assert int(ev.status.item()) == int(scored.status.item()) == int(pre.status.item()) == 0
+
+
+@pytest.mark.parametrize("dtype", ["f16", "e4m3"])
+def test_a_foreign_block_deep_in_a_prefix_ends_the_call_and_leaves_the_next_one_alone(H, dtype):
+    """The producer meets the id with tiles before it on their way and under the tensor cores: the call reports it and returns, again and again."""
+    import torch
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+    pool, tables, q, lens = batch(H, [3200] * 4, kv_heads=4, head_dim=128, dtype=dtype, seed=5)
+    tables[:, :200] = tables[0, :200]
+    good = H.PrefixAttention(pool, q, tables, lens, i32([0, 4]), i32([3200]), 3200, 3200)
+    want = good.enqueue(0).clone()
+    for at in (0, 7, 8, 9, 23, 100, 199):
+        broken = tables.clone()
+        broken[0, at] = pool.total_blocks + at
+        bad = H.PrefixAttention(pool, q, broken, lens, i32([0, 4]), i32([3200]), 3200, 3200)
+        for _ in range(10):
+            bad.enqueue(0)
+            good.enqueue(0)
+        assert int(bad.status.item()) == N.ERR_INVALID_CONFIG
+        assert int(good.status.item()) == 0 and torch.equal(good.out, want)
