@@ -616,7 +616,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             for (uint32_t t = issued[kv] > 2 ? issued[kv] - 2 : 0u; t < issued[kv]; t++)
                 for (uint32_t n = 0; n < (1u << 20) && !mbar_test((kv ? c->v_full : c->k_full) + (t & 1u), (t >> 1) & 1u); n++) {}
     }
-    if (warp >= SM + FEED && lane == 0) {                       // whatever ended the loop, no product is under way when tensor memory is given back
+    if (warp >= SM + FEED && elect_one()) {                     // (the lane that issued) whatever ended the loop, no product is under way when tensor memory goes back
         uint64_t* bar = c->drained + (warp - (SM + FEED));
         tc_commit(bar);
         for (uint32_t i = 0; i < (1u << 22) && !mbar_test(bar, 0u); i++) {}
