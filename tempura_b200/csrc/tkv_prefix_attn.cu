@@ -835,7 +835,8 @@ int32_t tkv_prefix_attn_enqueue(const TkvPool* pool, const TkvPrefixAttn* p, voi
     if (pool->n_kv_heads > CTAS * tkv_rows::WARPS) return fail(TKV_ERR_INVALID_CONFIG, "at most %llu kv heads (%llu)", CTAS * tkv_rows::WARPS, pool->n_kv_heads);
     if ((pool->k_scales == 0) != (pool->v_scales == 0)) return fail(TKV_ERR_INVALID_CONFIG, "k_scales and v_scales must both be set or both be 0");
     if (pool->k_scales && pool->dtype != TKV_DTYPE_E4M3) return fail(TKV_ERR_INVALID_CONFIG, "only an E4M3 pool carries scales");
-    if (!std::isfinite(p->sm_scale)) return fail(TKV_ERR_INVALID_CONFIG, "sm_scale is not finite");
+    const float scale_log2 = p->sm_scale * 1.4426950408889634f;
+    if (!std::isfinite(scale_log2)) return fail(TKV_ERR_INVALID_CONFIG, "sm_scale x log2(e) is not finite");
     if (p->n_seqs == 0 || p->n_groups == 0) return TKV_OK;
     if (!p->q || !p->out || !p->tables || !p->kv_lens || !p->group_starts || !p->prefix_lens || !pool->k_layer_ptrs || !pool->v_layer_ptrs || !pool->total_blocks)
         return fail(TKV_ERR_INVALID_CONFIG, "NULL buffer");
@@ -860,7 +861,6 @@ int32_t tkv_prefix_attn_enqueue(const TkvPool* pool, const TkvPrefixAttn* p, voi
 
     const uint32_t es = fp8 ? 1u : 2u;
     const size_t layer_scales = (size_t)p->layer * pool->total_blocks * pool->n_kv_heads;
-    const float scale_log2 = p->sm_scale * 1.4426950408889634f;
     Args a{};
     a.tables = reinterpret_cast<const uint32_t*>(p->tables);
     a.kv_lens = reinterpret_cast<const uint32_t*>(p->kv_lens);

@@ -250,7 +250,8 @@ int32_t tkv_scored_attn_enqueue(const TkvPool* pool, const TkvScoredAttn* p, voi
     if (pool->n_kv_heads > CTAS * tkv_rows::WARPS) return fail(TKV_ERR_INVALID_CONFIG, "at most %llu kv heads (%llu)", CTAS * tkv_rows::WARPS, pool->n_kv_heads);
     if ((pool->k_scales == 0) != (pool->v_scales == 0)) return fail(TKV_ERR_INVALID_CONFIG, "k_scales and v_scales must both be set or both be 0");
     if (pool->k_scales && pool->dtype != TKV_DTYPE_E4M3) return fail(TKV_ERR_INVALID_CONFIG, "only an E4M3 pool carries scales");
-    if (!std::isfinite(p->sm_scale)) return fail(TKV_ERR_INVALID_CONFIG, "sm_scale is not finite");
+    const float scale_log2 = p->sm_scale * 1.4426950408889634f;
+    if (!std::isfinite(scale_log2)) return fail(TKV_ERR_INVALID_CONFIG, "sm_scale x log2(e) is not finite");
     if (!(p->decay >= 0.0f && p->decay <= 1.0f)) return fail(TKV_ERR_INVALID_CONFIG, "decay must lie in [0, 1]");
     if (p->n_seqs == 0) return TKV_OK;
     if (!p->q || !p->out || !p->tables || !p->kv_lens || !p->scores || !pool->k_layer_ptrs || !pool->v_layer_ptrs || !pool->total_blocks)
@@ -302,7 +303,7 @@ int32_t tkv_scored_attn_enqueue(const TkvPool* pool, const TkvScoredAttn* p, voi
     a.max_kv_len = p->max_kv_len;
     a.total_blocks = pool->total_blocks;
     a.logit_stride = l.logit_stride;
-    a.scale_log2 = p->sm_scale * 1.4426950408889634f;
+    a.scale_log2 = scale_log2;
     FinishArgs f{};
     f.part_o = a.part_o;
     f.part_ml = a.part_ml;

@@ -151,3 +151,9 @@ def test_select_takes_neighbouring_buffers(L):
     """Side by side in one allocation is no overlap: the call goes on to the device (or, without one, to its error)."""
     for change in ({"protect": A + 4096 + 8}, {"protect": A + 4096 - 8}, {"kv_lens": A + 4096 + 8}, {"kv_lens": A + 4096 - 8}):
         assert L.tkv_evict_select_enqueue(C.byref(select(device=1 << 20, new_lens=A + 4096, **change)), None) == N.ERR_CUDA
+
+
+@pytest.mark.parametrize("scale", [3e38, -3e38])
+def test_attention_refuses_a_scale_that_is_infinite_in_the_log2_domain(L, scale):
+    assert L.tkv_scored_attn_enqueue(C.byref(pool()), C.byref(scored(sm_scale=scale)), None) == BAD
+    assert L.tkv_prefix_attn_enqueue(C.byref(pool()), C.byref(prefix(sm_scale=scale)), None) == BAD
