@@ -214,7 +214,7 @@ struct Layout {
 Layout layout_of(uint32_t n_seqs, uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t max_kv_len) {
     Layout l;
     l.split = tkv_rows::split_for((uint64_t)n_seqs * ((max_kv_len + 15ull) / 16), n_kv_heads, CTAS);
-    const uint64_t slots = ((uint64_t)l.split.parts + n_seqs) * 2;          // an E4M3 pool's slots hold two partial results
+    const uint64_t slots = (uint64_t)l.split.parts + n_seqs;                // part p and sequence s meet in slot p + s
     l.logit_stride = (uint32_t)up(max_kv_len, 16);
     l.ml = up(4ull * (n_seqs + 2ull), 256);
     l.o = l.ml + up(slots * n_q_heads * 8ull, 256);

@@ -157,3 +157,12 @@ def test_select_takes_neighbouring_buffers(L):
 def test_attention_refuses_a_scale_that_is_infinite_in_the_log2_domain(L, scale):
     assert L.tkv_scored_attn_enqueue(C.byref(pool()), C.byref(scored(sm_scale=scale)), None) == BAD
     assert L.tkv_prefix_attn_enqueue(C.byref(pool()), C.byref(prefix(sm_scale=scale)), None) == BAD
+
+
+@pytest.mark.parametrize("n_seqs,n_q_heads,n_kv_heads,head_dim,max_kv_len", [(64, 32, 8, 128, 4096), (1, 64, 8, 128, 131071), (3, 8, 1, 64, 100), (16, 32, 16, 128, 1)])
+def test_the_scored_workspace_holds_one_partial_result_per_part_and_sequence(L, n_seqs, n_q_heads, n_kv_heads, head_dim, max_kv_len):
+    """Scores of whole blocks, and (m, l, O) of at most 148 x 8 / min(kv heads, 8) parts and n_seqs sequences; the rest is a few words and alignment."""
+    parts = 148 * 8 // min(n_kv_heads, 8) // -(-n_kv_heads // 8)
+    scores = n_seqs * n_q_heads * -(-max_kv_len // 16) * 16 * 4
+    got = L.tkv_scored_attn_scratch_bytes(n_seqs, n_q_heads, n_kv_heads, head_dim, max_kv_len)
+    assert scores + n_seqs * n_q_heads * (head_dim + 2) * 4 < got <= scores + (parts + n_seqs) * n_q_heads * (head_dim + 2) * 4 + 4 * (n_seqs + 2) + 3 * 256
