@@ -435,9 +435,9 @@ typedef struct TkvScoredAttn {
     uint64_t scores;              /* f32 [n_seqs][n_kv_heads][score_stride] of this layer                          */
     uint64_t scratch;             /* tkv_scored_attn_scratch_bytes(...) bytes of device memory, 256-byte aligned   */
     uint64_t scratch_bytes;
-    uint64_t status;              /* 0, or a device u32 (zero it before the launch): TKV_ERR_INVALID_CONFIG if kv_lens held a value
-                                     above max_kv_len (clamped to it) or a table entry named a block outside the pool (never read);
-                                     out and scores are then not valid                                             */
+    uint64_t status;              /* 0, or a device u32 (zero it before the launch): TKV_ERR_TIMEOUT if a bounded wait gave up,
+                                     TKV_ERR_INVALID_CONFIG if kv_lens held a value above max_kv_len (clamped to it) or a table entry
+                                     named a block outside the pool (never read); out and scores are then not valid */
 } TkvScoredAttn;
 uint64_t tkv_scored_attn_scratch_bytes(uint32_t n_seqs, uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t max_kv_len);
 int32_t tkv_scored_attn_enqueue(const TkvPool* pool, const TkvScoredAttn* args, void* stream);

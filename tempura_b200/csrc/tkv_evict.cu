@@ -478,7 +478,7 @@ int32_t tkv_evict_select_enqueue(const TkvEvictSelect* p, void* stream) {
     if (e == cudaSuccess && prev != p->device) e = cudaSetDevice(p->device);
     if (e == cudaSuccess) {
         const size_t smem = a.staged ? (size_t)slice * 4 : 0;
-        // 256 threads take rows eight to an SM, 512 a row faster: 512 x 6 000 tokens 23 us and 27, but 64 x 8 192 20 us and 14, 512 x 16 384 92 and 46
+        // 256 threads take rows six to an SM (40 registers, one value spilled), 512 a row faster: 512 x 6 000 tokens 23 us and 27, but 64 x 8 192 20 us and 14, 512 x 16 384 92 and 46
         const bool large = slice > 8192 || (rows <= 296 && slice > 1024);
         auto kernel = large ? evict_select<512> : evict_select<256>;
         if (smem > 32 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(STAGE_TOKENS * 4));

@@ -632,7 +632,7 @@ prefix_attn_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
 // ---- joining ----------------------------------------------------------------------------------------------------------------------
 struct JoinArgs {
     const float *pre_o, *pre_ml, *own_o, *own_ml;   // partial results over the prefixes, over the tokens behind them
-    const uint32_t *pre_plan, *own_plan, *kv_lens, *group_starts, *prefix_lens;
+    const uint32_t *pre_plan, *own_plan, *group_starts, *prefix_lens;
     __half* out;
     uint32_t n_seqs, n_groups, n_q_heads, n_kv_heads, group;
 };
@@ -924,7 +924,6 @@ int32_t tkv_prefix_attn_enqueue(const TkvPool* pool, const TkvPrefixAttn* p, voi
     j.own_ml = r.part_ml;
     j.pre_plan = a.plan;
     j.own_plan = r.plan;
-    j.kv_lens = a.kv_lens;
     j.group_starts = a.group_starts;
     j.prefix_lens = a.prefix_lens;
     j.out = reinterpret_cast<__half*>(p->out);

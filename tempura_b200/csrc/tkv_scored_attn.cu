@@ -43,7 +43,7 @@ __host__ __device__ constexpr int tokens_of(int g) { return g > 4 ? 2 : 4; }
 
 // One CTA per (sequence, kv head, task): the first G tasks join the partial results of one query head each, the others turn the scores of 256 x TOK tokens into weights.  Bound by latency and L2:
 // everything it reads was written just before, so a thread asks for its scores before it joins the maxima and sums, and asks
-// for all of those at once.  V: rows of scores are aligned to a thread's tokens.
+// for all of those at once.  v4: rows of accumulated weights are aligned to 16 bytes, so that a thread stores its tokens together.
 template <int D, bool F32, int G> __global__ void __launch_bounds__(256) scored_finish(const FinishArgs a) {
     constexpr int TOK = tokens_of(G);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
