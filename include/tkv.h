@@ -501,8 +501,8 @@ int32_t tkv_evict_select_enqueue(const TkvEvictSelect* args, void* stream);
 /* Compact: row j of every (layer, sequence, kv head) becomes the row that kept[j] names, for K, V and (if given) scores, in place
  * through the block tables; scores from new_lens[s] to kv_lens[s] become 0.  Sequences with new_lens[s] == kv_lens[s] and rows with
  * kept[j] == j are not touched.  Afterwards the caller makes new_lens the lengths and may return the blocks behind them
- * (tkv_device_page_allocator_free with first = ceil(new_lens / 16), seq_lens = the old lengths).  A block that other
- * sequences use as well has to lie below protect[s] at selection.  An E4M3 pool with scales: a block's scale becomes the largest of
+ * (tkv_device_page_allocator_free with first = ceil(new_lens / 16), seq_lens = the old lengths).  A block that other sequences
+ * use as well, or that a prefix index still names (a later prompt would find other tokens there), has to lie below protect[s] at selection.  An E4M3 pool with scales: a block's scale becomes the largest of
  * its new rows' scales; rows that had another one are rounded to E4M3 again at the new scale.  F16 or E4M3 pool, 16-token
  * blocks, head_dim 64 or 128.                                                                                       */
 typedef struct TkvEvictCompact {

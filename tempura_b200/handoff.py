@@ -572,8 +572,8 @@ class CacheEviction:
     ``DevicePageAllocator.free(tables, first=ceil(new_lens / 16), seq_lens=old_lens)``.
 
     ``scores`` is f32 ``[n_layers, n_seqs, n_kv_heads, score_stride]``, ``kv_lens`` int32 ``[n_seqs]`` (at most ``score_stride``),
-    ``tables`` int32 ``[n_seqs, table_stride]``, ``protect`` int32 ``[n_seqs]`` or None.  A prefix that other sequences share has to
-    be protected.  ``kept`` int32 ``[n_layers, n_seqs, n_kv_heads, n]`` and ``new_lens`` are made here unless given; a sequence whose
+    ``tables`` int32 ``[n_seqs, table_stride]``, ``protect`` int32 ``[n_seqs]`` or None.  A prefix that other sequences share, or
+    that a :class:`PrefixIndex` still names, has to be protected.  ``kept`` int32 ``[n_layers, n_seqs, n_kv_heads, n]`` and ``new_lens`` are made here unless given; a sequence whose
     protected and recent tokens exceed both ``budget`` and ``n`` is not cut and sets ``status``.  ``pool`` and ``tables`` may be None
     for ``select`` alone."""
 
