@@ -464,7 +464,8 @@ class _Buffers:
     def __init__(self, device: int, *tensors: torch.Tensor):
         home = torch.cuda.current_stream(device)
         self._tensors, self._known = tensors, {home.cuda_stream}
-        self._made = None if self._capturing(home) else home.record_event()
+        capturing = torch.cuda.is_current_stream_capturing() if torch.cuda.current_device() == device else self._capturing(home)
+        self._made = None if capturing else home.record_event()
 
     @staticmethod
     def _capturing(stream: torch.cuda.Stream) -> bool:
