@@ -448,9 +448,10 @@ int32_t tkv_scored_attn_enqueue(const TkvPool* pool, const TkvScoredAttn* args, 
  * prefix_lens[g] tokens (whole blocks) are those that the table row of the group's FIRST sequence names.  The result is that of
  * attending every sequence to its own kv_lens[s] tokens; a sequence shorter than its group's prefix attends to as much of it.
  * Sequences outside [group_starts[0], group_starts[n_groups]) are not computed, whatever their lengths and table rows hold, and their
- * rows of out are left as they were (a padded batch); a sequence of length 0 inside gets zeros.  No counterpart in the reference.  F16 or E4M3 pool (per-block scales applied),
- * F16 q and out, 16-token blocks, head_dim 64 or 128, 1..8 query heads per kv head.  Lengths and groups are device memory read when the
- * kernels run.  Calls that share scratch have to be ordered, two graphs that were captured with the same scratch included.            */
+ * rows of out are left as they were (a padded batch); a sequence of length 0 inside gets zeros.  No counterpart in the reference.
+ * F16 or E4M3 pool (per-block scales applied, none negative), F16 q and out, 16-token blocks, head_dim 64 or 128, 1..8 query heads
+ * per kv head.  Lengths and groups are device memory read when the kernels run.  Calls that share scratch have to be ordered, two
+ * graphs that were captured with the same scratch included.                                                                     */
 typedef struct TkvPrefixAttn {
     uint32_t n_seqs, n_groups, n_q_heads, table_stride, layer;
     uint32_t max_kv_len;          /* bounds kv_lens                                                                */
@@ -499,12 +500,13 @@ typedef struct TkvEvictSelect {
 } TkvEvictSelect;
 int32_t tkv_evict_select_enqueue(const TkvEvictSelect* args, void* stream);
 /* Compact: row j of every (layer, sequence, kv head) becomes the row that kept[j] names, for K, V and (if given) scores, in place
- * through the block tables; scores from new_lens[s] to kv_lens[s] become 0.  Sequences with new_lens[s] == kv_lens[s] and rows with
- * kept[j] == j are not touched.  Afterwards the caller makes new_lens the lengths and may return the blocks behind them
- * (tkv_device_page_allocator_free with first = ceil(new_lens / 16), seq_lens = the old lengths).  A block that other sequences
- * use as well, or that a prefix index still names (a later prompt would find other tokens there), has to lie below protect[s] at selection.  An E4M3 pool with scales: a block's scale becomes the largest of
- * its new rows' scales; rows that had another one are rounded to E4M3 again at the new scale.  F16 or E4M3 pool, 16-token
- * blocks, head_dim 64 or 128.                                                                                       */
+ * through the block tables; scores from new_lens[s] to kv_lens[s] become 0.  Sequences with new_lens[s] == kv_lens[s], and blocks of
+ * which every row has kept[j] == j, are not touched.  Afterwards the caller makes new_lens the lengths and may return the blocks
+ * behind them (tkv_device_page_allocator_free with first = ceil(new_lens / 16), seq_lens = the old lengths).  A block that other
+ * sequences use as well, or that a prefix index still names (a later prompt would find other tokens there), has to lie below
+ * protect[s] at selection.  An E4M3 pool with scales: the scale of a block into which a row moves becomes the largest of its new
+ * rows' scales; rows of it that had another one, those with kept[j] == j among them, are rounded to E4M3 again at the new scale.
+ * F16 or E4M3 pool, 16-token blocks, head_dim 64 or 128.                                                            */
 typedef struct TkvEvictCompact {
     uint32_t layer_begin, n_layers, n_seqs, table_stride, max_kv_len, score_stride, kept_stride, reserved;
     uint64_t tables;              /* u32 [n_seqs][table_stride] block ids                                           */

@@ -28,8 +28,8 @@
 // chain is shorter than the time in which HBM delivers the block (131 071 tokens of 8 heads: 92 us, 5.9 TB/s).  An E4M3 block has half the bytes
 // and a conversion in the chain: 64 sequences of up to 4 096 tokens take 54 us (4.9 TB/s), one context of 131 071 the same, of which delivery alone
 // is 46 to 47 (consumers that only hand their stages back; 5.8 TB/s, the rate of F16 blocks) and 7 to 8 the arithmetic that the ring does not
-// hide.  The scales are not it (53 us without).  Two consumers per head on alternate blocks did not help: the same 71 us for the whole call, and 91 against 75 us for one context
-// of 131 071 tokens.
+// hide.  The scales are not it (53 us without).  Two consumers per head on alternate blocks did not help: the same 71 us for the whole call, and
+// 91 against 75 us for one context of 131 071 tokens.
 //
 // Work split: the batch's blocks, sequence after sequence, are cut into `parts` equal shares that may span sequences; part p and
 // sequence s meet in partial slot p + s, which is unique because both only grow along the batch.
